@@ -14,6 +14,7 @@ LIB_PATH = os.environ.get("GRWS_LIB_PATH") or os.path.join(_CSRC, "libgrws_b200.
 c_i64, c_i32, c_sz, c_vp = ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p
 
 F32, F16, BF16 = 0, 1, 2
+REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
 ALGO_AUTO, ALGO_WARP_MMA, ALGO_TCGEN05 = 0, 1, 2
 
 # name -> (restype, argtypes); must list every function include/grws_b200.h declares
@@ -31,6 +32,16 @@ SIGNATURES = {
     "grws_layer_norm_scratch_bytes": (c_sz, [c_i64]),
     "grws_layer_norm_fwd": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, ctypes.c_float, c_vp]),
     "grws_layer_norm_bwd": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_vp, c_sz, c_vp]),
+    "grws_linear_ce_scratch_bytes": (c_sz, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i64, c_i64, c_i32, c_i32]),
+    "grws_linear_ce_fwd": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32,
+                                   c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
+    "grws_linear_ce_bwd": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32,
+                                   c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
+    "grws_distill_scratch_bytes": (c_sz, [c_i64, c_i64]),
+    "grws_distill_fwd": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_i64, c_i32, c_vp, c_i64, c_i32, c_i64, c_i64, c_i64,
+                                 ctypes.c_float, c_i32, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
+    "grws_distill_bwd": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_i64, c_i32, c_vp, c_i64, c_i32, c_i64, c_i64, c_i64,
+                                 ctypes.c_float, c_i32, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
     "grws_spmm_plan_bytes": (c_sz, [c_i64, c_i64, c_i64, c_i64]),
     "grws_spmm_plan_build": (c_i32, [c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_sz, c_vp]),
     "grws_spmm_fwd_planned": (c_i32, [c_vp, c_vp, c_vp, c_i32, c_vp, c_i32, c_i64, c_vp, c_i32, c_i64,

@@ -1,0 +1,145 @@
+// What the losses over the class axis share (linear_ce.cu, distill.cu): element types in 16-byte pieces, running softmax
+// statistics, the reduction of row losses and the factor a row's gradient gets from the loss's.
+#pragma once
+
+#include "grws_common.cuh"
+
+namespace grws {
+namespace cls {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr float NEG_INF = -INFINITY;
+
+enum Reduction : int { RED_NONE = GRWS_REDUCE_NONE, RED_MEAN = GRWS_REDUCE_MEAN, RED_SUM = GRWS_REDUCE_SUM };
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// 16 bytes of a row as fp32 values and back
+template <typename T> struct Piece;
+template <> struct Piece<float> {
+    static constexpr int E = 4;
+    static __device__ __forceinline__ void unpack(const uint4 &u, float (&v)[4]) {
+        v[0] = __uint_as_float(u.x); v[1] = __uint_as_float(u.y); v[2] = __uint_as_float(u.z); v[3] = __uint_as_float(u.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&v)[4]) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+};
+template <> struct Piece<__half> {
+    static constexpr int E = 8;
+    static __device__ __forceinline__ void unpack(const uint4 &u, float (&v)[8]) {
+        const __half2 *h = reinterpret_cast<const __half2 *>(&u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { const float2 f = __half22float2(h[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&v)[8]) {
+        uint4 u;
+        __half2 *h = reinterpret_cast<__half2 *>(&u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        return u;
+    }
+};
+template <> struct Piece<__nv_bfloat16> {
+    static constexpr int E = 8;
+    static __device__ __forceinline__ void unpack(const uint4 &u, float (&v)[8]) {
+        const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { const float2 f = __bfloat1622float2(h[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&v)[8]) {
+        uint4 u;
+        __nv_bfloat162 *h = reinterpret_cast<__nv_bfloat162 *>(&u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        return u;
+    }
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Running maximum m and sum s = sum exp(scale * (x - m)) of a part of a row, scale * ln 2 in `c`.  A part without entries,
+// or of entries that are all -inf, is (-inf, 0); subtracting 0 instead of -inf keeps its exponentials at 0.
+__device__ __forceinline__ float finite_or_zero(float m) { return m == NEG_INF ? 0.0f : m; }
+
+__device__ __forceinline__ void join_stats(float &m, float &s, float m2, float s2, float c) {
+    const float top = fmaxf(m, m2), safe = finite_or_zero(top);
+    s = s * exp2_approx((m - safe) * c) + s2 * exp2_approx((m2 - safe) * c);
+    m = top;
+}
+
+template <int N> __device__ __forceinline__ void add_values(float &m, float &s, const float (&v)[N], float c) {
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, v[i]);
+    const float safe = finite_or_zero(top);
+    if (top != m) { s *= exp2_approx((m - safe) * c); m = top; }
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t += exp2_approx((v[i] - safe) * c);
+    s += t;
+}
+
+// The integer at i of an array of 4- or 8-byte integers
+__device__ __forceinline__ int64_t load_index(const void *p, int bytes, int64_t i) {
+    return bytes == 8 ? __ldg(static_cast<const long long *>(p) + i) : (int64_t)__ldg(static_cast<const int *>(p) + i);
+}
+
+// Sum of two values over the block's threads, valid in thread 0; red holds 2 * 32 floats.
+__device__ __forceinline__ void block_sum2(float &a, float &b, float *red) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
+    if (lane == 0) { red[warp] = a; red[32 + warp] = b; }
+    __syncthreads();
+    if (warp == 0) {
+        a = lane < warps ? red[lane] : 0.0f;
+        b = lane < warps ? red[32 + lane] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
+    }
+    __syncthreads();
+}
+
+// loss = sum (or mean over the counted rows) of the blocks' partial sums [blocks][2] = (loss, counted rows), added in a fixed order
+__device__ __forceinline__ void finish_loss(float sum, float count, int reduction, float *loss, float *count_out) {
+    *loss = reduction == RED_MEAN ? sum / count : sum;       // no counted row: 0 / 0
+    *count_out = count;
+}
+static __global__ void __launch_bounds__(512) loss_sum_kernel(const float2 *__restrict__ partial, int n, int reduction,
+                                                              float *__restrict__ loss, float *__restrict__ count_out) {
+    __shared__ float red[64];
+    float a = 0.0f, b = 0.0f;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) { const float2 p = partial[i]; a += p.x; b += p.y; }
+    block_sum2(a, b, red);
+    if (threadIdx.x == 0) finish_loss(a, b, reduction, loss, count_out);
+}
+
+// Factor of all rows from the gradient of the reduced loss.  Without counted rows nothing has a gradient.
+__device__ __forceinline__ float loss_factor(const float *grad_loss, const float *count, int reduction) {
+    const float g = __ldg(grad_loss);
+    if (reduction != RED_MEAN) return g;
+    const float n = __ldg(count);
+    return n > 0.0f ? g / n : 0.0f;
+}
+
+inline int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
+        sms = 148;
+    return sms;
+}
+
+}  // namespace cls
+}  // namespace grws

@@ -1,0 +1,508 @@
+// Distillation from a teacher's best scores.  A row of student scores z [V] is compared with K kept teacher scores t and their
+// class ids at temperature T:
+//
+//     p_j = softmax_j(t_j / T) over the row's entries (id >= 0),   log q_v = z_v / T - log sum_v exp(z_v / T)
+//     loss = T^2 sum_j p_j (log p_j - log q_id(j)),                dz_v = g T (q_v - sum of p_j with id(j) = v)
+//
+// Forward is one pass over z with a running maximum and sum, backward one pass that reads z and writes dz: both are bound by
+// memory.  A row's state (maximum and sum of z, of t) goes from one to the other as four floats.  The maximum is kept apart
+// from the sum because z - max is exact where q is large, z / T - log sum would round at the size of z.
+//
+// Rows are walked in 16-byte pieces from the first aligned address on; what is before and behind them is read and written
+// element by element, so that rows of any length, stride and offset work and nothing outside of a row is touched.
+#include "class_loss.cuh"
+
+namespace grws {
+namespace distill {
+
+using namespace cls;
+
+constexpr int MAX_KEPT = 1024;
+constexpr int THREADS = 256;
+constexpr int CTAS_PER_SM = 8;
+constexpr int SHORT_ROW = 1024;          // classes up to which a group of lanes takes a row (else a CTA)
+constexpr int SHORT_KEPT = 64;           // entries that such a group holds in shared memory
+constexpr int SPLIT_MIN = 4096;          // classes below which a row is not cut any further
+
+struct Args {
+    const void *z; int64_t ldz;
+    const void *t; int64_t ldt; int t_dtype;
+    const void *ids; int64_t ldi; int id_bytes;
+    int64_t n, V; int K;
+    float c;                             // log2(e) / T
+    float T;
+    int reduction;
+    float *loss;                         // forward: [n] (no reduction)
+    float4 *state;                       // [n]: max z, sum exp((z - max) / T), max t, sum exp((t - max) / T); sum of t 0: no entry
+    float2 *partial;                     // [grid] sums of (loss, counted rows)
+    float2 *stats;                       // [splits][n] of rows cut into parts
+    int splits; int64_t part;            // parts of a row and their length
+    const float *grad, *count;           // backward
+    void *dz; int64_t ldo;
+};
+
+__device__ __forceinline__ float teacher_at(const Args &a, int64_t row, int j) {
+    const int64_t i = row * a.ldt + j;
+    if (a.t_dtype == GRWS_F32) return __ldg(static_cast<const float *>(a.t) + i);
+    if (a.t_dtype == GRWS_F16) return to_float(static_cast<const __half *>(a.t)[i]);
+    return to_float(static_cast<const __nv_bfloat16 *>(a.t)[i]);
+}
+__device__ __forceinline__ int64_t id_at(const Args &a, int64_t row, int j) { return load_index(a.ids, a.id_bytes, row * a.ldi + j); }
+
+template <int L> __device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o, L));
+    return v;
+}
+template <int L> __device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o, L);
+    return v;
+}
+
+// The part [lo, hi) of a row that starts at p: elements before the first aligned address, whole pieces, the rest
+template <typename T> struct Span {
+    const T *p;
+    int64_t pieces;
+    int head, tail;
+    __device__ __forceinline__ Span(const T *row, int64_t lo, int64_t hi) {
+        constexpr int E = Piece<T>::E;
+        p = row + lo;
+        const int64_t len = hi - lo;
+        const int off = (int)((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
+        head = (int)min((int64_t)((E - off) & (E - 1)), len);
+        pieces = (len - head) / E;
+        tail = (int)(len - head - pieces * E);
+    }
+    __device__ __forceinline__ const uint4 *body() const { return reinterpret_cast<const uint4 *>(p + head); }
+    __device__ __forceinline__ const T *rest() const { return p + head + pieces * Piece<T>::E; }
+};
+
+// running statistics of a span by `lanes` threads
+template <typename T, int UNROLL> __device__ __forceinline__ void span_stats(const Span<T> &sp, int lane, int lanes, float c, float &m, float &s) {
+    constexpr int E = Piece<T>::E;
+    for (int i = lane; i < sp.head + sp.tail; i += lanes) {
+        const float v[1] = {to_float(i < sp.head ? sp.p[i] : sp.rest()[i - sp.head])};
+        add_values<1>(m, s, v, c);
+    }
+    const uint4 *b = sp.body();
+    int64_t k = lane;
+    for (; k + (int64_t)(UNROLL - 1) * lanes < sp.pieces; k += (int64_t)UNROLL * lanes) {
+        uint4 u[UNROLL];
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) u[i] = __ldg(b + k + (int64_t)i * lanes);
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) {
+            float v[E];
+            Piece<T>::unpack(u[i], v);
+            add_values<E>(m, s, v, c);
+        }
+    }
+    for (; k < sp.pieces; k += lanes) {
+        float v[E];
+        Piece<T>::unpack(__ldg(b + k), v);
+        add_values<E>(m, s, v, c);
+    }
+}
+
+// The row's loss from its statistics, by L lanes that hold the same (m, s); writes the state, returns the loss in every lane.
+template <typename T, int L> __device__ __forceinline__ float row_loss(const Args &a, int64_t row, int lane, bool active, float m, float s, float &counted) {
+    const T *z = static_cast<const T *>(a.z) + row * a.ldz;
+    float tm = NEG_INF;
+    bool any = false, bad = false;
+    if (active)
+        for (int j = lane; j < a.K; j += L) {
+            const int64_t id = id_at(a, row, j);
+            if (id < 0) continue;
+            const float t = teacher_at(a, row, j);
+            any |= t != NEG_INF;
+            bad |= id >= a.V;
+            tm = fmaxf(tm, t);
+        }
+    tm = group_max<L>(tm);
+    any = group_max<L>(any ? 1.0f : 0.0f) > 0.0f;
+    bad = group_max<L>(bad ? 1.0f : 0.0f) > 0.0f;
+    const float safe = finite_or_zero(tm);
+    float ts = 0.0f;
+    if (active)
+        for (int j = lane; j < a.K; j += L)
+            if (id_at(a, row, j) >= 0) ts += exp2_approx((teacher_at(a, row, j) - safe) * a.c);
+    ts = group_sum<L>(ts);
+    const float log_s = log2f(s), log_ts = log2f(ts);
+    float l = 0.0f;
+    if (active && any && !bad)
+        for (int j = lane; j < a.K; j += L) {
+            const int64_t id = id_at(a, row, j);
+            if (id < 0) continue;
+            const float lp = (teacher_at(a, row, j) - safe) * a.c - log_ts, p = exp2_approx(lp);
+            const float lq = (to_float(z[id]) - m) * a.c - log_s;
+            if (p != 0.0f) l += p * (lp - lq);
+        }
+    l = group_sum<L>(l) * (a.T * a.T * LN2);
+    if (bad) { l = NAN; ts = NAN; }
+    if (!any && !bad) ts = 0.0f;
+    counted = any || bad ? 1.0f : 0.0f;
+    if (active && lane == 0) {
+        a.state[row] = make_float4(m, s, safe, ts);
+        if (a.reduction == RED_NONE) a.loss[row] = l;
+    }
+    return l;
+}
+
+// ---- rows of up to SHORT_ROW classes: L lanes a row, the losses of a block's rows summed ----
+template <typename T, int L> __global__ void __launch_bounds__(THREADS) short_fwd_kernel(const Args a) {
+    __shared__ float red[64];
+    const int lane = threadIdx.x % L;
+    constexpr int ROWS = THREADS / L;
+    float sum = 0.0f, count = 0.0f;
+    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.n; r0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = r0 + threadIdx.x / L;
+        const bool active = row < a.n;
+        float m = NEG_INF, s = 0.0f;
+        if (active) {
+            const T *z = static_cast<const T *>(a.z) + row * a.ldz;
+            span_stats<T, 2>(Span<T>(z, 0, a.V), lane, L, a.c, m, s);
+        }
+        const float top = group_max<L>(m);
+        s = group_sum<L>(s * exp2_approx((m - finite_or_zero(top)) * a.c));
+        float counted;
+        const float l = row_loss<T, L>(a, row, lane, active, top, s, counted);
+        if (lane == 0 && active) { sum += l; count += counted; }
+    }
+    if (a.reduction == RED_NONE) return;
+    block_sum2(sum, count, red);
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = make_float2(sum, count);
+}
+
+__device__ __forceinline__ float row_factor(const Args &a, int64_t row, const float4 &st) {
+    if (st.w == 0.0f) return 0.0f;
+    const float g = a.reduction == RED_NONE ? __ldg(a.grad + row) : loss_factor(a.grad, a.count, a.reduction);
+    return g * a.T;
+}
+
+// dz over a span: f (q - 0); what the teacher's entries take off is put right by fix_entries
+template <typename T, int UNROLL> __device__ __forceinline__ void span_grad(const Span<T> &in, T *out, bool vector, int lane, int lanes, float c,
+                                                                            float m, float f) {
+    constexpr int E = Piece<T>::E;
+    const int64_t body0 = in.head, rest0 = in.head + in.pieces * E;
+    for (int i = lane; i < in.head + in.tail; i += lanes) {
+        const int64_t at = i < in.head ? i : rest0 + (i - in.head);
+        out[at] = from_float<T>(f * exp2_approx((to_float(in.p[at]) - m) * c));
+    }
+    const uint4 *b = in.body();
+    int64_t k = lane;
+    for (; k < in.pieces; k += (int64_t)UNROLL * lanes) {
+        uint4 u[UNROLL];
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) if (k + (int64_t)i * lanes < in.pieces) u[i] = __ldg(b + k + (int64_t)i * lanes);
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) {
+            if (k + (int64_t)i * lanes >= in.pieces) break;
+            float v[E];
+            Piece<T>::unpack(u[i], v);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = f * exp2_approx((v[e] - m) * c);
+            T *o = out + body0 + (k + (int64_t)i * lanes) * E;
+            if (vector) {
+                *reinterpret_cast<uint4 *>(o) = Piece<T>::pack(v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = from_float<T>(v[e]);
+            }
+        }
+    }
+}
+
+// Classes of the teacher's entries within [lo, hi): q minus the sum of all the row's entries of that class, so that an id
+// that occurs several times gets the same value from each.  ids, p: the row's K entries in shared memory, ids below 0 absent.
+template <typename T> __device__ __forceinline__ void fix_entries(const Args &a, const T *z, T *dz, const int *ids, const float *p, int64_t lo, int64_t hi,
+                                                                  int lane, int lanes, float m, float inv_s, float f) {
+    for (int j = lane; j < a.K; j += lanes) {
+        const int id = ids[j];
+        if (id < lo || id >= hi) continue;
+        float taken = 0.0f;
+        for (int i = 0; i < a.K; ++i) if (ids[i] == id) taken += p[i];
+        dz[id] = from_float<T>(f * (exp2_approx((to_float(z[id]) - m) * a.c) * inv_s - taken));
+    }
+}
+
+__device__ __forceinline__ void stage_entries(const Args &a, int64_t row, const float4 &st, int *ids, float *p, int lane, int lanes) {
+    const float inv = 1.0f / st.w;
+    for (int j = lane; j < a.K; j += lanes) {
+        const int64_t id = id_at(a, row, j);
+        ids[j] = id < 0 || id >= a.V ? -1 : (int)id;
+        p[j] = id < 0 ? 0.0f : exp2_approx((teacher_at(a, row, j) - st.z) * a.c) * inv;
+    }
+}
+
+template <typename T> __device__ __forceinline__ bool same_offset(const T *in, const T *out) {
+    return ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+}
+
+template <typename T, int L> __global__ void __launch_bounds__(THREADS) short_bwd_kernel(const Args a) {
+    constexpr int ROWS = THREADS / L;
+    __shared__ int s_ids[ROWS][SHORT_KEPT];
+    __shared__ float s_p[ROWS][SHORT_KEPT];
+    const int lane = threadIdx.x % L, group = threadIdx.x / L;
+    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.n; r0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t row = r0 + group;
+        const bool active = row < a.n;
+        const T *z = nullptr;
+        T *dz = nullptr;
+        float4 st = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
+        float f = 0.0f, inv_s = 0.0f;
+        if (active) {
+            z = static_cast<const T *>(a.z) + row * a.ldz;
+            dz = static_cast<T *>(a.dz) + row * a.ldo;
+            st = a.state[row];
+            f = row_factor(a, row, st);
+            inv_s = 1.0f / st.y;
+            if (st.w != 0.0f) {
+                if (st.w != st.w) f = NAN;
+                span_grad<T, 2>(Span<T>(z, 0, a.V), dz, same_offset(z, dz), lane, L, a.c, st.x, f * inv_s);
+                stage_entries(a, row, st, s_ids[group], s_p[group], lane, L);
+            } else {
+                for (int64_t i = lane; i < a.V; i += L) dz[i] = from_float<T>(0.0f);
+            }
+        }
+        __syncwarp();                                    // the group's stores and staged entries before its corrections
+        if (active && st.w > 0.0f) fix_entries<T>(a, z, dz, s_ids[group], s_p[group], 0, a.V, lane, L, st.x, inv_s, f);
+        __syncwarp();
+    }
+}
+
+// ---- longer rows: a CTA per row, or per part of a row where there are few rows ----
+template <typename T> __global__ void __launch_bounds__(THREADS) long_fwd_kernel(const Args a) {
+    __shared__ float red_m[THREADS / 32], red_s[THREADS / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float sum = 0.0f, count = 0.0f;
+    const int64_t items = a.n * a.splits;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t row = item / a.splits;
+        const int split = (int)(item - row * a.splits);
+        const int64_t lo = split * a.part, hi = min(a.V, lo + a.part);
+        float m = NEG_INF, s = 0.0f;
+        const T *z = static_cast<const T *>(a.z) + row * a.ldz;
+        span_stats<T, 4>(Span<T>(z, lo, hi), threadIdx.x, THREADS, a.c, m, s);
+        float top = group_max<32>(m);
+        s = group_sum<32>(s * exp2_approx((m - finite_or_zero(top)) * a.c));
+        if (lane == 0) { red_m[warp] = top; red_s[warp] = s; }
+        __syncthreads();
+        if (warp == 0) {
+            m = lane < THREADS / 32 ? red_m[lane] : NEG_INF;
+            s = lane < THREADS / 32 ? red_s[lane] : 0.0f;
+            top = group_max<32>(m);
+            s = group_sum<32>(s * exp2_approx((m - finite_or_zero(top)) * a.c));
+            if (a.splits == 1) {
+                float counted;
+                sum += row_loss<T, 32>(a, row, lane, true, top, s, counted);
+                count += counted;
+            } else if (lane == 0) {
+                a.stats[(int64_t)split * a.n + row] = make_float2(top, s);
+            }
+        }
+        __syncthreads();
+    }
+    if (a.splits == 1 && a.reduction != RED_NONE && threadIdx.x == 0) a.partial[blockIdx.x] = make_float2(sum, count);
+}
+
+// joins the parts of the rows of long_fwd_kernel; a warp per row
+template <typename T> __global__ void __launch_bounds__(THREADS) join_fwd_kernel(const Args a) {
+    __shared__ float red[64];
+    const int lane = threadIdx.x & 31;
+    float sum = 0.0f, count = 0.0f;
+    for (int64_t row = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); row < a.n; row += (int64_t)gridDim.x * (THREADS / 32)) {
+        float m = NEG_INF, s = 0.0f;
+        for (int i = lane; i < a.splits; i += 32) {
+            const float2 p = a.stats[(int64_t)i * a.n + row];
+            join_stats(m, s, p.x, p.y, a.c);
+        }
+        const float top = group_max<32>(m);
+        s = group_sum<32>(s * exp2_approx((m - finite_or_zero(top)) * a.c));
+        float counted;
+        const float l = row_loss<T, 32>(a, row, lane, true, top, s, counted);
+        if (lane == 0) { sum += l; count += counted; }
+    }
+    if (a.reduction == RED_NONE) return;
+    block_sum2(sum, count, red);
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = make_float2(sum, count);
+}
+
+template <typename T> __global__ void __launch_bounds__(THREADS) long_bwd_kernel(const Args a) {
+    __shared__ int s_ids[MAX_KEPT];
+    __shared__ float s_p[MAX_KEPT];
+    const int64_t items = a.n * a.splits;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t row = item / a.splits;
+        const int64_t lo = (item - row * a.splits) * a.part, hi = min(a.V, lo + a.part);
+        const T *z = static_cast<const T *>(a.z) + row * a.ldz;
+        T *dz = static_cast<T *>(a.dz) + row * a.ldo;
+        const float4 st = a.state[row];
+        const float inv_s = 1.0f / st.y;
+        float f = row_factor(a, row, st);
+        if (st.w == 0.0f) {
+            for (int64_t i = lo + threadIdx.x; i < hi; i += THREADS) dz[i] = from_float<T>(0.0f);
+        } else {
+            if (st.w != st.w) f = NAN;
+            stage_entries(a, row, st, s_ids, s_p, threadIdx.x, THREADS);
+            span_grad<T, 4>(Span<T>(z, lo, hi), dz + lo, same_offset(z, dz), threadIdx.x, THREADS, a.c, st.x, f * inv_s);
+        }
+        __syncthreads();
+        if (st.w > 0.0f) fix_entries<T>(a, z, dz, s_ids, s_p, lo, hi, threadIdx.x, THREADS, st.x, inv_s, f);
+        __syncthreads();
+    }
+}
+
+static int64_t grid_limit() { return (int64_t)sm_count() * CTAS_PER_SM; }
+
+static bool short_rows(int64_t V, int K) { return V <= SHORT_ROW && K <= SHORT_KEPT; }
+// lanes of a short row: about two 16-byte pieces each
+static int short_lanes(int64_t V, size_t es) {
+    const int64_t pieces = ceil_div(V * (int64_t)es, (int64_t)16);
+    return pieces <= 8 ? 4 : pieces <= 16 ? 8 : pieces <= 32 ? 16 : 32;
+}
+// Parts of a long row: as many as give every SM work, none shorter than SPLIT_MIN classes; part lengths are whole pieces.
+static void split_rows(int64_t n, int64_t V, int *splits, int64_t *part) {
+    int64_t s = ceil_div(grid_limit() / 2, n > 0 ? n : 1);
+    const int64_t most = V / SPLIT_MIN;
+    if (s > most) s = most;
+    if (s < 1) s = 1;
+    *part = ceil_div(ceil_div(V, s), (int64_t)64) * 64;
+    *splits = (int)ceil_div(V, *part);
+}
+
+struct Layout { size_t partial, stats, bytes; };
+static Layout layout(int64_t n, int64_t V) {
+    int splits;
+    int64_t part;
+    split_rows(n, V, &splits, &part);
+    Layout l;
+    l.partial = 0;
+    l.stats = (size_t)grid_limit() * sizeof(float2);
+    l.bytes = l.stats + (splits > 1 ? (size_t)splits * (size_t)n * sizeof(float2) : 0);
+    return l;
+}
+
+template <typename T, int L> static int launch_short(const Args &a, bool fwd, int64_t *grid, cudaStream_t st) {
+    int64_t g = ceil_div(a.n, (int64_t)(THREADS / L));
+    if (g > grid_limit()) g = grid_limit();
+    *grid = g;
+    if (fwd) short_fwd_kernel<T, L><<<(unsigned)g, THREADS, 0, st>>>(a);
+    else short_bwd_kernel<T, L><<<(unsigned)g, THREADS, 0, st>>>(a);
+    GRWS_CUDA_TRY(cudaGetLastError());
+    return GRWS_OK;
+}
+
+template <typename T> static int launch(Args a, bool fwd, float *loss, float *count, cudaStream_t st) {
+    int64_t grid = 0;
+    if (short_rows(a.V, a.K)) {
+        int rc;
+        switch (short_lanes(a.V, sizeof(T))) {
+            case 4: rc = launch_short<T, 4>(a, fwd, &grid, st); break;
+            case 8: rc = launch_short<T, 8>(a, fwd, &grid, st); break;
+            case 16: rc = launch_short<T, 16>(a, fwd, &grid, st); break;
+            default: rc = launch_short<T, 32>(a, fwd, &grid, st); break;
+        }
+        if (rc != GRWS_OK) return rc;
+    } else {
+        split_rows(a.n, a.V, &a.splits, &a.part);
+        grid = a.n * a.splits < grid_limit() ? a.n * a.splits : grid_limit();
+        if (fwd) long_fwd_kernel<T><<<(unsigned)grid, THREADS, 0, st>>>(a);
+        else long_bwd_kernel<T><<<(unsigned)grid, THREADS, 0, st>>>(a);
+        GRWS_CUDA_TRY(cudaGetLastError());
+        if (fwd && a.splits > 1) {
+            grid = ceil_div(a.n, (int64_t)(THREADS / 32));
+            if (grid > grid_limit()) grid = grid_limit();
+            join_fwd_kernel<T><<<(unsigned)grid, THREADS, 0, st>>>(a);
+            GRWS_CUDA_TRY(cudaGetLastError());
+        }
+    }
+    if (fwd && a.reduction != RED_NONE) {
+        loss_sum_kernel<<<1, 512, 0, st>>>(a.partial, (int)grid, a.reduction, loss, count);
+        GRWS_CUDA_TRY(cudaGetLastError());
+    }
+    return GRWS_OK;
+}
+
+static int check(int64_t n, int64_t V, int64_t K, int64_t ldz, int64_t ldt, int64_t ldi, int dtype, int t_dtype, int id_bytes, float T, int reduction) {
+    GRWS_REQUIRE(n >= 0 && V > 0 && K > 0, "bad size (rows = %lld, classes = %lld, kept = %lld)", (long long)n, (long long)V, (long long)K);
+    GRWS_REQUIRE(V <= INT32_MAX && n <= INT32_MAX, "rows and classes must fit 31 bits");
+    if (K > MAX_KEPT) return fail(GRWS_ERR_UNSUPPORTED, "at most %d teacher entries per row (kept = %lld)", MAX_KEPT, (long long)K);
+    GRWS_REQUIRE(ldz >= V && ldt >= K && ldi >= K, "leading dimension smaller than the row");
+    if (dtype < GRWS_F32 || dtype > GRWS_BF16) return fail(GRWS_ERR_UNSUPPORTED, "bad dtype %d", dtype);
+    if (t_dtype < GRWS_F32 || t_dtype > GRWS_BF16) return fail(GRWS_ERR_UNSUPPORTED, "bad teacher dtype %d", t_dtype);
+    GRWS_REQUIRE(id_bytes == 4 || id_bytes == 8, "ids are 4- or 8-byte integers");
+    GRWS_REQUIRE(T >= 0.99e-6f && T <= 1.01e6f, "the temperature must lie between 1e-6 and 1e6");
+    GRWS_REQUIRE(reduction >= RED_NONE && reduction <= RED_SUM, "bad reduction %d", reduction);
+    return GRWS_OK;
+}
+
+}  // namespace distill
+}  // namespace grws
+
+using namespace grws;
+
+extern "C" {
+
+__attribute__((visibility("default")))
+size_t grws_distill_scratch_bytes(int64_t rows, int64_t classes) {
+    if (rows < 0 || classes <= 0) return 0;
+    return distill::layout(rows, classes).bytes;
+}
+
+__attribute__((visibility("default")))
+int grws_distill_fwd(const void *logits, int64_t ldz, int dtype, const void *teacher, int64_t ldt, int teacher_dtype, const void *ids,
+                     int64_t ldi, int id_bytes, int64_t rows, int64_t classes, int64_t kept, float temperature, int reduction,
+                     float *loss, float *state, float *count, void *scratch, size_t scratch_bytes, void *stream) {
+    int rc = distill::check(rows, classes, kept, ldz, ldt, ldi, dtype, teacher_dtype, id_bytes, temperature, reduction);
+    if (rc != GRWS_OK) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    GRWS_REQUIRE(reduction == cls::RED_NONE || (loss && count), "null pointer");
+    if (rows == 0) {
+        if (reduction == cls::RED_NONE) return GRWS_OK;
+        cls::loss_sum_kernel<<<1, 32, 0, st>>>(nullptr, 0, reduction, loss, count);
+        GRWS_CUDA_TRY(cudaGetLastError());
+        return GRWS_OK;
+    }
+    GRWS_REQUIRE(logits && teacher && ids && loss && state && scratch, "null pointer");
+    GRWS_REQUIRE(aligned16(state) && aligned16(scratch), "state and scratch must be 16-byte aligned");
+    const distill::Layout l = distill::layout(rows, classes);
+    if (scratch_bytes < l.bytes) return fail(GRWS_ERR_SCRATCH, "distillation scratch too small");
+    distill::Args a = {};
+    a.z = logits; a.ldz = ldz; a.t = teacher; a.ldt = ldt; a.t_dtype = teacher_dtype; a.ids = ids; a.ldi = ldi; a.id_bytes = id_bytes;
+    a.n = rows; a.V = classes; a.K = (int)kept; a.T = temperature; a.c = cls::LOG2E / temperature; a.reduction = reduction;
+    a.loss = loss; a.state = reinterpret_cast<float4 *>(state); a.splits = 1; a.part = classes;
+    a.partial = reinterpret_cast<float2 *>(static_cast<char *>(scratch) + l.partial);
+    a.stats = reinterpret_cast<float2 *>(static_cast<char *>(scratch) + l.stats);
+    switch (dtype) {
+        case GRWS_F32: return distill::launch<float>(a, true, loss, count, st);
+        case GRWS_F16: return distill::launch<__half>(a, true, loss, count, st);
+        default: return distill::launch<__nv_bfloat16>(a, true, loss, count, st);
+    }
+}
+
+__attribute__((visibility("default")))
+int grws_distill_bwd(const void *logits, int64_t ldz, int dtype, const void *teacher, int64_t ldt, int teacher_dtype, const void *ids,
+                     int64_t ldi, int id_bytes, int64_t rows, int64_t classes, int64_t kept, float temperature, int reduction,
+                     const float *grad_loss, const float *state, const float *count, void *dlogits, int64_t ldo, void *stream) {
+    int rc = distill::check(rows, classes, kept, ldz, ldt, ldi, dtype, teacher_dtype, id_bytes, temperature, reduction);
+    if (rc != GRWS_OK) return rc;
+    GRWS_REQUIRE(ldo >= classes, "leading dimension smaller than the row");
+    if (rows == 0) return GRWS_OK;
+    GRWS_REQUIRE(logits && teacher && ids && grad_loss && state && dlogits, "null pointer");
+    GRWS_REQUIRE(reduction != cls::RED_MEAN || count, "null pointer");
+    GRWS_REQUIRE(aligned16(state), "state must be 16-byte aligned");
+    distill::Args a = {};
+    a.z = logits; a.ldz = ldz; a.t = teacher; a.ldt = ldt; a.t_dtype = teacher_dtype; a.ids = ids; a.ldi = ldi; a.id_bytes = id_bytes;
+    a.n = rows; a.V = classes; a.K = (int)kept; a.T = temperature; a.c = cls::LOG2E / temperature; a.reduction = reduction;
+    a.state = reinterpret_cast<float4 *>(const_cast<float *>(state)); a.splits = 1; a.part = classes;
+    a.grad = grad_loss; a.count = count; a.dz = dlogits; a.ldo = ldo;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case GRWS_F32: return distill::launch<float>(a, false, nullptr, nullptr, st);
+        case GRWS_F16: return distill::launch<__half>(a, false, nullptr, nullptr, st);
+        default: return distill::launch<__nv_bfloat16>(a, false, nullptr, nullptr, st);
+    }
+}
+
+}  // extern "C"

@@ -1,0 +1,186 @@
+"""Losses over the class axis on the library's kernels (csrc/linear_ce.cu, csrc/distill.cu): softmax cross entropy of a
+linear classifier that never keeps its scores, and distillation from a teacher's best scores.  The reference's steps take
+F.cross_entropy of the last layer's output (helper/engine.py:66-75)."""
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from ..core import _native
+from ..core import _DT, _ptr, _scratch, _stream
+
+_REDUCTIONS = {'none': _native.REDUCE_NONE, 'mean': _native.REDUCE_MEAN, 'sum': _native.REDUCE_SUM}
+_INDEX_BYTES = {torch.int64: 8, torch.int32: 4}
+MAX_KEPT = 1024
+
+
+def _reduction(name):
+    if name not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {', '.join(_REDUCTIONS)}, got {name!r}")
+    return _REDUCTIONS[name]
+
+
+def _matrix(t, name):
+    if t.dim() != 2:
+        raise RuntimeError(f"{name} must be a matrix, got shape {tuple(t.shape)}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if t.dtype not in _DT:
+        raise RuntimeError(f"unsupported dtype {t.dtype} of {name}")
+
+
+def _same_device(t, device, name):
+    if t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, expected {device}")
+
+
+def _rows_of(t):
+    """``t`` with unit column stride and rows that do not overlap; what has neither is copied."""
+    n, d = t.shape
+    return t if (t.stride(1) == 1 or d == 1) and (t.stride(0) >= d or n == 1) and t.stride(0) > 0 else t.contiguous()
+
+
+def _stride(t):
+    """Row stride of a matrix of ``_rows_of`` (that of a single row means nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _outputs(rows, per_row, reduction, device):
+    loss = torch.empty(rows if reduction == _native.REDUCE_NONE else (), dtype=torch.float32, device=device)
+    state = torch.empty(rows * per_row + 4, dtype=torch.float32, device=device)      # the last four: the count of the rows
+    return loss, state
+
+
+class _LinearCrossEntropyFunction(Function):
+    @staticmethod
+    def forward(ctx, x, weight, labels, ignore_index, reduction):
+        lib = _native.lib()
+        x, labels = _rows_of(x), labels.contiguous()
+        class_major = weight.stride(1) != 1 and weight.stride(0) == 1
+        w = _rows_of(weight.t() if class_major else weight)
+        (n, d), V = x.shape, weight.shape[1]
+        loss, state = _outputs(n, 2, reduction, x.device)
+        count = state.data_ptr() + 8 * n
+        args = (_ptr(x), _stride(x), _ptr(w), _stride(w), int(class_major))
+        with torch.cuda.device(x.device):
+            scratch = _scratch(lib.grws_linear_ce_scratch_bytes(*args, n, d, V, _DT[x.dtype], 0), x.device)
+            _native.check(lib.grws_linear_ce_fwd(*args, _ptr(labels), _INDEX_BYTES[labels.dtype], ignore_index, n, d, V, _DT[x.dtype],
+                                                 reduction, loss.data_ptr(), state.data_ptr(), count, scratch.data_ptr(),
+                                                 scratch.numel(), _stream(x.device)))
+        ctx.save_for_backward(x, w, labels, state)
+        ctx.args = (ignore_index, reduction, class_major)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss):
+        lib = _native.lib()
+        x, w, labels, state = ctx.saved_tensors
+        ignore_index, reduction, class_major = ctx.args
+        (n, d), V = x.shape, w.shape[0] if class_major else w.shape[1]
+        grad_loss = grad_loss.contiguous()
+        dx = torch.empty((n, d), dtype=x.dtype, device=x.device) if ctx.needs_input_grad[0] else None
+        dw = torch.empty(w.shape, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[1] else None
+        args = (_ptr(x), _stride(x), _ptr(w), _stride(w), int(class_major))
+        with torch.cuda.device(x.device):
+            scratch = _scratch(lib.grws_linear_ce_scratch_bytes(*args, n, d, V, _DT[x.dtype], 1), x.device)
+            _native.check(lib.grws_linear_ce_bwd(*args, _ptr(labels), _INDEX_BYTES[labels.dtype], ignore_index, n, d, V, _DT[x.dtype],
+                                                 reduction, _ptr(grad_loss), state.data_ptr(), state.data_ptr() + 8 * n, _ptr(dx),
+                                                 _ptr(dw), scratch.data_ptr(), scratch.numel(), _stream(x.device)))
+        return dx, dw.t() if class_major and dw is not None else dw, None, None, None
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
+                         reduction: str = 'mean') -> torch.Tensor:
+    """Softmax cross entropy of the scores ``x @ weight`` against ``labels``, in fp32, without keeping the scores.
+
+    x [rows, width] and weight [width, classes] (the layout of the layers' weights; the transpose of a
+    [classes, width] matrix is as good) are fp32, fp16 or bf16 CUDA matrices of one type, labels [rows] int32 or
+    int64.  Rows labelled ``ignore_index`` count nothing; any other label outside [0, classes) makes the loss
+    and the gradients NaN.  'mean' divides by the number of counted rows (none: NaN, and no gradient),
+    'none' returns a loss per row.  The backward pass computes the scores again, a piece of the classes
+    at a time, and returns gradients of the operands' type; there is no second derivative.  Results do
+    not change from call to call."""
+    red = _reduction(reduction)
+    _matrix(x, "x")
+    _matrix(weight, "weight")
+    if weight.dtype != x.dtype:
+        raise RuntimeError(f"x is {x.dtype} and weight is {weight.dtype}: one dtype is expected")
+    if weight.shape[0] != x.shape[1] or x.shape[1] == 0 or weight.shape[1] == 0:
+        raise RuntimeError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not multiply to class scores")
+    if labels.dtype not in _INDEX_BYTES:
+        raise RuntimeError(f"labels must be int32 or int64, got {labels.dtype}")
+    if tuple(labels.shape) != (x.shape[0],):
+        raise RuntimeError(f"labels must have shape ({x.shape[0]},), got {tuple(labels.shape)}")
+    _same_device(weight, x.device, "weight")
+    _same_device(labels, x.device, "labels")
+    return _LinearCrossEntropyFunction.apply(x, weight, labels, int(ignore_index), red)
+
+
+class _DistillationFunction(Function):
+    @staticmethod
+    def forward(ctx, logits, teacher, ids, temperature, reduction):
+        lib = _native.lib()
+        logits, teacher, ids = _rows_of(logits), _rows_of(teacher), _rows_of(ids)
+        (n, V), K = logits.shape, ids.shape[1]
+        loss, state = _outputs(n, 4, reduction, logits.device)
+        with torch.cuda.device(logits.device):
+            scratch = _scratch(lib.grws_distill_scratch_bytes(n, V), logits.device)
+            _native.check(lib.grws_distill_fwd(
+                _ptr(logits), _stride(logits), _DT[logits.dtype], _ptr(teacher), _stride(teacher), _DT[teacher.dtype], _ptr(ids),
+                _stride(ids), _INDEX_BYTES[ids.dtype], n, V, K, temperature, reduction, loss.data_ptr(), state.data_ptr(),
+                state.data_ptr() + 16 * n, scratch.data_ptr(), scratch.numel(), _stream(logits.device)))
+        ctx.save_for_backward(logits, teacher, ids, state)
+        ctx.args = (temperature, reduction)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss):
+        lib = _native.lib()
+        logits, teacher, ids, state = ctx.saved_tensors
+        temperature, reduction = ctx.args
+        (n, V), K = logits.shape, ids.shape[1]
+        grad_loss = grad_loss.contiguous()
+        # rows as far apart as the scores' (or, where these are a narrow cut, in whole 16-byte pieces), so that both
+        # can be walked in the same 16-byte pieces
+        ld = _stride(logits)
+        ldo = ld if ld <= V + 16 else -(-V // 8) * 8
+        dlogits = torch.empty((n, ldo), dtype=logits.dtype, device=logits.device)[:, :V]
+        with torch.cuda.device(logits.device):
+            _native.check(lib.grws_distill_bwd(
+                _ptr(logits), ld, _DT[logits.dtype], _ptr(teacher), _stride(teacher), _DT[teacher.dtype], _ptr(ids), _stride(ids),
+                _INDEX_BYTES[ids.dtype], n, V, K, temperature, reduction, _ptr(grad_loss), state.data_ptr(), state.data_ptr() + 16 * n,
+                _ptr(dlogits), ldo, _stream(logits.device)))
+        return dlogits, None, None, None, None
+
+
+def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor, temperature: float = 1.0,
+                      reduction: str = 'mean') -> torch.Tensor:
+    """``T^2 KL(p || softmax(logits / T))`` per row, in fp32, where p is the softmax over the teacher's kept scores at
+    temperature T: a student learns the classes that its teacher finds best.
+
+    logits [rows, classes] and teacher_logits [rows, kept] are fp32, fp16 or bf16 CUDA matrices, each of its own
+    type, teacher_ids [rows, kept] the classes of the kept scores (int32 or int64, at most 1,024 a row).  An id
+    below 0 is a missing entry, as padded column ids are; a row without entries counts nothing.  A class
+    that occurs twice in a row counts with both scores; an id past the classes makes the row's loss
+    and gradient NaN.  'mean' divides by the number of rows with entries (none: NaN, and no gradient), 'none'
+    returns a loss per row.  Only ``logits`` has a gradient, and no second one."""
+    red = _reduction(reduction)
+    _matrix(logits, "logits")
+    _matrix(teacher_logits, "teacher_logits")
+    if teacher_ids.dtype not in _INDEX_BYTES:
+        raise RuntimeError(f"teacher_ids must be int32 or int64, got {teacher_ids.dtype}")
+    if teacher_ids.shape != teacher_logits.shape or teacher_ids.shape[0] != logits.shape[0]:
+        raise RuntimeError(f"teacher_logits {tuple(teacher_logits.shape)} and teacher_ids {tuple(teacher_ids.shape)} must both be "
+                           f"[{logits.shape[0]}, kept]")
+    if logits.shape[1] == 0 or not 1 <= teacher_ids.shape[1] <= MAX_KEPT:
+        raise RuntimeError(f"at least one class and between 1 and {MAX_KEPT} kept scores are expected, got {logits.shape[1]} and "
+                           f"{teacher_ids.shape[1]}")
+    _same_device(teacher_logits, logits.device, "teacher_logits")
+    _same_device(teacher_ids, logits.device, "teacher_ids")
+    if torch.is_grad_enabled() and teacher_logits.requires_grad:
+        raise RuntimeError("teacher_logits gets no gradient: detach it")
+    temperature = float(temperature)
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"temperature must lie between 1e-6 and 1e6, got {temperature}")
+    return _DistillationFunction.apply(logits, teacher_logits, teacher_ids, temperature, red)

@@ -261,6 +261,59 @@ int grws_layer_norm_bwd(const void *x, const void *gamma, const void *dy, const 
                         void *stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Losses over the class axis.  `reduction`: GRWS_REDUCE_NONE writes one loss per row, MEAN the mean
+ * over the counted rows (none: NaN), SUM their sum.  Losses, gradients of losses and states are fp32,
+ * whatever the type of the scores; sums are added in a fixed order, so calls repeat bit by bit.
+ *
+ * Softmax cross entropy of a linear classifier (the step's loss is F.cross_entropy of the last
+ * layer's output in the reference, helper/engine.py:66-75), without keeping the scores x w:
+ *   x      [rows, width] of `dtype`, unit column stride, row stride ldx;
+ *   w      width x classes of the same type: w(k, v) at k * ldw + v (class_major = 0, the layout of
+ *          the layers' weights) or at v * ldw + k (class_major = 1);
+ *   labels [rows] integers of label_bytes (4 or 8); a row with `ignore_index` counts nothing and has
+ *          no gradient, any other label outside [0, classes) makes its loss and gradients NaN;
+ *   loss   [1], or [rows] without a reduction; state [2 * rows] and count [1] (with a reduction) go
+ *          from the forward to the backward call, 16-byte aligned state;
+ *   grad_loss  gradient of `loss`, of its size;
+ *   dx [rows, width] and dw (in w's order) contiguous, of `dtype`; either may be null.
+ * The scratch of a call depends on where its operands lie (x, w: looked at, not read).
+ * ------------------------------------------------------------------------------------------ */
+typedef enum { GRWS_REDUCE_NONE = 0, GRWS_REDUCE_MEAN = 1, GRWS_REDUCE_SUM = 2 } grws_reduction;
+
+size_t grws_linear_ce_scratch_bytes(const void *x, int64_t ldx, const void *w, int64_t ldw, int class_major,
+                                    int64_t rows, int64_t width, int64_t classes, int dtype, int backward);
+int grws_linear_ce_fwd(const void *x, int64_t ldx, const void *w, int64_t ldw, int class_major,
+                       const void *labels, int label_bytes, int64_t ignore_index, int64_t rows,
+                       int64_t width, int64_t classes, int dtype, int reduction, float *loss,
+                       float *state, float *count, void *scratch, size_t scratch_bytes, void *stream);
+int grws_linear_ce_bwd(const void *x, int64_t ldx, const void *w, int64_t ldw, int class_major,
+                       const void *labels, int label_bytes, int64_t ignore_index, int64_t rows,
+                       int64_t width, int64_t classes, int dtype, int reduction, const float *grad_loss,
+                       const float *state, const float *count, void *dx, void *dw, void *scratch,
+                       size_t scratch_bytes, void *stream);
+
+/* Distillation from a teacher's best scores: T^2 KL(p || softmax(logits / T)), p the softmax over a row's
+ * kept teacher scores at temperature T.
+ *   logits  [rows, classes] of `dtype`, unit column stride, row stride ldz;
+ *   teacher [rows, kept] scores of `teacher_dtype` and ids [rows, kept] of id_bytes (4 or 8), unit
+ *           column stride; kept <= 1024.  An id below 0 is a missing entry, a row without entries
+ *           counts nothing and has a zero gradient; an id that occurs twice counts twice; an id past
+ *           the classes makes the row's loss and gradient NaN;
+ *   state   [4 * rows], 16-byte aligned; count, loss, grad_loss as above;
+ *   dlogits [rows, classes] of `dtype`, row stride ldo; only the classes are written.
+ * Forward scratch: grws_distill_scratch_bytes; backward needs none. */
+size_t grws_distill_scratch_bytes(int64_t rows, int64_t classes);
+int grws_distill_fwd(const void *logits, int64_t ldz, int dtype, const void *teacher, int64_t ldt,
+                     int teacher_dtype, const void *ids, int64_t ldi, int id_bytes, int64_t rows,
+                     int64_t classes, int64_t kept, float temperature, int reduction, float *loss,
+                     float *state, float *count, void *scratch, size_t scratch_bytes, void *stream);
+int grws_distill_bwd(const void *logits, int64_t ldz, int dtype, const void *teacher, int64_t ldt,
+                     int teacher_dtype, const void *ids, int64_t ldi, int id_bytes, int64_t rows,
+                     int64_t classes, int64_t kept, float temperature, int reduction,
+                     const float *grad_loss, const float *state, const float *count, void *dlogits,
+                     int64_t ldo, void *stream);
+
+/* ------------------------------------------------------------------------------------------
  * BCSR -> CSR of the transposed matrix (rows = the BCSR's column ids), the first half of
  * building the cached transposed BCSR that the backward product runs on.  The reference has
  * no such structure: its backward is an atomicAdd scatter over the forward graph
