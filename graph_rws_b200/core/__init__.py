@@ -52,12 +52,13 @@ def _device_visible(t: torch.Tensor, name: str):
 
 def check_device_status(device=None):
     """Synchronises the current stream of ``device`` and raises RuntimeError (status -5) if any
-    tcgen05 SpMM launch on that device gave up on a pipeline wait since the last check: its output
+    tcgen05 SpMM or linear cross entropy launch on that device gave up on a pipeline wait since the last check: its output
     is then incomplete.  The kernels' waits are bounded, so a broken pipeline ends with this status
     instead of hanging the GPU.  Call it where the host synchronises anyway (end of an epoch)."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with torch.cuda.device(device):
         _native.check(_native.lib().grws_spmm_check(_stream(device)))
+        _native.check(_native.lib().grws_linear_ce_check(_stream(device)))
 
 
 def _scratch(nbytes: int, device):

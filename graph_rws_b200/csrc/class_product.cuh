@@ -1,0 +1,592 @@
+// Dense products on the 5th-generation tensor cores for the linear classifier's loss: A [M, K] B [K, N] with fp16 or bf16
+// operands, fp32 accumulators in tensor memory and an epilogue per use (scores to statistics, scores to gradients, sums to
+// an output), fed by TMA.
+//
+// Operands lie in memory with either axis contiguous: tiles of an operand whose inner axis K is contiguous are 128-byte
+// swizzled rows of 64 elements of K; of one whose outer axis is contiguous, 64 x 64 pieces of 64 outer elements a line.  Both
+// are read by the MMA as they are, so that no operand is ever transposed in memory.
+//
+// fp32 operands come as three bf16 planes (x = hi + mid + lo exactly to 24 bits), the inner axis is walked once per pair
+// of planes, the smallest products first: lo hi, hi lo, mid mid, mid hi, hi mid, hi hi.  What is left out (mid lo and below)
+// is 2^-24 of a product.
+//
+// A persistent CTA (or a pair of CTAs that share the tile's columns, CG = 2) owns output tiles of 128 CG x up to 256; two
+// accumulators alternate, so the epilogue of one tile runs under the MMAs of the next.  Warps: 0-7 epilogue (warp % 4
+// is the quarter of tensor memory, warp / 4 takes every second 32 columns), 8 TMA, 9 MMA.  All waits are bounded.
+#pragma once
+
+#include <cuda.h>
+
+#include "class_loss.cuh"
+
+namespace grws {
+namespace prod {
+
+using namespace cls;
+
+constexpr int BM = 128, BN = 256, BK = 64;          // rows per CTA, columns per tile at most, inner elements per stage
+constexpr int EPILOGUE_WARPS = 8, TMA_WARP = 8, MMA_WARP = 9, THREADS = 320;
+constexpr long long WAIT_LIMIT_CYCLES = 3000000000ll;   // about 1.5 to 2.5 s of SM clocks
+constexpr int MAX_TASKS = 2;
+
+template <int CG> struct Cfg {
+    static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN / CG * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STAGES = CG == 2 ? 6 : 4;
+    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024;      // + alignment of the first stage
+};
+
+enum Mode : int { STATS = 0, GRAD = 1, SUM = 2 };
+
+// status codes: which wait ran out
+enum : int { WAIT_OPERANDS = 1, WAIT_STAGE = 2, WAIT_ACCUMULATOR = 3, WAIT_TILE = 4 };
+
+struct Task {
+    int m_tiles, n_tiles, run, runs;      // a unit is one m tile and `run` n tiles
+    int splits, k_blocks, k_len;          // parts of the inner axis, 64-element blocks in all and per part
+    int bn;                               // columns per tile (a multiple of 32 CG)
+    int group;                            // m tiles side by side in the order of the units
+    int a_outer, b_outer;                 // operand's outer axis contiguous
+    int b_row0, b_k0;                     // first column / inner element of B within its tensor map
+    int64_t M, N;
+    // SUM
+    float *sum;                           // [splits][M][N] partial sums, added to if `add`; or
+    void *out; int64_t ldo;               // the rounded output (splits == 1, nothing before)
+    int add, out_dtype;
+    __host__ __device__ int units() const { return m_tiles * runs * splits; }
+};
+
+struct Params {
+    Task task[MAX_TASKS];
+    int tasks;
+    int pairs;                            // 1, or 6 pairs of planes
+    int bf16;
+    // STATS, GRAD
+    const void *labels; int label_bytes;
+    int64_t ignore_index, V, v0;          // number of classes, first class of column 0
+    float2 *part;                         // STATS: [2 runs][M]
+    float *label_score;                   // STATS writes, GRAD reads
+    const float2 *state;
+    int reduction;
+    const float *grad, *count, *norm;
+    float scale;                          // GRAD: power of two that keeps G within its type; SUM: its inverse
+    void *G; int64_t ldg, plane;          // rows of ldg, planes `plane` elements apart
+    int *status;
+    long long wait_limit;
+};
+
+struct alignas(64) Maps { CUtensorMap a[MAX_TASKS], b[MAX_TASKS]; };
+
+// ---------------------------------------------------------------------------------------------
+// PTX
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// address in the cluster's shared memory of what lies at `addr` in CTA `rank`
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok;
+}
+// bounded wait: gives up after `limit` SM clocks, or when another role of the CTA has
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, long long limit) {
+    if (mbar_try_wait(bar, parity)) return true;
+    long long t0 = 0;
+    for (uint32_t i = 0;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63u) == 63u) {
+            if (*abort_flag) return false;
+            const long long now = clock64();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > limit) return false;
+        }
+    }
+}
+// the same wherever another role has given up already
+__device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity, long long limit) {
+    const long long t0 = clock64();
+    for (uint32_t i = 0;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63u) == 63u && clock64() - t0 > limit) return false;
+    }
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
+template <int CG> __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    if constexpr (CG == 1)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+template <int CG> __device__ __forceinline__ void tmem_alloc(uint32_t smem_dst) {
+    if constexpr (CG == 1) asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_dst) : "memory");
+    else asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_dst) : "memory");
+}
+template <int CG> __device__ __forceinline__ void tmem_relinquish() {
+    if constexpr (CG == 1) asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    else asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+template <int CG> __device__ __forceinline__ void tmem_dealloc(uint32_t taddr) {
+    if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+template <int CG> __device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CG == 1)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// arrives on `bar` (in both CTAs of a pair) when the MMAs issued so far have finished
+template <int CG> __device__ __forceinline__ void umma_commit(uint32_t bar) {
+    if constexpr (CG == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+                   "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+                   "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// shared-memory matrix descriptor, 128-byte swizzle.  Inner axis contiguous: 8-row groups 1,024 bytes apart, a step of 16
+// inner elements is 32 bytes.  Outer axis contiguous: 64-element pieces of it `lbo` apart, groups of 8 inner elements 1,024
+// bytes apart, a step of 16 inner elements is 2,048 bytes.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, int outer) {
+    const uint64_t lbo = outer ? (64 * BK * 2) >> 4 : 1, sbo = 1024 >> 4;
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (lbo << 16) | (sbo << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// ---------------------------------------------------------------------------------------------
+// order of the units: groups of `group` m tiles, within a group the n runs one after the other, so that the CTAs at work share
+// the columns of B; parts of the inner axis outermost
+// ---------------------------------------------------------------------------------------------
+struct Unit { int task, m, n0, n1, split; };
+__device__ __forceinline__ Unit unit_at(const Params &p, int u) {
+    Unit r;
+    r.task = 0;
+    if (p.tasks > 1 && u >= p.task[0].units()) { u -= p.task[0].units(); r.task = 1; }
+    const Task &t = p.task[r.task];
+    const int per = t.m_tiles * t.runs;
+    r.split = u / per;
+    u -= r.split * per;
+    const int g = u / (t.group * t.runs), first = g * t.group, size = min(t.group, t.m_tiles - first);
+    u -= g * t.group * t.runs;
+    const int run = u / size;
+    r.m = first + (u - run * size);
+    r.n0 = run * t.run;
+    r.n1 = min(t.n_tiles, r.n0 + t.run);
+    return r;
+}
+
+struct Shared {
+    uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
+    uint32_t tmem;
+    int abort_flag;
+};
+
+__device__ __forceinline__ void give_up(Shared *ss, const Params &p, int code) {
+    ss->abort_flag = 1;
+    if (p.status) atomicMax(p.status, code);
+}
+
+// a row's own factor: 0 for an ignored row, NaN for a label that is no class; and the factor of all rows
+template <typename P> __device__ __forceinline__ float grad_row_factor(const P &p, int64_t row, int64_t label) {
+    if (label == p.ignore_index) return 0.0f;
+    if (label < 0 || label >= p.V) return NAN;
+    if (p.reduction != RED_NONE) return 1.0f;
+    const float norm = __ldg(p.norm);
+    return norm > 0.0f ? __ldg(p.grad + row) / norm : __ldg(p.grad + row);
+}
+template <typename P> __device__ __forceinline__ float grad_alpha(const P &p) {
+    if (p.reduction != RED_NONE) return loss_factor(p.grad, p.count, p.reduction);
+    const float norm = __ldg(p.norm);
+    return norm > 0.0f ? norm : 1.0f;
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, int bf16) {
+    if (bf16) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ void store16(void *p, int64_t i, float v, int bf16) {
+    if (bf16) static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half *>(p)[i] = __float2half_rn(v);
+}
+// v as three bf16 numbers; what is not finite goes into the first alone
+__device__ __forceinline__ void split3(float v, float &a, float &b, float &c) {
+    a = __bfloat162float(__float2bfloat16_rn(v));
+    const bool fin = fabsf(a) < INFINITY;
+    const float r = fin ? v - a : 0.0f;
+    b = __bfloat162float(__float2bfloat16_rn(r));
+    c = r - b;
+}
+
+template <int CG, int MODE> __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+    using C = Cfg<CG>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Shared shared;
+    Shared *ss = &shared;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;      // (the same offset in both CTAs of a pair)
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+    const int first = blockIdx.x / CG, stride = gridDim.x / CG;
+    int units = p.task[0].units();
+    if (p.tasks > 1) units += p.task[1].units();
+    const long long limit = p.wait_limit;
+    volatile int *abort_flag = &ss->abort_flag;
+
+    if (threadIdx.x == 0) {
+        ss->abort_flag = 0;
+        for (int i = 0; i < C::STAGES; ++i) { mbar_init(smem_u32(&ss->full[i]), 1); mbar_init(smem_u32(&ss->empty[i]), 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&ss->acc_full[i]), 1); mbar_init(smem_u32(&ss->acc_empty[i]), EPILOGUE_WARPS * CG); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == MMA_WARP) {
+        tmem_alloc<CG>(smem_u32(&ss->tmem));
+        tmem_relinquish<CG>();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&ss->tmem);
+
+    if (warp == TMA_WARP) {
+        if (elect_one()) {
+            // the pair's copies all count on the barrier of its first CTA, whose MMA warp issues for both
+            int stage = 0, issued = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int u = first; ok && u < units; u += stride) {
+                const Unit w = unit_at(p, u);
+                const Task &t = p.task[w.task];
+                const CUtensorMap *ma = &maps.a[w.task], *mb = &maps.b[w.task];
+                const int k0 = w.split * t.k_len, k1 = min(t.k_blocks, k0 + t.k_len);
+                const int a_row = (w.m * CG + (int)rank) * BM;
+                for (int n = w.n0; ok && n < w.n1; ++n) {
+                    const int b_row = t.b_row0 + n * t.bn + (int)rank * (t.bn / CG);
+                    for (int pair = p.pairs == 1 ? 5 : 0; ok && pair < 6; ++pair) {
+                        const int pa = pair == 0 ? 2 : pair == 2 || pair == 3 ? 1 : 0, pb = pair == 1 ? 2 : pair == 2 || pair == 4 ? 1 : 0;
+                        for (int kb = k0; kb < k1; ++kb) {
+                            if (!mbar_wait(smem_u32(&ss->empty[stage]), phase ^ 1u, abort_flag, limit)) { give_up(ss, p, WAIT_STAGE); ok = false; break; }
+                            uint32_t bar = smem_u32(&ss->full[stage]);
+                            if (rank == 0) mbar_expect_tx(bar, CG * C::STAGE_BYTES);
+                            if constexpr (CG == 2) bar = map_to_rank(bar, 0);
+                            const uint32_t a = ring + stage * C::STAGE_BYTES, b = a + C::A_BYTES;
+                            const int ka = kb * BK, kB = t.b_k0 + kb * BK;
+                            if (t.a_outer) {
+                                for (int j = 0; j < BM / 64; ++j) tma_load<CG>(a + j * (64 * BK * 2), ma, bar, a_row + j * 64, ka, pa);
+                            } else {
+                                tma_load<CG>(a, ma, bar, ka, a_row, pa);
+                            }
+                            if (t.b_outer) {
+                                for (int j = 0; j < BN / CG / 64; ++j) tma_load<CG>(b + j * (64 * BK * 2), mb, bar, b_row + j * 64, kB, pb);
+                            } else {
+                                tma_load<CG>(b, mb, bar, kB, b_row, pb);
+                            }
+                            ++issued;
+                            if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                        }
+                    }
+                }
+            }
+            // every stage that was filled has been read (and, in a pair, the other CTA's commits have arrived here)
+            // before this CTA may end
+            const long long drain = ok ? limit : limit / 8;
+            for (int i = 0; i < min(issued, (int)C::STAGES); ++i) {
+                if (stage == 0) { stage = C::STAGES; phase ^= 1u; }
+                --stage;
+                if (rank == 0 && !ok) mbar_wait_drain(smem_u32(&ss->full[stage]), phase, drain);   // copies in flight
+                if (ok && !mbar_wait(smem_u32(&ss->empty[stage]), phase, abort_flag, limit)) { give_up(ss, p, WAIT_STAGE); ok = false; }
+            }
+            if (!ok) { const long long t0 = clock64(); while (clock64() - t0 < 2000000) { } }          // the other CTA's copies
+        }
+        __syncwarp();
+    } else if (warp == MMA_WARP) {
+        if (rank == 0 && elect_one()) {
+            int stage = 0;
+            uint32_t phase = 0, tile = 0;
+            bool ok = true;
+            for (int u = first; ok && u < units; u += stride) {
+                const Unit w = unit_at(p, u);
+                const Task &t = p.task[w.task];
+                const int k0 = w.split * t.k_len, steps = (min(t.k_blocks, k0 + t.k_len) - k0) * p.pairs;
+                const uint32_t idesc = (1u << 4) | ((uint32_t)p.bf16 << 7) | ((uint32_t)p.bf16 << 10) | ((uint32_t)t.a_outer << 15) |
+                                       ((uint32_t)t.b_outer << 16) | ((uint32_t)(t.bn >> 3) << 17) | ((uint32_t)(BM * CG >> 4) << 24);
+                const uint64_t a_step = t.a_outer ? 2048 >> 4 : 32 >> 4, b_step = t.b_outer ? 2048 >> 4 : 32 >> 4;
+                for (int n = w.n0; ok && n < w.n1; ++n, ++tile) {
+                    const uint32_t buf = tile & 1u, d = tmem + buf * BN;
+                    if (!mbar_wait(smem_u32(&ss->acc_empty[buf]), ((tile >> 1) & 1u) ^ 1u, abort_flag, limit)) { give_up(ss, p, WAIT_ACCUMULATOR); ok = false; break; }
+                    tc_fence_after();
+                    for (int k = 0; k < steps; ++k) {
+                        if (!mbar_wait(smem_u32(&ss->full[stage]), phase, abort_flag, limit)) { give_up(ss, p, WAIT_OPERANDS); ok = false; break; }
+                        tc_fence_after();
+                        const uint32_t a = ring + stage * C::STAGE_BYTES;
+                        const uint64_t ad = smem_desc(a, t.a_outer), bd = smem_desc(a + C::A_BYTES, t.b_outer);
+#pragma unroll
+                        for (int i = 0; i < BK / 16; ++i) umma<CG>(d, ad + i * a_step, bd + i * b_step, idesc, k > 0 || i > 0);
+                        umma_commit<CG>(smem_u32(&ss->empty[stage]));
+                        if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                    }
+                    if (ok) umma_commit<CG>(smem_u32(&ss->acc_full[buf]));
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        const int quarter = warp & 3, half = warp >> 2;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        uint32_t acc_empty[2];
+        for (int i = 0; i < 2; ++i) {
+            acc_empty[i] = smem_u32(&ss->acc_empty[i]);
+            if constexpr (CG == 2) acc_empty[i] = map_to_rank(acc_empty[i], 0);
+        }
+        uint32_t tile = 0;
+        bool ok = true;
+        for (int u = first; ok && u < units; u += stride) {
+            const Unit w = unit_at(p, u);
+            const Task &t = p.task[w.task];
+            const int64_t row = (int64_t)(w.m * CG + (int)rank) * BM + quarter * 32 + lane;
+            const bool in = row < t.M;
+            [[maybe_unused]] float m = NEG_INF, s = 0.0f, factor = 0.0f, base = 0.0f, inv = 0.0f;
+            [[maybe_unused]] int64_t label = -1;
+            if constexpr (MODE != SUM) {
+                if (in) label = load_index(p.labels, p.label_bytes, row);
+            }
+            if constexpr (MODE == GRAD) {
+                if (in) {
+                    const float2 st = p.state[row];
+                    factor = grad_row_factor(p, row, label) * p.scale;
+                    m = st.x;
+                    inv = 1.0f / st.y;
+                    base = st.x * LOG2E + log2f(st.y);
+                }
+                if (label == p.ignore_index) label = -1;
+            }
+            if constexpr (MODE == SUM) factor = t.out ? grad_alpha(p) * p.scale : 1.0f;
+            for (int n = w.n0; ok && n < w.n1; ++n, ++tile) {
+                const uint32_t buf = tile & 1u;
+                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ss->acc_full[buf]), (tile >> 1) & 1u, abort_flag, limit));
+                if (!ok) { give_up(ss, p, WAIT_TILE); break; }
+                tc_fence_after();
+                const int64_t col0 = (int64_t)n * t.bn;
+                const int cols = (int)min((int64_t)t.bn, t.N - col0);          // of this tile
+                const int mine = (int)max((int64_t)-1, min((int64_t)BN, label - p.v0 - col0));    // label's column, if within
+                (void)mine;
+                for (int c = half * 32; c < cols; c += 64) {
+                    uint32_t r[32];
+                    tmem_ld32(tmem + buf * BN + lanes + c, r);
+                    tmem_ld_wait();
+                    if constexpr (MODE == STATS) {
+                        float v[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+                        if (__any_sync(0xffffffffu, mine >= c && mine < c + 32)) {
+                            float score = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) if (mine == c + i) score = v[i];
+                            if (in && mine >= c && mine < c + 32 && mine < cols) p.label_score[row] = score;
+                        }
+                        if (c + 32 > cols) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) if (c + i >= cols) v[i] = NEG_INF;
+                        }
+                        add_values<32>(m, s, v, LOG2E);
+                    } else if constexpr (MODE == GRAD) {
+                        if (in && p.pairs == 1) {
+                            uint16_t *o = static_cast<uint16_t *>(p.G) + row * p.ldg + col0 + c;
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8) {
+                                uint32_t q[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const float g0 = exp2_approx(fmaf(__uint_as_float(r[i + 2 * j]), LOG2E, -base)) * factor;
+                                    const float g1 = exp2_approx(fmaf(__uint_as_float(r[i + 2 * j + 1]), LOG2E, -base)) * factor;
+                                    q[j] = factor == 0.0f ? 0u : pack2(g0, g1, p.bf16);
+                                }
+                                if (c + i < cols) *reinterpret_cast<uint4 *>(o + i) = make_uint4(q[0], q[1], q[2], q[3]);
+                            }
+                            if (mine >= c && mine < c + 32 && mine < cols)      // the label's own: written last, by the same thread
+                                store16(p.G, row * p.ldg + col0 + mine, factor * (exp2_approx((p.label_score[row] - m) * LOG2E) * inv - 1.0f), p.bf16);
+                        } else if (in) {
+                            uint16_t *o = static_cast<uint16_t *>(p.G) + row * p.ldg + col0 + c;
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8) {
+                                uint32_t q[3][4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    float a[2], b[2], d[2];
+#pragma unroll
+                                    for (int h = 0; h < 2; ++h) {
+                                        const int e = i + 2 * j + h;
+                                        float g = exp2_approx((__uint_as_float(r[e]) - m) * LOG2E) * inv - (mine == c + e ? 1.0f : 0.0f);
+                                        g = factor == 0.0f ? 0.0f : g * factor;
+                                        split3(g, a[h], b[h], d[h]);
+                                    }
+                                    q[0][j] = pack2(a[0], a[1], 1);
+                                    q[1][j] = pack2(b[0], b[1], 1);
+                                    q[2][j] = pack2(d[0], d[1], 1);
+                                }
+                                if (c + i < cols) {
+#pragma unroll
+                                    for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4 *>(o + k * p.plane + i) = make_uint4(q[k][0], q[k][1], q[k][2], q[k][3]);
+                                }
+                            }
+                        }
+                    } else if (in) {
+                        if (t.out) {
+                            const int64_t at = row * t.ldo + col0 + c;
+                            const size_t es = t.out_dtype == GRWS_F32 ? 4 : 2;
+                            char *o = static_cast<char *>(t.out) + at * es;
+                            const bool vec = (reinterpret_cast<uintptr_t>(o) & 15u) == 0;
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8) {
+                                float v[8];
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[i + j]) * factor;
+                                if (t.out_dtype == GRWS_F32) {
+                                    float *f = reinterpret_cast<float *>(o) + i;
+                                    if (vec && c + i + 8 <= cols) {
+                                        *reinterpret_cast<float4 *>(f) = make_float4(v[0], v[1], v[2], v[3]);
+                                        *reinterpret_cast<float4 *>(f + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                                    } else {
+#pragma unroll
+                                        for (int j = 0; j < 8; ++j) if (c + i + j < cols) f[j] = v[j];
+                                    }
+                                } else if (vec && c + i + 8 <= cols) {
+                                    *reinterpret_cast<uint4 *>(o + i * 2) = make_uint4(pack2(v[0], v[1], p.bf16), pack2(v[2], v[3], p.bf16),
+                                                                                        pack2(v[4], v[5], p.bf16), pack2(v[6], v[7], p.bf16));
+                                } else {
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j) if (c + i + j < cols) store16(t.out, at + i + j, v[j], p.bf16);
+                                }
+                            }
+                        } else {
+                            float *f = t.sum + ((int64_t)w.split * t.M + row) * t.N + col0 + c;
+                            const bool vec = (reinterpret_cast<uintptr_t>(f) & 15u) == 0;
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) {
+                                float4 v = make_float4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]), __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+                                if (vec && c + i + 4 <= cols) {
+                                    if (t.add) {
+                                        const float4 q = *reinterpret_cast<const float4 *>(f + i);
+                                        v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+                                    }
+                                    *reinterpret_cast<float4 *>(f + i) = v;
+                                } else {
+                                    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) if (c + i + j < cols) f[i + j] = t.add ? f[i + j] + e[j] : e[j];
+                                }
+                            }
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CG == 2) mbar_arrive_cluster(acc_empty[buf]);
+                    else mbar_arrive(acc_empty[buf]);
+                }
+            }
+            if constexpr (MODE == STATS) {
+                if (ok && in) p.part[(int64_t)((w.n0 / t.run) * 2 + half) * t.M + row] = make_float2(m, s);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
+    tc_fence_after();
+    if (warp == MMA_WARP) tmem_dealloc<CG>(tmem);
+    if constexpr (CG == 2) cluster_sync();
+}
+
+// ---------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------
+// Map of a [planes][rows][cols] operand, cols contiguous, rows `ld` and planes `plane` elements apart; boxes of 64 columns
+// and `box` rows, 128-byte swizzle, zeros outside.
+inline int encode_map(CUtensorMap *map, const void *base, int bf16, int64_t cols, int64_t rows, int64_t ld, int planes, int64_t plane, int box) {
+    typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                 CUtensorMapFloatOOBfill);
+    static EncodeFn encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return reinterpret_cast<EncodeFn>(fn);
+    }();
+    if (!encode) return fail(GRWS_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    // (a single row or plane: any legal distance)
+    const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, planes > 1 ? (cuuint64_t)plane * 2 : (cuuint64_t)ld * 2};
+    const cuuint32_t boxes[3] = {64, (cuuint32_t)box, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims,
+                              strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(GRWS_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    return GRWS_OK;
+}
+
+template <int CG, int MODE> static int launch_product(const Maps &maps, const Params &p, cudaStream_t st) {
+    int64_t units = 0;
+    for (int i = 0; i < p.tasks; ++i) units += p.task[i].units();
+    const int64_t clusters = units < sm_count() / CG ? units : sm_count() / CG;
+    GRWS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<CG, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<CG>::SMEM));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(clusters * CG));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = Cfg<CG>::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    GRWS_CUDA_TRY(cudaLaunchKernelEx(&cfg, product_kernel<CG, MODE>, maps, p));
+    return GRWS_OK;
+}
+
+}  // namespace prod
+}  // namespace grws

@@ -8,7 +8,7 @@
 //
 // r_i comes in two factors: alpha, one number for all rows, applied where dx and dw are rounded to their type, and a row's own
 // factor in G, which is 1 (or 0 for an ignored row) where the loss is a mean or a sum.
-#include "class_loss.cuh"
+#include "class_product.cuh"
 
 namespace grws {
 namespace lce {
@@ -24,25 +24,12 @@ struct Problem {
     int64_t n, d, V;
     int dtype, reduction;
     const float2 *state;                 // [n]: maximum, sum of exponentials
+    const float *label_score;            // [n], behind them
     const float *grad, *count;           // backward: gradient of the loss, number of counted rows
     const float *norm;                   // backward without a reduction: largest |gradient| of a row
     __host__ __device__ int64_t w_k() const { return class_major ? 1 : ldw; }
     __host__ __device__ int64_t w_v() const { return class_major ? ldw : 1; }
 };
-
-// 0 for an ignored row, NaN for a label that is no class
-__device__ __forceinline__ float row_factor(const Problem &p, int64_t row, int64_t label) {
-    if (label == p.ignore_index) return 0.0f;
-    if (label < 0 || label >= p.V) return NAN;
-    if (p.reduction != RED_NONE) return 1.0f;
-    const float norm = __ldg(p.norm);
-    return norm > 0.0f ? __ldg(p.grad + row) / norm : __ldg(p.grad + row);
-}
-__device__ __forceinline__ float alpha_of(const Problem &p) {
-    if (p.reduction != RED_NONE) return loss_factor(p.grad, p.count, p.reduction);
-    const float norm = __ldg(p.norm);
-    return norm > 0.0f ? norm : 1.0f;
-}
 
 // largest finite |gradient| of a row: with it a row's factor is at most 1, whatever the scale of the loss
 __global__ void __launch_bounds__(1024) grad_norm_kernel(const float *__restrict__ grad, int64_t n, float *__restrict__ norm) {
@@ -182,7 +169,7 @@ template <typename T> __global__ void __launch_bounds__(256) plain_grad_kernel(c
         const int64_t row = m0 + ty * 4 + i;
         if (row >= p.n) continue;
         const int64_t label = load_index(p.labels, p.label_bytes, row);
-        const float r = row_factor(p, row, label);
+        const float r = prod::grad_row_factor(p, row, label);
         const float2 st = p.state[row];
         const float inv = 1.0f / st.y;
 #pragma unroll
@@ -219,7 +206,7 @@ __global__ void __launch_bounds__(256) plain_product_kernel(const TA *A, int64_t
 // out(m, n) = alpha * sum of the partial planes in order, rounded once to the output's type; out(m, n) at m * om + n * on
 template <typename T> __global__ void __launch_bounds__(256) round_kernel(const Problem p, const float *__restrict__ part, int parts, int64_t M, int64_t N,
                                                                           float scale, T *__restrict__ out, int64_t om, int64_t on) {
-    const float alpha = alpha_of(p) * scale;
+    const float alpha = prod::grad_alpha(p) * scale;
     const int64_t total = M * N;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         float s = 0.0f;
@@ -229,18 +216,62 @@ template <typename T> __global__ void __launch_bounds__(256) round_kernel(const 
     }
 }
 
+// Operand for the tensor cores from one whose rows no TMA copy can start at (or of fp32: three bf16 planes): rows of `ldp`
+// elements, a multiple of 8.  A thread per 8 elements.
+template <typename T> __global__ void __launch_bounds__(256) pack_kernel(const T *__restrict__ src, int64_t ld, int64_t rows, int64_t cols,
+                                                                         uint16_t *__restrict__ dst, int64_t ldp, int64_t plane) {
+    const int64_t per_row = ldp / 8, total = rows * per_row;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / per_row, c = (i - row * per_row) * 8;
+        const T *s = src + row * ld + c;
+        uint16_t *d = dst + row * ldp + c;
+        if constexpr (sizeof(T) == 2) {
+            uint32_t q[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t lo = c + 2 * j < cols ? reinterpret_cast<const uint16_t *>(s)[2 * j] : 0;
+                const uint32_t hi = c + 2 * j + 1 < cols ? reinterpret_cast<const uint16_t *>(s)[2 * j + 1] : 0;
+                q[j] = lo | hi << 16;
+            }
+            *reinterpret_cast<uint4 *>(d) = make_uint4(q[0], q[1], q[2], q[3]);
+        } else {
+            uint32_t q[3][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float a[2], b[2], e[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) prod::split3(c + 2 * j + h < cols ? to_float(s[2 * j + h]) : 0.0f, a[h], b[h], e[h]);
+                q[0][j] = prod::pack2(a[0], a[1], 1);
+                q[1][j] = prod::pack2(b[0], b[1], 1);
+                q[2][j] = prod::pack2(e[0], e[1], 1);
+            }
+#pragma unroll
+            for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4 *>(d + k * plane) = make_uint4(q[k][0], q[k][1], q[k][2], q[k][3]);
+        }
+    }
+}
+
+// Worst status of a tensor-core launch on this device since it was last read
+static __device__ int g_status;
+
 // ---------------------------------------------------------------------------------------------
 // plan: how a call is cut up, and where its workspace lies
 // ---------------------------------------------------------------------------------------------
 constexpr size_t PIECE_BYTES = 256ull << 20;       // workspace for G
+constexpr double TENSOR_PRODUCTS = 1 << 22;        // n d V from which the tensor cores take the call
 
 struct Plan {
-    int64_t parts;                                 // forward: parts of the class axis
+    bool tensor;
+    int planes;                                    // of an operand: 1, or 3 of bf16 for fp32
+    bool pack_x, pack_w;
+    int64_t ldx, ldw, ldg;                         // rows of the operands as the tensor cores read them
+    int64_t run, parts;                            // forward: class tiles per unit, parts of the class axis
     int64_t piece;                                 // backward: classes per piece
     int64_t dx_parts, dx_len, dw_parts, dw_len;    // parts of the two products' inner axes (classes of a piece, rows)
-    size_t stats, label_score, partial;            // forward scratch
+    size_t x, w;                                   // packed operands
+    size_t stats, partial;                         // forward scratch
     size_t norm, G, dx_sum, dw_sum;                // backward scratch
-    size_t fwd_bytes, bwd_bytes;
+    size_t bytes;
 };
 
 static size_t place(size_t &at, size_t bytes) {
@@ -257,28 +288,112 @@ static void cut(int64_t tiles, int64_t K, int64_t least, int64_t unit, int64_t *
     *parts = ceil_div(K > 0 ? K : 1, *len);
 }
 
-static Plan make_plan(int64_t n, int64_t d, int64_t V) {
+static int columns_per_tile(int64_t N, int cg) {
+    const int64_t tiles = ceil_div(N, (int64_t)prod::BN);
+    return (int)(ceil_div(ceil_div(N, tiles), (int64_t)(32 * cg)) * 32 * cg);
+}
+// CTAs that share a tile: pairs where there are more rows than one CTA's
+static int cta_group(int64_t M) { (void)M; return 1; }
+
+static bool needs_packing(const void *p, int64_t ld, int dtype) { return dtype == GRWS_F32 || !aligned16(p) || ld % 8 != 0; }
+
+// Class tiles that one unit of the forward pass takes: as many as leave the SMs equally busy to a few per cent
+static void cut_runs(int64_t m_tiles, int64_t n_tiles, int64_t ctas, int64_t *run, int64_t *runs) {
+    int64_t best = 1;
+    double best_cost = 1e300;
+    for (int64_t r = 1; r <= n_tiles && r <= 64; ++r) {
+        const int64_t k = ceil_div(n_tiles, r);
+        const double cost = (double)ceil_div(m_tiles * k, ctas) * (double)r + 0.05 * (double)k;      // a part costs a write and a read per row
+        if (cost <= best_cost) { best_cost = cost; best = r; }
+    }
+    *run = best;
+    *runs = ceil_div(n_tiles, best);
+}
+
+// Parts of the inner axes of dx (classes of a piece) and dw (rows), which run in one launch: a unit should be short against the
+// launch, since units are dealt out round robin, but every part is one more plane of fp32 sums through memory.  In units of one
+// 64-element step of one tile: about 0.4 us of a pair of SMs.
+static void cut_products(int64_t tiles0, int64_t k0, double sums0, int64_t tiles1, int64_t k1, double sums1, int64_t ctas, int64_t *parts0, int64_t *parts1) {
+    static const int64_t tries[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128};
+    double best = 1e300;
+    for (int64_t a : tries) {
+        if (a > 1 && k0 / a < 8) break;
+        for (int64_t b : tries) {
+            if (b > 1 && k1 / b < 8) break;
+            const int64_t l0 = ceil_div(k0, a), l1 = ceil_div(k1, b), units = tiles0 * a + tiles1 * b;
+            const double all = (double)(tiles0 * k0 + tiles1 * k1) / (double)ctas;
+            const double longest = (double)(l0 > l1 ? l0 : l1);
+            const double rounds = (double)ceil_div(units, ctas) * ((double)(tiles0 * k0 + tiles1 * k1) / (double)units);
+            double cost = rounds > all ? rounds : all;
+            if (cost < longest) cost = longest;
+            cost += ((a > 1 ? (double)a * sums0 : 0.0) + (b > 1 ? (double)b * sums1 : 0.0)) * 8.0 / 6.0e12 / 0.4e-6;
+            if (cost < best) { best = cost; *parts0 = a; *parts1 = b; }
+        }
+    }
+}
+
+static Plan make_plan(const Problem &p, bool backward) {
     Plan q = {};
-    const int64_t row_tiles = ceil_div(n, (int64_t)TM), class_tiles = ceil_div(V, (int64_t)TN), width_tiles = ceil_div(d, (int64_t)TN);
-    q.parts = ceil_div((int64_t)sm_count() * 2, row_tiles > 0 ? row_tiles : 1);
-    if (q.parts > class_tiles) q.parts = class_tiles;
+    const int64_t n = p.n, d = p.d, V = p.V;
+    q.tensor = (double)n * (double)d * (double)V >= TENSOR_PRODUCTS;
     size_t at = 0;
-    q.stats = place(at, (size_t)q.parts * n * sizeof(float2));
-    q.label_score = place(at, (size_t)n * sizeof(float));
-    q.partial = place(at, (size_t)ceil_div(n, (int64_t)256) * sizeof(float2));
-    q.fwd_bytes = at;
-    q.piece = (int64_t)(PIECE_BYTES / sizeof(float)) / (n > 0 ? n : 1) / TN * TN;
-    if (q.piece < TN) q.piece = TN;
-    if (q.piece > 32768) q.piece = 32768;           // (a grid has at most 65,535 tiles in y)
-    if (q.piece > V) q.piece = V;
-    cut(row_tiles * width_tiles, q.piece, 128, TK, &q.dx_parts, &q.dx_len);
-    cut(width_tiles * ceil_div(q.piece, (int64_t)TN), n, 128, TK, &q.dw_parts, &q.dw_len);
-    at = 0;
-    q.norm = place(at, sizeof(float));
-    q.G = place(at, (size_t)n * q.piece * sizeof(float));
-    q.dx_sum = place(at, (size_t)q.dx_parts * n * d * sizeof(float));
-    q.dw_sum = place(at, (size_t)q.dw_parts * d * q.piece * sizeof(float));
-    q.bwd_bytes = at;
+    if (!q.tensor) {
+        const int64_t row_tiles = ceil_div(n, (int64_t)TM), class_tiles = ceil_div(V, (int64_t)TN), width_tiles = ceil_div(d, (int64_t)TN);
+        if (!backward) {
+            q.parts = ceil_div((int64_t)sm_count() * 2, row_tiles > 0 ? row_tiles : 1);
+            if (q.parts > class_tiles) q.parts = class_tiles;
+            q.stats = place(at, (size_t)q.parts * n * sizeof(float2));
+            q.partial = place(at, (size_t)ceil_div(n, (int64_t)256) * sizeof(float2));
+        } else {
+            q.piece = (int64_t)(PIECE_BYTES / sizeof(float)) / (n > 0 ? n : 1) / TN * TN;
+            if (q.piece < TN) q.piece = TN;
+            if (q.piece > 32768) q.piece = 32768;           // (a grid has at most 65,535 tiles in y)
+            if (q.piece > V) q.piece = V;
+            cut(row_tiles * width_tiles, q.piece, 128, TK, &q.dx_parts, &q.dx_len);
+            cut(width_tiles * ceil_div(q.piece, (int64_t)TN), n, 128, TK, &q.dw_parts, &q.dw_len);
+            q.norm = place(at, sizeof(float));
+            q.G = place(at, (size_t)n * q.piece * sizeof(float));
+            q.dx_sum = place(at, (size_t)q.dx_parts * n * d * sizeof(float));
+            q.dw_sum = place(at, (size_t)q.dw_parts * d * q.piece * sizeof(float));
+        }
+        q.bytes = at;
+        return q;
+    }
+    q.planes = p.dtype == GRWS_F32 ? 3 : 1;
+    const int64_t w_rows = p.class_major ? V : d, w_cols = p.class_major ? d : V;
+    q.pack_x = needs_packing(p.x, p.ldx, p.dtype);
+    q.pack_w = needs_packing(p.w, p.ldw, p.dtype);
+    q.ldx = q.pack_x ? ceil_div(d, (int64_t)8) * 8 : p.ldx;
+    q.ldw = q.pack_w ? ceil_div(w_cols, (int64_t)8) * 8 : p.ldw;
+    if (q.pack_x) q.x = place(at, (size_t)q.planes * n * q.ldx * 2);
+    if (q.pack_w) q.w = place(at, (size_t)q.planes * w_rows * q.ldw * 2);
+    const int cg = cta_group(n);
+    if (!backward) {
+        const int64_t bn = columns_per_tile(V, cg);
+        cut_runs(ceil_div(n, (int64_t)(prod::BM * cg)), ceil_div(V, bn), sm_count() / cg, &q.run, &q.parts);
+        q.stats = place(at, (size_t)q.parts * 2 * n * sizeof(float2));
+        q.partial = place(at, (size_t)ceil_div(n, (int64_t)256) * sizeof(float2));
+    } else {
+        q.piece = (int64_t)(PIECE_BYTES / (2 * q.planes)) / n / prod::BN * prod::BN;
+        if (q.piece < prod::BN) q.piece = prod::BN;
+        if (q.piece > V) q.piece = V;
+        q.ldg = ceil_div(q.piece, (int64_t)8) * 8;
+        const int pg = cta_group(n > d ? n : d);
+        const int64_t rows0 = n, cols0 = d, rows1 = p.class_major ? q.piece : d, cols1 = p.class_major ? d : q.piece;
+        const int64_t tiles0 = ceil_div(rows0, (int64_t)(prod::BM * pg)) * ceil_div(cols0, (int64_t)columns_per_tile(cols0, pg));
+        const int64_t tiles1 = ceil_div(rows1, (int64_t)(prod::BM * pg)) * ceil_div(cols1, (int64_t)columns_per_tile(cols1, pg));
+        const int64_t k0 = ceil_div(q.piece, (int64_t)prod::BK), k1 = ceil_div(n, (int64_t)prod::BK);
+        cut_products(tiles0, k0, (double)rows0 * cols0, tiles1, k1, (double)rows1 * cols1, sm_count() / pg, &q.dx_parts, &q.dw_parts);
+        q.dx_len = ceil_div(k0, q.dx_parts);
+        q.dx_parts = ceil_div(k0, q.dx_len);
+        q.dw_len = ceil_div(k1, q.dw_parts);
+        q.dw_parts = ceil_div(k1, q.dw_len);
+        q.norm = place(at, sizeof(float));
+        q.G = place(at, (size_t)q.planes * n * q.ldg * 2);
+        if (q.dx_parts > 1 || q.piece < V) q.dx_sum = place(at, (size_t)q.dx_parts * n * d * sizeof(float));
+        if (q.dw_parts > 1) q.dw_sum = place(at, (size_t)q.dw_parts * d * q.piece * sizeof(float));
+    }
+    q.bytes = at;
     return q;
 }
 
@@ -292,13 +407,165 @@ template <typename T> static int launch_round(const Problem &p, const float *par
     return GRWS_OK;
 }
 
-template <typename T> static int forward(const Problem &p, const Plan &q, float *loss, float2 *state, float *count, char *scratch, cudaStream_t st) {
-    float2 *part = reinterpret_cast<float2 *>(scratch + q.stats), *partial = reinterpret_cast<float2 *>(scratch + q.partial);
-    float *label_score = reinterpret_cast<float *>(scratch + q.label_score);
-    plain_stats_kernel<T><<<dim3((unsigned)ceil_div(p.n, (int64_t)TM), (unsigned)q.parts), 256, 0, st>>>(p, part, label_score);
+// ---- the tensor cores' way ----
+struct Operands { const void *x, *w; int64_t ldx, ldw, x_plane, w_plane, w_rows, w_cols; };
+
+template <typename T> static int launch_pack(const void *src, int64_t ld, int64_t rows, int64_t cols, void *dst, int64_t ldp, cudaStream_t st) {
+    int64_t g = ceil_div(rows * (ldp / 8), (int64_t)256);
+    const int64_t most = (int64_t)sm_count() * 8;
+    if (g > most) g = most;
+    pack_kernel<T><<<(unsigned)g, 256, 0, st>>>(static_cast<const T *>(src), ld, rows, cols, static_cast<uint16_t *>(dst), ldp, rows * ldp);
     GRWS_CUDA_TRY(cudaGetLastError());
+    return GRWS_OK;
+}
+
+template <typename T> static int pack_operands(const Problem &p, const Plan &q, char *scratch, Operands *o, cudaStream_t st) {
+    o->w_rows = p.class_major ? p.V : p.d;
+    o->w_cols = p.class_major ? p.d : p.V;
+    o->x = q.pack_x ? scratch + q.x : p.x;
+    o->w = q.pack_w ? scratch + q.w : p.w;
+    o->ldx = q.ldx; o->ldw = q.ldw;
+    o->x_plane = p.n * q.ldx;
+    o->w_plane = o->w_rows * q.ldw;
+    if (q.pack_x) if (int rc = launch_pack<T>(p.x, p.ldx, p.n, p.d, scratch + q.x, q.ldx, st)) return rc;
+    if (q.pack_w) if (int rc = launch_pack<T>(p.w, p.ldw, o->w_rows, o->w_cols, scratch + q.w, q.ldw, st)) return rc;
+    return GRWS_OK;
+}
+
+// sets a product up: its tile counts, and the maps of its operands ([rows][cols] in memory, cols contiguous)
+static int set_task(prod::Task *t, CUtensorMap *ma, CUtensorMap *mb, int cg, int bf16, int planes, const void *a, int64_t a_rows, int64_t a_cols, int64_t lda,
+                    int64_t a_plane, int a_outer, const void *b, int64_t b_rows, int64_t b_cols, int64_t ldb, int64_t b_plane, int b_outer, int64_t M, int64_t N,
+                    int64_t K) {
+    t->M = M; t->N = N;
+    t->bn = columns_per_tile(N, cg);
+    t->m_tiles = (int)ceil_div(M, (int64_t)(prod::BM * cg));
+    t->n_tiles = (int)ceil_div(N, (int64_t)t->bn);
+    t->run = 1; t->runs = t->n_tiles; t->splits = 1;
+    t->k_blocks = t->k_len = (int)ceil_div(K, (int64_t)prod::BK);
+    t->group = t->m_tiles < 16 ? t->m_tiles : 16;
+    t->a_outer = a_outer; t->b_outer = b_outer;
+    if (int rc = prod::encode_map(ma, a, bf16, a_cols, a_rows, lda, planes, a_plane, a_outer ? prod::BK : prod::BM)) return rc;
+    return prod::encode_map(mb, b, bf16, b_cols, b_rows, ldb, planes, b_plane, b_outer ? prod::BK : prod::BN / cg);
+}
+
+static int product_params(const Problem &p, const Plan &q, prod::Params *r) {
+    void *status = nullptr;
+    GRWS_CUDA_TRY(cudaGetSymbolAddress(&status, g_status));
+    *r = prod::Params{};
+    r->tasks = 1;
+    r->pairs = q.planes == 3 ? 6 : 1;
+    r->bf16 = p.dtype != GRWS_F16;
+    r->labels = p.labels; r->label_bytes = p.label_bytes; r->ignore_index = p.ignore_index; r->V = p.V;
+    r->reduction = p.reduction; r->grad = p.grad; r->count = p.count; r->norm = p.norm;
+    r->state = p.state;
+    r->scale = 1.0f;
+    r->status = static_cast<int *>(status);
+    r->wait_limit = prod::WAIT_LIMIT_CYCLES;
+    return GRWS_OK;
+}
+
+template <int MODE> static int launch_grouped(int cg, const prod::Maps &maps, const prod::Params &r, cudaStream_t st) {
+    return cg == 2 ? prod::launch_product<2, MODE>(maps, r, st) : prod::launch_product<1, MODE>(maps, r, st);
+}
+
+template <typename T> static int tensor_forward(const Problem &p, const Plan &q, float2 *part, float *label_score, char *scratch, cudaStream_t st) {
+    Operands o;
+    if (int rc = pack_operands<T>(p, q, scratch, &o, st)) return rc;
+    prod::Params r;
+    if (int rc = product_params(p, q, &r)) return rc;
+    prod::Maps maps;
+    const int cg = cta_group(p.n);
+    if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, r.bf16, q.planes, o.x, p.n, p.d, o.ldx, o.x_plane, 0, o.w, o.w_rows, o.w_cols, o.ldw, o.w_plane,
+                          !p.class_major, p.n, p.V, p.d)) return rc;
+    r.task[0].run = (int)q.run;
+    r.task[0].runs = (int)q.parts;
+    r.part = part;
+    r.label_score = label_score;
+    return launch_grouped<prod::STATS>(cg, maps, r, st);
+}
+
+// G in fp16 is held as 2^12 G: |G| <= 1, and a probability of 2^-26 is still a normal number
+static float stored_scale(const Problem &p) { return p.dtype == GRWS_F16 ? 4096.0f : 1.0f; }
+
+template <typename T> static int tensor_backward(const Problem &p, const Plan &q, void *dx, void *dw, char *scratch, cudaStream_t st) {
+    Operands o;
+    if (int rc = pack_operands<T>(p, q, scratch, &o, st)) return rc;
+    void *G = scratch + q.G;
+    float *dx_sum = reinterpret_cast<float *>(scratch + q.dx_sum), *dw_sum = reinterpret_cast<float *>(scratch + q.dw_sum);
+    const int64_t g_plane = p.n * q.ldg;
+    const bool sum_dx = q.dx_parts > 1 || q.piece < p.V;
+    for (int64_t v0 = 0; v0 < p.V; v0 += q.piece) {
+        const int64_t cols = p.V - v0 < q.piece ? p.V - v0 : q.piece;
+        prod::Params r;
+        if (int rc = product_params(p, q, &r)) return rc;
+        prod::Maps maps;
+        const int cg = cta_group(p.n);
+        if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, r.bf16, q.planes, o.x, p.n, p.d, o.ldx, o.x_plane, 0, o.w, o.w_rows, o.w_cols, o.ldw,
+                              o.w_plane, !p.class_major, p.n, cols, p.d)) return rc;
+        r.task[0].b_row0 = (int)v0;
+        r.v0 = v0;
+        r.label_score = const_cast<float *>(p.label_score);
+        r.scale = stored_scale(p);
+        r.G = G; r.ldg = q.ldg; r.plane = g_plane;
+        if (int rc = launch_grouped<prod::GRAD>(cg, maps, r, st)) return rc;
+
+        if (int rc = product_params(p, q, &r)) return rc;
+        r.scale = 1.0f / stored_scale(p);
+        r.tasks = 0;
+        const int pg = cta_group(p.n > p.d ? p.n : p.d);
+        int64_t dw_parts = 1;
+        if (dw) {
+            prod::Task *t = &r.task[r.tasks];
+            // [d, V]: x^T G; [V, d]: G^T x
+            const int64_t M = p.class_major ? cols : p.d, N = p.class_major ? p.d : cols;
+            int rc;
+            if (p.class_major)
+                rc = set_task(t, &maps.a[r.tasks], &maps.b[r.tasks], pg, r.bf16, q.planes, G, p.n, cols, q.ldg, g_plane, 1, o.x, p.n, p.d, o.ldx, o.x_plane, 1, M, N, p.n);
+            else
+                rc = set_task(t, &maps.a[r.tasks], &maps.b[r.tasks], pg, r.bf16, q.planes, o.x, p.n, p.d, o.ldx, o.x_plane, 1, G, p.n, cols, q.ldg, g_plane, 1, M, N, p.n);
+            if (rc != GRWS_OK) return rc;
+            t->k_len = (int)q.dw_len;
+            t->splits = (int)(dw_parts = q.dw_parts);
+            t->sum = dw_sum;
+            t->out_dtype = p.dtype;
+            t->ldo = p.class_major ? p.d : p.V;
+            if (dw_parts == 1) t->out = static_cast<T *>(dw) + (p.class_major ? v0 * p.d : v0);
+            ++r.tasks;
+        }
+        if (dx) {
+            prod::Task *t = &r.task[r.tasks];
+            if (int rc = set_task(t, &maps.a[r.tasks], &maps.b[r.tasks], pg, r.bf16, q.planes, G, p.n, cols, q.ldg, g_plane, 0, o.w, o.w_rows, o.w_cols, o.ldw,
+                                  o.w_plane, p.class_major, p.n, p.d, cols)) return rc;
+            t->b_k0 = (int)v0;
+            t->k_len = (int)q.dx_len;
+            t->splits = (int)ceil_div((int64_t)t->k_blocks, q.dx_len);      // (a last, shorter piece has fewer)
+            t->sum = dx_sum;
+            t->add = v0 > 0;
+            t->out_dtype = p.dtype;
+            t->ldo = p.d;
+            if (!sum_dx) t->out = dx;
+            ++r.tasks;
+        }
+        if (int rc = launch_grouped<prod::SUM>(pg, maps, r, st)) return rc;
+        if (dw && dw_parts > 1) {
+            const int64_t M = p.class_major ? cols : p.d, N = p.class_major ? p.d : cols, ld = p.class_major ? p.d : p.V;
+            if (int rc = launch_round<T>(p, dw_sum, dw_parts, M, N, r.scale, static_cast<T *>(dw) + (p.class_major ? v0 * p.d : v0), ld, 1, st)) return rc;
+        }
+    }
+    return dx && sum_dx ? launch_round<T>(p, dx_sum, q.dx_parts, p.n, p.d, 1.0f / stored_scale(p), dx, p.d, 1, st) : GRWS_OK;
+}
+
+template <typename T> static int forward(const Problem &p, const Plan &q, float *loss, float2 *state, float *label_score, float *count, char *scratch,
+                                         cudaStream_t st) {
+    float2 *part = reinterpret_cast<float2 *>(scratch + q.stats), *partial = reinterpret_cast<float2 *>(scratch + q.partial);
+    if (q.tensor) {
+        if (int rc = tensor_forward<T>(p, q, part, label_score, scratch, st)) return rc;
+    } else {
+        plain_stats_kernel<T><<<dim3((unsigned)ceil_div(p.n, (int64_t)TM), (unsigned)q.parts), 256, 0, st>>>(p, part, label_score);
+        GRWS_CUDA_TRY(cudaGetLastError());
+    }
     const int64_t blocks = ceil_div(p.n, (int64_t)256);
-    rows_kernel<<<(unsigned)blocks, 256, 0, st>>>(p, part, (int)q.parts, label_score, state, loss, count, partial);
+    rows_kernel<<<(unsigned)blocks, 256, 0, st>>>(p, part, (int)(q.tensor ? 2 * q.parts : q.parts), label_score, state, loss, count, partial);
     GRWS_CUDA_TRY(cudaGetLastError());
     if (p.reduction != RED_NONE && blocks > 1) {
         loss_sum_kernel<<<1, 512, 0, st>>>(partial, (int)blocks, p.reduction, loss, count);
@@ -315,6 +582,7 @@ template <typename T> static int backward(Problem p, const Plan &q, void *dx, vo
         GRWS_CUDA_TRY(cudaGetLastError());
         p.norm = norm;
     }
+    if (q.tensor) return tensor_backward<T>(p, q, dx, dw, scratch, st);
     const unsigned row_tiles = (unsigned)ceil_div(p.n, (int64_t)TM), width_tiles = (unsigned)ceil_div(p.d, (int64_t)TN);
     const T *x = static_cast<const T *>(p.x), *w = static_cast<const T *>(p.w);
     for (int64_t v0 = 0; v0 < p.V; v0 += q.piece) {
@@ -368,10 +636,8 @@ extern "C" {
 __attribute__((visibility("default")))
 size_t grws_linear_ce_scratch_bytes(const void *x, int64_t ldx, const void *w, int64_t ldw, int class_major, int64_t rows, int64_t width,
                                     int64_t classes, int dtype, int backward) {
-    (void)x; (void)ldx; (void)w; (void)ldw; (void)class_major; (void)dtype;
     if (rows <= 0 || width <= 0 || classes <= 0) return 0;
-    const lce::Plan q = lce::make_plan(rows, width, classes);
-    return backward ? q.bwd_bytes : q.fwd_bytes;
+    return lce::make_plan(lce::problem(x, ldx, w, ldw, class_major, nullptr, 8, 0, rows, width, classes, dtype, 0), backward != 0).bytes;
 }
 
 __attribute__((visibility("default")))
@@ -391,14 +657,15 @@ int grws_linear_ce_fwd(const void *x, int64_t ldx, const void *w, int64_t ldw, i
     }
     GRWS_REQUIRE(x && w && labels && loss && state && scratch, "null pointer");
     GRWS_REQUIRE(aligned16(state) && aligned16(scratch), "state and scratch must be 16-byte aligned");
-    const lce::Plan q = lce::make_plan(rows, width, classes);
-    if (scratch_bytes < q.fwd_bytes) return fail(GRWS_ERR_SCRATCH, "linear cross entropy scratch too small");
+    const lce::Plan q = lce::make_plan(p, false);
+    if (scratch_bytes < q.bytes) return fail(GRWS_ERR_SCRATCH, "linear cross entropy scratch too small");
     char *s = static_cast<char *>(scratch);
     float2 *state2 = reinterpret_cast<float2 *>(state);
+    float *label_score = state + 2 * rows;
     switch (dtype) {
-        case GRWS_F32: return lce::forward<float>(p, q, loss, state2, count, s, st);
-        case GRWS_F16: return lce::forward<__half>(p, q, loss, state2, count, s, st);
-        default: return lce::forward<__nv_bfloat16>(p, q, loss, state2, count, s, st);
+        case GRWS_F32: return lce::forward<float>(p, q, loss, state2, label_score, count, s, st);
+        case GRWS_F16: return lce::forward<__half>(p, q, loss, state2, label_score, count, s, st);
+        default: return lce::forward<__nv_bfloat16>(p, q, loss, state2, label_score, count, s, st);
     }
 }
 
@@ -419,9 +686,10 @@ int grws_linear_ce_bwd(const void *x, int64_t ldx, const void *w, int64_t ldw, i
     GRWS_REQUIRE(x && w && labels && grad_loss && state && scratch, "null pointer");
     GRWS_REQUIRE(reduction != cls::RED_MEAN || count, "null pointer");
     GRWS_REQUIRE(aligned16(state) && aligned16(scratch), "state and scratch must be 16-byte aligned");
-    const lce::Plan q = lce::make_plan(rows, width, classes);
-    if (scratch_bytes < q.bwd_bytes) return fail(GRWS_ERR_SCRATCH, "linear cross entropy scratch too small");
+    const lce::Plan q = lce::make_plan(p, true);
+    if (scratch_bytes < q.bytes) return fail(GRWS_ERR_SCRATCH, "linear cross entropy scratch too small");
     p.state = reinterpret_cast<const float2 *>(state);
+    p.label_score = state + 2 * rows;
     p.grad = grad_loss;
     p.count = count;
     char *s = static_cast<char *>(scratch);
@@ -430,6 +698,22 @@ int grws_linear_ce_bwd(const void *x, int64_t ldx, const void *w, int64_t ldw, i
         case GRWS_F16: return lce::backward<__half>(p, q, dx, dw, s, st);
         default: return lce::backward<__nv_bfloat16>(p, q, dx, dw, s, st);
     }
+}
+
+__attribute__((visibility("default")))
+int grws_linear_ce_check(void *stream) {
+    void *word = nullptr;
+    int status = 0;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    GRWS_CUDA_TRY(cudaGetSymbolAddress(&word, lce::g_status));
+    GRWS_CUDA_TRY(cudaMemcpyAsync(&status, word, sizeof(int), cudaMemcpyDeviceToHost, s));
+    GRWS_CUDA_TRY(cudaStreamSynchronize(s));
+    if (status == 0) return GRWS_OK;
+    GRWS_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(int), s));
+    static const char *const what[] = {"", "operand tiles never arrived", "a stage was never released", "an accumulator was never released",
+                                       "a tile was never finished"};
+    return fail(GRWS_ERR_DEVICE, "a linear cross entropy launch on this device gave up waiting: %s (code %d); its output is incomplete",
+                status >= 1 && status <= 4 ? what[status] : "unknown wait", status);
 }
 
 }  // extern "C"

@@ -58,8 +58,8 @@ class _LinearCrossEntropyFunction(Function):
         class_major = weight.stride(1) != 1 and weight.stride(0) == 1
         w = _rows_of(weight.t() if class_major else weight)
         (n, d), V = x.shape, weight.shape[1]
-        loss, state = _outputs(n, 2, reduction, x.device)
-        count = state.data_ptr() + 8 * n
+        loss, state = _outputs(n, 3, reduction, x.device)
+        count = state.data_ptr() + 12 * n
         args = (_ptr(x), _stride(x), _ptr(w), _stride(w), int(class_major))
         with torch.cuda.device(x.device):
             scratch = _scratch(lib.grws_linear_ce_scratch_bytes(*args, n, d, V, _DT[x.dtype], 0), x.device)
@@ -84,7 +84,7 @@ class _LinearCrossEntropyFunction(Function):
         with torch.cuda.device(x.device):
             scratch = _scratch(lib.grws_linear_ce_scratch_bytes(*args, n, d, V, _DT[x.dtype], 1), x.device)
             _native.check(lib.grws_linear_ce_bwd(*args, _ptr(labels), _INDEX_BYTES[labels.dtype], ignore_index, n, d, V, _DT[x.dtype],
-                                                 reduction, _ptr(grad_loss), state.data_ptr(), state.data_ptr() + 8 * n, _ptr(dx),
+                                                 reduction, _ptr(grad_loss), state.data_ptr(), state.data_ptr() + 12 * n, _ptr(dx),
                                                  _ptr(dw), scratch.data_ptr(), scratch.numel(), _stream(x.device)))
         return dx, dw.t() if class_major and dw is not None else dw, None, None, None
 

@@ -272,7 +272,7 @@ int grws_layer_norm_bwd(const void *x, const void *gamma, const void *dy, const 
  *          the layers' weights) or at v * ldw + k (class_major = 1);
  *   labels [rows] integers of label_bytes (4 or 8); a row with `ignore_index` counts nothing and has
  *          no gradient, any other label outside [0, classes) makes its loss and gradients NaN;
- *   loss   [1], or [rows] without a reduction; state [2 * rows] and count [1] (with a reduction) go
+ *   loss   [1], or [rows] without a reduction; state [3 * rows] and count [1] (with a reduction) go
  *          from the forward to the backward call, 16-byte aligned state;
  *   grad_loss  gradient of `loss`, of its size;
  *   dx [rows, width] and dw (in w's order) contiguous, of `dtype`; either may be null.
@@ -291,6 +291,10 @@ int grws_linear_ce_bwd(const void *x, int64_t ldx, const void *w, int64_t ldw, i
                        int64_t width, int64_t classes, int dtype, int reduction, const float *grad_loss,
                        const float *state, const float *count, void *dx, void *dw, void *scratch,
                        size_t scratch_bytes, void *stream);
+
+/* Every wait of the tensor-core kernel is bounded; a launch whose wait ran out leaves its output incomplete and its code in a
+ * word of the device.  Synchronises `stream`, reads and clears the word: GRWS_ERR_DEVICE if a launch gave up. */
+int grws_linear_ce_check(void *stream);
 
 /* Distillation from a teacher's best scores: T^2 KL(p || softmax(logits / T)), p the softmax over a row's
  * kept teacher scores at temperature T.
