@@ -293,7 +293,7 @@ static int columns_per_tile(int64_t N, int cg) {
     return (int)(ceil_div(ceil_div(N, tiles), (int64_t)(32 * cg)) * 32 * cg);
 }
 // CTAs that share a tile: pairs where there are more rows than one CTA's
-static int cta_group(int64_t M) { (void)M; return 1; }
+static int cta_group(int64_t M) { return M > prod::BM ? 2 : 1; }
 
 static bool needs_packing(const void *p, int64_t ld, int dtype) { return dtype == GRWS_F32 || !aligned16(p) || ld % 8 != 0; }
 
