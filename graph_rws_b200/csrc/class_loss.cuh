@@ -2,6 +2,8 @@
 // statistics, the reduction of row losses and the factor a row's gradient gets from the loss's.
 #pragma once
 
+#include <utility>
+
 #include "grws_common.cuh"
 
 namespace grws {
@@ -91,6 +93,31 @@ template <int N> __device__ __forceinline__ void add_values(float &m, float &s, 
     s += t;
 }
 
+// Kernels of one call follow each other as programmatic dependents: the next one is launched while this one still runs, sets
+// itself up and waits here before it touches memory.  Every kernel waits, so each may rely on all before it.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... P, typename... A>
+inline int launch_next(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster, A &&...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    GRWS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...));
+    return GRWS_OK;
+}
+
 // The integer at i of an array of 4- or 8-byte integers
 __device__ __forceinline__ int64_t load_index(const void *p, int bytes, int64_t i) {
     return bytes == 8 ? __ldg(static_cast<const long long *>(p) + i) : (int64_t)__ldg(static_cast<const int *>(p) + i);
@@ -121,6 +148,7 @@ static __global__ void __launch_bounds__(512) loss_sum_kernel(const float2 *__re
                                                               float *__restrict__ loss, float *__restrict__ count_out) {
     __shared__ float red[64];
     float a = 0.0f, b = 0.0f;
+    wait_for_previous();
     for (int i = threadIdx.x; i < n; i += blockDim.x) { const float2 p = partial[i]; a += p.x; b += p.y; }
     block_sum2(a, b, red);
     if (threadIdx.x == 0) finish_loss(a, b, reduction, loss, count_out);

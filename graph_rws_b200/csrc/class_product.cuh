@@ -8,11 +8,16 @@
 //
 // fp32 operands come as three bf16 planes (x = hi + mid + lo exactly to 24 bits), the inner axis is walked once per pair
 // of planes, the smallest products first: lo hi, hi lo, mid mid, mid hi, hi mid, hi hi.  What is left out (mid lo and below)
-// is 2^-24 of a product.
+// is 2^-24 of a product.  The tensor cores cut every sum off towards zero, so these sums are kept short: the five small pairs
+// are one of them, the big pair one for every two stages, and the epilogue adds them up in registers, rounding to nearest.
 //
 // A persistent CTA (or a pair of CTAs that share the tile's columns, CG = 2) owns output tiles of 128 CG x up to 256; two
 // accumulators alternate, so the epilogue of one tile runs under the MMAs of the next.  Warps: 0-7 epilogue (warp % 4
-// is the quarter of tensor memory, warp / 4 takes every second 32 columns), 8 TMA, 9 MMA.  All waits are bounded.
+// is the quarter of tensor memory, warp / 4 takes every second 64 columns), 8 TMA, 9 MMA.  All waits are bounded.
+//
+// Outputs leave through shared memory as 32-row boxes of 128-byte lines (a warp's own 4 KB) and TMA stores, which also
+// clip them: rows stored from registers reach memory as 32 separate 16-byte pieces per instruction, which held the
+// gradient pass of 1,024 x 512 x 32,768 at 54 us.
 #pragma once
 
 #include <cuda.h>
@@ -28,11 +33,13 @@ constexpr int BM = 128, BN = 256, BK = 64;          // rows per CTA, columns per
 constexpr int EPILOGUE_WARPS = 8, TMA_WARP = 8, MMA_WARP = 9, THREADS = 320;
 constexpr long long WAIT_LIMIT_CYCLES = 3000000000ll;   // about 1.5 to 2.5 s of SM clocks
 constexpr int MAX_TASKS = 2;
+constexpr int BOX_BYTES = 32 * 128;                     // what a warp stores at once: 32 rows of 64 16-bit or 32 fp32 numbers
+constexpr int SUB_STAGES = 2;                           // fp32: stages of the big pair that are summed in tensor memory
 
 template <int CG> struct Cfg {
     static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN / CG * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int STAGES = CG == 2 ? 6 : 4;
-    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024;      // + alignment of the first stage
+    static constexpr int SMEM = STAGES * STAGE_BYTES + EPILOGUE_WARPS * BOX_BYTES + 1024;      // + alignment of the first stage
 };
 
 enum Mode : int { STATS = 0, GRAD = 1, SUM = 2 };
@@ -48,33 +55,32 @@ struct Task {
     int a_outer, b_outer;                 // operand's outer axis contiguous
     int b_row0, b_k0;                     // first column / inner element of B within its tensor map
     int64_t M, N;
-    // SUM
-    float *sum;                           // [splits][M][N] partial sums, added to if `add`; or
-    void *out; int64_t ldo;               // the rounded output (splits == 1, nothing before)
-    int add, out_dtype;
+    // SUM: partial sums [splits][M][] in fp32 (added to what is there if `add`), or the rounded output, through the map of
+    // the outputs; `out` with rows of ldo where its rows are no multiple of 16 bytes apart
+    int rounded, add, out_dtype;
+    void *out; int64_t ldo;
     __host__ __device__ int units() const { return m_tiles * runs * splits; }
 };
 
 struct Params {
     Task task[MAX_TASKS];
     int tasks;
-    int pairs;                            // 1, or 6 pairs of planes
     int bf16;
     // STATS, GRAD
     const void *labels; int label_bytes;
     int64_t ignore_index, V, v0;          // number of classes, first class of column 0
     float2 *part;                         // STATS: [2 runs][M]
-    float *label_score;                   // STATS writes, GRAD reads
+    float *label_score;                   // STATS: [M]
+    int *done;                            // STATS: set to 0 for the kernel behind
     const float2 *state;
     int reduction;
     const float *grad, *count, *norm;
     float scale;                          // GRAD: power of two that keeps G within its type; SUM: its inverse
-    void *G; int64_t ldg, plane;          // rows of ldg, planes `plane` elements apart
     int *status;
     long long wait_limit;
 };
 
-struct alignas(64) Maps { CUtensorMap a[MAX_TASKS], b[MAX_TASKS]; };
+struct alignas(64) Maps { CUtensorMap a[MAX_TASKS], b[MAX_TASKS], c[MAX_TASKS]; };       // operands, output
 
 // ---------------------------------------------------------------------------------------------
 // PTX
@@ -143,6 +149,27 @@ template <int CG> __device__ __forceinline__ void tma_load(uint32_t dst, const C
         asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];"
                      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
+// box of shared memory to its place in the output (what lies outside is dropped), or added to it
+__device__ __forceinline__ void tma_store(const CUtensorMap *map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(map), "r"(src), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void tma_add(const CUtensorMap *map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(map), "r"(src), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_shared32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
 template <int CG> __device__ __forceinline__ void tmem_alloc(uint32_t smem_dst) {
     if constexpr (CG == 1) asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_dst) : "memory");
     else asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_dst) : "memory");
@@ -180,6 +207,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
                    "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
                    "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
                    "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -244,10 +277,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, int bf16) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-__device__ __forceinline__ void store16(void *p, int64_t i, float v, int bf16) {
-    if (bf16) static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
-    else static_cast<__half *>(p)[i] = __float2half_rn(v);
-}
 // v as three bf16 numbers; what is not finite goes into the first alone
 __device__ __forceinline__ void split3(float v, float &a, float &b, float &c) {
     a = __bfloat162float(__float2bfloat16_rn(v));
@@ -257,7 +286,7 @@ __device__ __forceinline__ void split3(float v, float &a, float &b, float &c) {
     c = r - b;
 }
 
-template <int CG, int MODE> __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
     using C = Cfg<CG>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Shared shared;
@@ -286,6 +315,9 @@ template <int CG, int MODE> __global__ void __launch_bounds__(THREADS, 1) produc
     if constexpr (CG == 2) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&ss->tmem);
+    wait_for_previous();
+    let_next_start();
+    if (MODE == STATS && blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0;
 
     if (warp == TMA_WARP) {
         if (elect_one()) {
@@ -301,7 +333,7 @@ template <int CG, int MODE> __global__ void __launch_bounds__(THREADS, 1) produc
                 const int a_row = (w.m * CG + (int)rank) * BM;
                 for (int n = w.n0; ok && n < w.n1; ++n) {
                     const int b_row = t.b_row0 + n * t.bn + (int)rank * (t.bn / CG);
-                    for (int pair = p.pairs == 1 ? 5 : 0; ok && pair < 6; ++pair) {
+                    for (int pair = SPLIT ? 0 : 5; ok && pair < 6; ++pair) {
                         const int pa = pair == 0 ? 2 : pair == 2 || pair == 3 ? 1 : 0, pb = pair == 1 ? 2 : pair == 2 || pair == 4 ? 1 : 0;
                         for (int kb = k0; kb < k1; ++kb) {
                             if (!mbar_wait(smem_u32(&ss->empty[stage]), phase ^ 1u, abort_flag, limit)) { give_up(ss, p, WAIT_STAGE); ok = false; break; }
@@ -346,25 +378,31 @@ template <int CG, int MODE> __global__ void __launch_bounds__(THREADS, 1) produc
             for (int u = first; ok && u < units; u += stride) {
                 const Unit w = unit_at(p, u);
                 const Task &t = p.task[w.task];
-                const int k0 = w.split * t.k_len, steps = (min(t.k_blocks, k0 + t.k_len) - k0) * p.pairs;
+                const int k0 = w.split * t.k_len, steps = (min(t.k_blocks, k0 + t.k_len) - k0) * (SPLIT ? 6 : 1);
                 const uint32_t idesc = (1u << 4) | ((uint32_t)p.bf16 << 7) | ((uint32_t)p.bf16 << 10) | ((uint32_t)t.a_outer << 15) |
                                        ((uint32_t)t.b_outer << 16) | ((uint32_t)(t.bn >> 3) << 17) | ((uint32_t)(BM * CG >> 4) << 24);
                 const uint64_t a_step = t.a_outer ? 2048 >> 4 : 32 >> 4, b_step = t.b_outer ? 2048 >> 4 : 32 >> 4;
-                for (int n = w.n0; ok && n < w.n1; ++n, ++tile) {
-                    const uint32_t buf = tile & 1u, d = tmem + buf * BN;
-                    if (!mbar_wait(smem_u32(&ss->acc_empty[buf]), ((tile >> 1) & 1u) ^ 1u, abort_flag, limit)) { give_up(ss, p, WAIT_ACCUMULATOR); ok = false; break; }
-                    tc_fence_after();
-                    for (int k = 0; k < steps; ++k) {
-                        if (!mbar_wait(smem_u32(&ss->full[stage]), phase, abort_flag, limit)) { give_up(ss, p, WAIT_OPERANDS); ok = false; break; }
+                const int small = SPLIT ? steps / 6 * 5 : 0;
+                for (int n = w.n0; ok && n < w.n1; ++n) {
+                    // sums of the tile: all steps, or for fp32 the small pairs' and SUB_STAGES steps each of the big one's
+                    for (int k0s = 0; ok && k0s < steps; ++tile) {
+                        const int k1s = !SPLIT ? steps : k0s < small ? small : min(steps, k0s + SUB_STAGES);
+                        const uint32_t buf = tile & 1u, d = tmem + buf * BN;
+                        if (!mbar_wait(smem_u32(&ss->acc_empty[buf]), ((tile >> 1) & 1u) ^ 1u, abort_flag, limit)) { give_up(ss, p, WAIT_ACCUMULATOR); ok = false; break; }
                         tc_fence_after();
-                        const uint32_t a = ring + stage * C::STAGE_BYTES;
-                        const uint64_t ad = smem_desc(a, t.a_outer), bd = smem_desc(a + C::A_BYTES, t.b_outer);
+                        for (int k = k0s; k < k1s; ++k) {
+                            if (!mbar_wait(smem_u32(&ss->full[stage]), phase, abort_flag, limit)) { give_up(ss, p, WAIT_OPERANDS); ok = false; break; }
+                            tc_fence_after();
+                            const uint32_t a = ring + stage * C::STAGE_BYTES;
+                            const uint64_t ad = smem_desc(a, t.a_outer), bd = smem_desc(a + C::A_BYTES, t.b_outer);
 #pragma unroll
-                        for (int i = 0; i < BK / 16; ++i) umma<CG>(d, ad + i * a_step, bd + i * b_step, idesc, k > 0 || i > 0);
-                        umma_commit<CG>(smem_u32(&ss->empty[stage]));
-                        if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                            for (int i = 0; i < BK / 16; ++i) umma<CG>(d, ad + i * a_step, bd + i * b_step, idesc, k > k0s || i > 0);
+                            umma_commit<CG>(smem_u32(&ss->empty[stage]));
+                            if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                        }
+                        if (ok) umma_commit<CG>(smem_u32(&ss->acc_full[buf]));
+                        k0s = k1s;
                     }
-                    if (ok) umma_commit<CG>(smem_u32(&ss->acc_full[buf]));
                 }
             }
         }
@@ -372,6 +410,7 @@ template <int CG, int MODE> __global__ void __launch_bounds__(THREADS, 1) produc
     } else {
         const int quarter = warp & 3, half = warp >> 2;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const uint32_t box = ring + C::STAGES * C::STAGE_BYTES + warp * BOX_BYTES;
         uint32_t acc_empty[2];
         for (int i = 0; i < 2; ++i) {
             acc_empty[i] = smem_u32(&ss->acc_empty[i]);
@@ -379,10 +418,45 @@ template <int CG, int MODE> __global__ void __launch_bounds__(THREADS, 1) produc
         }
         uint32_t tile = 0;
         bool ok = true;
+        auto wait_tile = [&]() {
+            const uint32_t buf = tile & 1u;
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ss->acc_full[buf]), (tile >> 1) & 1u, abort_flag, limit));
+            if (!ok) give_up(ss, p, WAIT_TILE);
+            tc_fence_after();
+            return tmem + buf * BN + lanes;
+        };
+        auto release_tile = [&]() {
+            const uint32_t buf = tile & 1u;
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 2) mbar_arrive_cluster(acc_empty[buf]);
+                else mbar_arrive(acc_empty[buf]);
+            }
+            ++tile;
+        };
+        // 16 bytes of this lane's row of the box, swizzled as the store expects them
+        auto put = [&](int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+            st_shared16(box + lane * 128 + ((piece ^ (lane & 7)) << 4), a, b, c, d);
+        };
+        auto box_free = [&]() {
+            if (lane == 0) bulk_wait_read();
+            __syncwarp();
+        };
+        auto box_out = [&](const CUtensorMap *map, int x, int y, int z, bool add) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (add) tma_add(map, box, x, y, z); else tma_store(map, box, x, y, z);
+                bulk_commit();
+            }
+        };
         for (int u = first; ok && u < units; u += stride) {
             const Unit w = unit_at(p, u);
             const Task &t = p.task[w.task];
-            const int64_t row = (int64_t)(w.m * CG + (int)rank) * BM + quarter * 32 + lane;
+            const CUtensorMap *mc = &maps.c[w.task];
+            const int row0 = (w.m * CG + (int)rank) * BM + quarter * 32;
+            const int64_t row = row0 + lane;
             const bool in = row < t.M;
             [[maybe_unused]] float m = NEG_INF, s = 0.0f, factor = 0.0f, base = 0.0f, inv = 0.0f;
             [[maybe_unused]] int64_t label = -1;
@@ -399,24 +473,15 @@ template <int CG, int MODE> __global__ void __launch_bounds__(THREADS, 1) produc
                 }
                 if (label == p.ignore_index) label = -1;
             }
-            if constexpr (MODE == SUM) factor = t.out ? grad_alpha(p) * p.scale : 1.0f;
-            for (int n = w.n0; ok && n < w.n1; ++n, ++tile) {
-                const uint32_t buf = tile & 1u;
-                ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ss->acc_full[buf]), (tile >> 1) & 1u, abort_flag, limit));
-                if (!ok) { give_up(ss, p, WAIT_TILE); break; }
-                tc_fence_after();
+            if constexpr (MODE == SUM) factor = t.rounded ? grad_alpha(p) * p.scale : 1.0f;
+            for (int n = w.n0; ok && n < w.n1; ++n) {
                 const int64_t col0 = (int64_t)n * t.bn;
                 const int cols = (int)min((int64_t)t.bn, t.N - col0);          // of this tile
                 const int mine = (int)max((int64_t)-1, min((int64_t)BN, label - p.v0 - col0));    // label's column, if within
                 (void)mine;
-                for (int c = half * 32; c < cols; c += 64) {
-                    uint32_t r[32];
-                    tmem_ld32(tmem + buf * BN + lanes + c, r);
-                    tmem_ld_wait();
+                // 32 columns from c on, the first or second half of this warp's 64
+                auto use = [&](float (&v)[32], int c, int second) {
                     if constexpr (MODE == STATS) {
-                        float v[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
                         if (__any_sync(0xffffffffu, mine >= c && mine < c + 32)) {
                             float score = 0.0f;
 #pragma unroll
@@ -429,106 +494,137 @@ template <int CG, int MODE> __global__ void __launch_bounds__(THREADS, 1) produc
                         }
                         add_values<32>(m, s, v, LOG2E);
                     } else if constexpr (MODE == GRAD) {
-                        if (in && p.pairs == 1) {
-                            uint16_t *o = static_cast<uint16_t *>(p.G) + row * p.ldg + col0 + c;
+                        const bool has = __any_sync(0xffffffffu, mine >= c && mine < c + 32);
+                        if constexpr (!SPLIT) {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 8) {
-                                uint32_t q[4];
+                            for (int i = 0; i < 32; ++i) v[i] = exp2_approx(fmaf(v[i], LOG2E, -base)) * factor;
+                        } else {
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    const float g0 = exp2_approx(fmaf(__uint_as_float(r[i + 2 * j]), LOG2E, -base)) * factor;
-                                    const float g1 = exp2_approx(fmaf(__uint_as_float(r[i + 2 * j + 1]), LOG2E, -base)) * factor;
-                                    q[j] = factor == 0.0f ? 0u : pack2(g0, g1, p.bf16);
-                                }
-                                if (c + i < cols) *reinterpret_cast<uint4 *>(o + i) = make_uint4(q[0], q[1], q[2], q[3]);
-                            }
-                            if (mine >= c && mine < c + 32 && mine < cols)      // the label's own: written last, by the same thread
-                                store16(p.G, row * p.ldg + col0 + mine, factor * (exp2_approx((p.label_score[row] - m) * LOG2E) * inv - 1.0f), p.bf16);
-                        } else if (in) {
-                            uint16_t *o = static_cast<uint16_t *>(p.G) + row * p.ldg + col0 + c;
+                            for (int i = 0; i < 32; ++i) v[i] = exp2_approx((v[i] - m) * LOG2E) * inv * factor;
+                        }
+                        if (has) {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 8) {
-                                uint32_t q[3][4];
+                            for (int i = 0; i < 32; ++i) if (mine == c + i) v[i] -= factor;
+                        }
+                        if (factor == 0.0f) {
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) {
+                            for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+                        }
+                        if constexpr (!SPLIT) {
+                            if (!second) box_free();
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8)
+                                put(second * 4 + i / 8, pack2(v[i], v[i + 1], p.bf16), pack2(v[i + 2], v[i + 3], p.bf16), pack2(v[i + 4], v[i + 5], p.bf16),
+                                    pack2(v[i + 6], v[i + 7], p.bf16));
+                            if (second) box_out(mc, (int)col0 + c - 32, row0, 0, false);
+                        } else {
+                            // a plane of 64 columns at a time would keep all of them in registers: boxes of 32 columns here
+#pragma unroll
+                            for (int k = 0; k < 3; ++k) {
+                                uint32_t q[16];
+#pragma unroll
+                                for (int i = 0; i < 32; i += 2) {
                                     float a[2], b[2], d[2];
-#pragma unroll
-                                    for (int h = 0; h < 2; ++h) {
-                                        const int e = i + 2 * j + h;
-                                        float g = exp2_approx((__uint_as_float(r[e]) - m) * LOG2E) * inv - (mine == c + e ? 1.0f : 0.0f);
-                                        g = factor == 0.0f ? 0.0f : g * factor;
-                                        split3(g, a[h], b[h], d[h]);
-                                    }
-                                    q[0][j] = pack2(a[0], a[1], 1);
-                                    q[1][j] = pack2(b[0], b[1], 1);
-                                    q[2][j] = pack2(d[0], d[1], 1);
+                                    split3(v[i], a[0], b[0], d[0]);
+                                    split3(v[i + 1], a[1], b[1], d[1]);
+                                    q[i / 2] = k == 0 ? pack2(a[0], a[1], 1) : k == 1 ? pack2(b[0], b[1], 1) : pack2(d[0], d[1], 1);
                                 }
-                                if (c + i < cols) {
+                                box_free();
 #pragma unroll
-                                    for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4 *>(o + k * p.plane + i) = make_uint4(q[k][0], q[k][1], q[k][2], q[k][3]);
-                                }
+                                for (int j = 0; j < 4; ++j)      // lines of 64 bytes, not swizzled
+                                    st_shared16(box + lane * 64 + j * 16, q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
+                                box_out(mc, (int)col0 + c, row0, k, false);
                             }
                         }
-                    } else if (in) {
-                        if (t.out) {
-                            const int64_t at = row * t.ldo + col0 + c;
-                            const size_t es = t.out_dtype == GRWS_F32 ? 4 : 2;
-                            char *o = static_cast<char *>(t.out) + at * es;
-                            const bool vec = (reinterpret_cast<uintptr_t>(o) & 15u) == 0;
+                    } else {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 8) {
-                                float v[8];
+                        for (int i = 0; i < 32; ++i) v[i] *= factor;
+                        if (!SPLIT && t.rounded && t.out_dtype != GRWS_F32) {
+                            if (!second) box_free();
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[i + j]) * factor;
-                                if (t.out_dtype == GRWS_F32) {
-                                    float *f = reinterpret_cast<float *>(o) + i;
-                                    if (vec && c + i + 8 <= cols) {
-                                        *reinterpret_cast<float4 *>(f) = make_float4(v[0], v[1], v[2], v[3]);
-                                        *reinterpret_cast<float4 *>(f + 4) = make_float4(v[4], v[5], v[6], v[7]);
-                                    } else {
-#pragma unroll
-                                        for (int j = 0; j < 8; ++j) if (c + i + j < cols) f[j] = v[j];
-                                    }
-                                } else if (vec && c + i + 8 <= cols) {
-                                    *reinterpret_cast<uint4 *>(o + i * 2) = make_uint4(pack2(v[0], v[1], p.bf16), pack2(v[2], v[3], p.bf16),
-                                                                                        pack2(v[4], v[5], p.bf16), pack2(v[6], v[7], p.bf16));
-                                } else {
-#pragma unroll
-                                    for (int j = 0; j < 8; ++j) if (c + i + j < cols) store16(t.out, at + i + j, v[j], p.bf16);
-                                }
+                            for (int i = 0; i < 32; i += 8)
+                                put(second * 4 + i / 8, pack2(v[i], v[i + 1], p.bf16), pack2(v[i + 2], v[i + 3], p.bf16), pack2(v[i + 4], v[i + 5], p.bf16),
+                                    pack2(v[i + 6], v[i + 7], p.bf16));
+                            if (!second) return;
+                            if (!t.out) { box_out(mc, (int)col0 + c - 32, row0, 0, false); return; }
+                            __syncwarp();
+                            for (int r = 0; r < 32 && row0 + r < t.M; ++r) {
+                                const uint32_t two = ld_shared32(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                                uint16_t *o = static_cast<uint16_t *>(t.out) + (row0 + r) * t.ldo + col0 + c - 32 + lane * 2;
+                                if (c - 32 + lane * 2 < cols) o[0] = (uint16_t)two;
+                                if (c - 32 + lane * 2 + 1 < cols) o[1] = (uint16_t)(two >> 16);
                             }
+                            __syncwarp();
                         } else {
-                            float *f = t.sum + ((int64_t)w.split * t.M + row) * t.N + col0 + c;
-                            const bool vec = (reinterpret_cast<uintptr_t>(f) & 15u) == 0;
+                            box_free();
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4) {
-                                float4 v = make_float4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]), __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
-                                if (vec && c + i + 4 <= cols) {
-                                    if (t.add) {
-                                        const float4 q = *reinterpret_cast<const float4 *>(f + i);
-                                        v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
-                                    }
-                                    *reinterpret_cast<float4 *>(f + i) = v;
-                                } else {
-                                    const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j) if (c + i + j < cols) f[i + j] = t.add ? f[i + j] + e[j] : e[j];
-                                }
+                            for (int i = 0; i < 32; i += 4)
+                                put(i / 4, __float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]));
+                            if (!t.out) { box_out(mc, (int)col0 + c, row0, w.split, t.add); return; }
+                            __syncwarp();
+                            for (int r = 0; r < 32 && row0 + r < t.M; ++r) {
+                                const uint32_t one = ld_shared32(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                                if (c + lane < cols) static_cast<float *>(t.out)[(row0 + r) * t.ldo + col0 + c + lane] = __uint_as_float(one);
                             }
+                            __syncwarp();
                         }
                     }
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if constexpr (CG == 2) mbar_arrive_cluster(acc_empty[buf]);
-                    else mbar_arrive(acc_empty[buf]);
+                };
+                if constexpr (!SPLIT) {
+                    const uint32_t at = wait_tile();
+                    if (!ok) break;
+                    const int last = (cols - 1 - half * 64) >> 7;          // 64-column pieces of this warp, less one (-1: none)
+                    if (last < 0) release_tile();
+                    for (int k = 0; k <= last; ++k) {
+                        const int c = half * 64 + k * 128;
+                        float v[32];
+                        uint32_t r[32], r2[32];
+                        tmem_ld32(at + c, r);
+                        tmem_ld32(at + c + 32, r2);
+                        tmem_ld_wait();
+                        if (k == last) release_tile();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+                        use(v, c, 0);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r2[i]);
+                        use(v, c + 32, 1);
+                    }
+                } else {
+                    const int k0 = w.split * t.k_len, big = min(t.k_blocks, k0 + t.k_len) - k0;
+                    float acc[4][32];
+                    for (int sub = 0; ok && sub <= (big + SUB_STAGES - 1) / SUB_STAGES; ++sub) {
+                        const uint32_t at = wait_tile();
+                        if (!ok) break;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int c = half * 64 + (k >> 1) * 128 + (k & 1) * 32;
+                            if (c >= cols) continue;
+#pragma unroll
+                            for (int h = 0; h < 32; h += 16) {
+                                uint32_t r[16];
+                                tmem_ld16(at + c + h, r);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) acc[k][h + i] = sub ? acc[k][h + i] + __uint_as_float(r[i]) : __uint_as_float(r[i]);
+                            }
+                        }
+                        release_tile();
+                    }
+                    if (!ok) break;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int c = half * 64 + (k >> 1) * 128 + (k & 1) * 32;
+                        if (c < cols) use(acc[k], c, k & 1);
+                    }
                 }
             }
             if constexpr (MODE == STATS) {
                 if (ok && in) p.part[(int64_t)((w.n0 / t.run) * 2 + half) * t.M + row] = make_float2(m, s);
             }
         }
+        if (lane == 0) bulk_wait();
+        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
@@ -541,9 +637,10 @@ template <int CG, int MODE> __global__ void __launch_bounds__(THREADS, 1) produc
 // ---------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------
-// Map of a [planes][rows][cols] operand, cols contiguous, rows `ld` and planes `plane` elements apart; boxes of 64 columns
-// and `box` rows, 128-byte swizzle, zeros outside.
-inline int encode_map(CUtensorMap *map, const void *base, int bf16, int64_t cols, int64_t rows, int64_t ld, int planes, int64_t plane, int box) {
+// Map of a [planes][rows][cols] matrix, cols contiguous, rows `ld` and planes `plane` elements apart; boxes of `box_cols`
+// columns and `box_rows` rows, zeros outside; 128-byte swizzle where a box's line has 128 bytes.
+inline int encode_map(CUtensorMap *map, const void *base, int dtype, int64_t cols, int64_t rows, int64_t ld, int planes, int64_t plane, int box_cols,
+                      int box_rows) {
     typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                                  CUtensorMapFloatOOBfill);
@@ -555,37 +652,26 @@ inline int encode_map(CUtensorMap *map, const void *base, int bf16, int64_t cols
         return reinterpret_cast<EncodeFn>(fn);
     }();
     if (!encode) return fail(GRWS_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    const cuuint64_t es = dtype_bytes(dtype);
     const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
-    // (a single row or plane: any legal distance)
-    const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, planes > 1 ? (cuuint64_t)plane * 2 : (cuuint64_t)ld * 2};
-    const cuuint32_t boxes[3] = {64, (cuuint32_t)box, 1};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld * es, (cuuint64_t)(planes > 1 ? plane : ld) * es};
+    const cuuint32_t boxes[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
     const cuuint32_t estr[3] = {1, 1, 1};
-    const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims,
-                              strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    const CUtensorMapDataType type = dtype == GRWS_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == GRWS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                                                              : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const CUresult r = encode(map, type, 3, const_cast<void *>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              box_cols * es == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(GRWS_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
     return GRWS_OK;
 }
 
-template <int CG, int MODE> static int launch_product(const Maps &maps, const Params &p, cudaStream_t st) {
+template <int CG, int MODE, bool SPLIT> static int launch_product(const Maps &maps, const Params &p, cudaStream_t st) {
     int64_t units = 0;
     for (int i = 0; i < p.tasks; ++i) units += p.task[i].units();
     const int64_t clusters = units < sm_count() / CG ? units : sm_count() / CG;
-    GRWS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<CG, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<CG>::SMEM));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(clusters * CG));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = Cfg<CG>::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    GRWS_CUDA_TRY(cudaLaunchKernelEx(&cfg, product_kernel<CG, MODE>, maps, p));
-    return GRWS_OK;
+    GRWS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<CG, MODE, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<CG>::SMEM));
+    return launch_next(product_kernel<CG, MODE, SPLIT>, dim3((unsigned)(clusters * CG)), THREADS, Cfg<CG>::SMEM, st, CG, maps, p);
 }
 
 }  // namespace prod

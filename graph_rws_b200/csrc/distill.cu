@@ -151,6 +151,8 @@ template <typename T, int L> __device__ __forceinline__ float row_loss(const Arg
 
 // ---- rows of up to SHORT_ROW classes: L lanes a row, the losses of a block's rows summed ----
 template <typename T, int L> __global__ void __launch_bounds__(THREADS) short_fwd_kernel(const Args a) {
+    wait_for_previous();
+    let_next_start();
     __shared__ float red[64];
     const int lane = threadIdx.x % L;
     constexpr int ROWS = THREADS / L;
@@ -240,6 +242,8 @@ template <typename T> __device__ __forceinline__ bool same_offset(const T *in, c
 }
 
 template <typename T, int L> __global__ void __launch_bounds__(THREADS) short_bwd_kernel(const Args a) {
+    wait_for_previous();
+    let_next_start();
     constexpr int ROWS = THREADS / L;
     __shared__ int s_ids[ROWS][SHORT_KEPT];
     __shared__ float s_p[ROWS][SHORT_KEPT];
@@ -273,6 +277,8 @@ template <typename T, int L> __global__ void __launch_bounds__(THREADS) short_bw
 
 // ---- longer rows: a CTA per row, or per part of a row where there are few rows ----
 template <typename T> __global__ void __launch_bounds__(THREADS) long_fwd_kernel(const Args a) {
+    wait_for_previous();
+    let_next_start();
     __shared__ float red_m[THREADS / 32], red_s[THREADS / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float sum = 0.0f, count = 0.0f;
@@ -308,6 +314,8 @@ template <typename T> __global__ void __launch_bounds__(THREADS) long_fwd_kernel
 
 // joins the parts of the rows of long_fwd_kernel; a warp per row
 template <typename T> __global__ void __launch_bounds__(THREADS) join_fwd_kernel(const Args a) {
+    wait_for_previous();
+    let_next_start();
     __shared__ float red[64];
     const int lane = threadIdx.x & 31;
     float sum = 0.0f, count = 0.0f;
@@ -329,6 +337,8 @@ template <typename T> __global__ void __launch_bounds__(THREADS) join_fwd_kernel
 }
 
 template <typename T> __global__ void __launch_bounds__(THREADS) long_bwd_kernel(const Args a) {
+    wait_for_previous();
+    let_next_start();
     __shared__ int s_ids[MAX_KEPT];
     __shared__ float s_p[MAX_KEPT];
     const int64_t items = a.n * a.splits;
@@ -387,10 +397,7 @@ template <typename T, int L> static int launch_short(const Args &a, bool fwd, in
     int64_t g = ceil_div(a.n, (int64_t)(THREADS / L));
     if (g > grid_limit()) g = grid_limit();
     *grid = g;
-    if (fwd) short_fwd_kernel<T, L><<<(unsigned)g, THREADS, 0, st>>>(a);
-    else short_bwd_kernel<T, L><<<(unsigned)g, THREADS, 0, st>>>(a);
-    GRWS_CUDA_TRY(cudaGetLastError());
-    return GRWS_OK;
+    return launch_next(fwd ? short_fwd_kernel<T, L> : short_bwd_kernel<T, L>, dim3((unsigned)g), THREADS, 0, st, 1, a);
 }
 
 template <typename T> static int launch(Args a, bool fwd, float *loss, float *count, cudaStream_t st) {
@@ -407,19 +414,15 @@ template <typename T> static int launch(Args a, bool fwd, float *loss, float *co
     } else {
         split_rows(a.n, a.V, &a.splits, &a.part);
         grid = a.n * a.splits < grid_limit() ? a.n * a.splits : grid_limit();
-        if (fwd) long_fwd_kernel<T><<<(unsigned)grid, THREADS, 0, st>>>(a);
-        else long_bwd_kernel<T><<<(unsigned)grid, THREADS, 0, st>>>(a);
-        GRWS_CUDA_TRY(cudaGetLastError());
+        if (int rc = launch_next(fwd ? long_fwd_kernel<T> : long_bwd_kernel<T>, dim3((unsigned)grid), THREADS, 0, st, 1, a)) return rc;
         if (fwd && a.splits > 1) {
             grid = ceil_div(a.n, (int64_t)(THREADS / 32));
             if (grid > grid_limit()) grid = grid_limit();
-            join_fwd_kernel<T><<<(unsigned)grid, THREADS, 0, st>>>(a);
-            GRWS_CUDA_TRY(cudaGetLastError());
+            if (int rc = launch_next(join_fwd_kernel<T>, dim3((unsigned)grid), THREADS, 0, st, 1, a)) return rc;
         }
     }
     if (fwd && a.reduction != RED_NONE) {
-        loss_sum_kernel<<<1, 512, 0, st>>>(a.partial, (int)grid, a.reduction, loss, count);
-        GRWS_CUDA_TRY(cudaGetLastError());
+        if (int rc = launch_next(loss_sum_kernel, dim3(1), 512, 0, st, 1, a.partial, (int)grid, a.reduction, loss, count)) return rc;
     }
     return GRWS_OK;
 }

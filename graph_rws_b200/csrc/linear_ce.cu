@@ -24,7 +24,6 @@ struct Problem {
     int64_t n, d, V;
     int dtype, reduction;
     const float2 *state;                 // [n]: maximum, sum of exponentials
-    const float *label_score;            // [n], behind them
     const float *grad, *count;           // backward: gradient of the loss, number of counted rows
     const float *norm;                   // backward without a reduction: largest |gradient| of a row
     __host__ __device__ int64_t w_k() const { return class_major ? 1 : ldw; }
@@ -35,6 +34,8 @@ struct Problem {
 __global__ void __launch_bounds__(1024) grad_norm_kernel(const float *__restrict__ grad, int64_t n, float *__restrict__ norm) {
     __shared__ float red[32];
     float m = 0.0f;
+    wait_for_previous();
+    let_next_start();
     for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
         const float g = fabsf(grad[i]);
         if (g < INFINITY) m = fmaxf(m, g);
@@ -51,33 +52,60 @@ __global__ void __launch_bounds__(1024) grad_norm_kernel(const float *__restrict
     }
 }
 
-// Joins the parts of the rows' statistics in order and takes the rows' losses; a thread per row.
+// Joins the parts of the rows' statistics and takes the rows' losses: 32 rows a block, 8 threads a row, in a fixed order.  The
+// block that is done last adds the blocks' sums up; `done` was set to 0 by the kernel before.
+constexpr int ROWS_PER_BLOCK = 32;
 __global__ void __launch_bounds__(256) rows_kernel(const Problem p, const float2 *__restrict__ part, int parts, const float *__restrict__ label_score,
                                                    float2 *__restrict__ state, float *__restrict__ loss, float *__restrict__ count,
-                                                   float2 *__restrict__ partial) {
+                                                   float2 *__restrict__ partial, int *__restrict__ done) {
     __shared__ float red[64];
-    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    float l = 0.0f, counted = 0.0f;
+    __shared__ float2 joined[8][ROWS_PER_BLOCK];
+    __shared__ bool last;
+    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+    const int64_t row = (int64_t)blockIdx.x * ROWS_PER_BLOCK + lane;
+    float l = 0.0f, counted = 0.0f, m = NEG_INF, s = 0.0f, score = 0.0f;
+    int64_t label = -1;
+    wait_for_previous();
     if (row < p.n) {
-        float m = NEG_INF, s = 0.0f;
-        for (int i = 0; i < parts; ++i) {
+        if (group == 0) {
+            label = load_index(p.labels, p.label_bytes, row);
+            score = label_score[row];          // (nothing was written there for a label that is no class)
+        }
+#pragma unroll 4
+        for (int i = group; i < parts; i += 8) {
             const float2 q = part[(int64_t)i * p.n + row];
             join_stats(m, s, q.x, q.y, LOG2E);
         }
+    }
+    joined[group][lane] = make_float2(m, s);
+    __syncthreads();
+    if (group == 0 && row < p.n) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) join_stats(m, s, joined[i][lane].x, joined[i][lane].y, LOG2E);
         state[row] = make_float2(m, s);
-        const int64_t label = load_index(p.labels, p.label_bytes, row);
         if (label != p.ignore_index) {
-            l = label >= 0 && label < p.V ? logf(s) - (label_score[row] - m) : NAN;
+            l = label >= 0 && label < p.V ? logf(s) - (score - m) : NAN;
             counted = 1.0f;
         }
         if (p.reduction == RED_NONE) loss[row] = l;
     }
     if (p.reduction == RED_NONE) return;
-    block_sum2(l, counted, red);
-    if (threadIdx.x == 0) {
-        if (gridDim.x == 1) finish_loss(l, counted, p.reduction, loss, count);
-        else partial[blockIdx.x] = make_float2(l, counted);
+    if (group == 0) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) { l += __shfl_xor_sync(0xffffffffu, l, o); counted += __shfl_xor_sync(0xffffffffu, counted, o); }
+        if (lane == 0) {
+            partial[blockIdx.x] = make_float2(l, counted);
+            __threadfence();
+            last = atomicAdd(done, 1) == (int)gridDim.x - 1;
+        }
     }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    l = counted = 0.0f;
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) { const float2 q = __ldcg(partial + i); l += q.x; counted += q.y; }
+    block_sum2(l, counted, red);
+    if (threadIdx.x == 0) finish_loss(l, counted, p.reduction, loss, count);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -121,8 +149,12 @@ __device__ __forceinline__ void tile_product(const TA *A, int64_t am, int64_t ak
 }
 
 // statistics of 64 rows over the class tiles blockIdx.y, + gridDim.y, ...
-template <typename T> __global__ void __launch_bounds__(256) plain_stats_kernel(const Problem p, float2 *__restrict__ part, float *__restrict__ label_score) {
+template <typename T> __global__ void __launch_bounds__(256) plain_stats_kernel(const Problem p, float2 *__restrict__ part, float *__restrict__ label_score,
+                                                                               int *__restrict__ done) {
     __shared__ __align__(16) Tiles t;
+    wait_for_previous();
+    let_next_start();
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *done = 0;
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
     const int64_t m0 = (int64_t)blockIdx.x * TM;
     float m[4], s[4], acc[4][4];
@@ -163,6 +195,8 @@ template <typename T> __global__ void __launch_bounds__(256) plain_grad_kernel(c
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
     const int64_t m0 = (int64_t)blockIdx.x * TM, n0 = (int64_t)blockIdx.y * TN;
     float acc[4][4];
+    wait_for_previous();
+    let_next_start();
     tile_product(static_cast<const T *>(p.x), p.ldx, (int64_t)1, static_cast<const T *>(p.w) + v0 * p.w_v(), p.w_k(), p.w_v(), p.n, cols, m0, n0, 0, p.d, t, acc);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -182,37 +216,79 @@ template <typename T> __global__ void __launch_bounds__(256) plain_grad_kernel(c
     }
 }
 
-// part blockIdx.z of the product A [M, K] B [K, N] into (or onto) its own plane of fp32 partial sums [parts][M][N]
-template <typename TA, typename TB>
-__global__ void __launch_bounds__(256) plain_product_kernel(const TA *A, int64_t am, int64_t ak, const TB *B, int64_t bk, int64_t bn, int64_t M, int64_t N,
-                                                            int64_t K, int64_t k_part, float *__restrict__ out, int add) {
+// A product A [M, K] B [K, N] in parts of K: element strides, tiles, and its plane of fp32 partial sums [parts][M][N], or (one
+// part) the output itself at m * om + n * on
+struct PlainTask {
+    const void *a, *b;
+    int64_t am, ak, bk, bn, M, N, K, k_part;
+    int m_tiles, n_tiles, parts, add;
+    float *sum;
+    void *out;
+    int64_t om, on;
+    __host__ __device__ int blocks() const { return m_tiles * n_tiles * parts; }
+};
+
+// dx = G w^T (task 0) and dw = x^T G (task 1) of one piece
+template <typename T> __global__ void __launch_bounds__(256) plain_products_kernel(const Problem p, const PlainTask dx, const PlainTask dw) {
     __shared__ __align__(16) Tiles t;
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    const int64_t m0 = (int64_t)blockIdx.x * TM, n0 = (int64_t)blockIdx.y * TN, k0 = (int64_t)blockIdx.z * k_part;
+    wait_for_previous();
+    let_next_start();
+    int i = blockIdx.x;
+    const bool second = i >= dx.blocks();
+    const PlainTask &q = second ? dw : dx;
+    if (second) i -= dx.blocks();
+    const int part = i / (q.m_tiles * q.n_tiles), tile = i - part * (q.m_tiles * q.n_tiles);
+    const int64_t m0 = (int64_t)(tile % q.m_tiles) * TM, n0 = (int64_t)(tile / q.m_tiles) * TN, k0 = part * q.k_part, k1 = min(q.K, k0 + q.k_part);
     float acc[4][4];
-    tile_product(A, am, ak, B, bk, bn, M, N, m0, n0, k0, min(K, k0 + k_part), t, acc);
-    out += (int64_t)blockIdx.z * M * N;
+    if (second) tile_product(static_cast<const T *>(q.a), q.am, q.ak, static_cast<const float *>(q.b), q.bk, q.bn, q.M, q.N, m0, n0, k0, k1, t, acc);
+    else tile_product(static_cast<const float *>(q.a), q.am, q.ak, static_cast<const T *>(q.b), q.bk, q.bn, q.M, q.N, m0, n0, k0, k1, t, acc);
+    const float alpha = q.out ? prod::grad_alpha(p) : 1.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int a = 0; a < 4; ++a)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (m >= M || n >= N) continue;
-            float *o = out + m * N + n;
-            *o = add ? *o + acc[i][j] : acc[i][j];
+        for (int b = 0; b < 4; ++b) {
+            const int64_t m = m0 + ty * 4 + a, n = n0 + tx * 4 + b;
+            if (m >= q.M || n >= q.N) continue;
+            if (q.out) {
+                static_cast<T *>(q.out)[m * q.om + n * q.on] = from_float<T>(acc[a][b] * alpha);
+            } else {
+                float *o = q.sum + ((int64_t)part * q.M + m) * q.N + n;
+                *o = q.add ? *o + acc[a][b] : acc[a][b];
+            }
         }
 }
 
-// out(m, n) = alpha * sum of the partial planes in order, rounded once to the output's type; out(m, n) at m * om + n * on
+// out(m, n) = alpha * sum of the partial planes [parts][M][ldp] in order, rounded once to the output's type; out(m, n) at
+// m * om + n * on.  Four columns a thread.
 template <typename T> __global__ void __launch_bounds__(256) round_kernel(const Problem p, const float *__restrict__ part, int parts, int64_t M, int64_t N,
-                                                                          float scale, T *__restrict__ out, int64_t om, int64_t on) {
+                                                                          int64_t ldp, float scale, T *__restrict__ out, int64_t om, int64_t on) {
+    wait_for_previous();
+    let_next_start();
     const float alpha = prod::grad_alpha(p) * scale;
-    const int64_t total = M * N;
+    const int64_t per_row = (N + 3) / 4, total = M * per_row, plane = M * ldp;
+    const bool vector = on == 1 && om % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0 && ldp % 4 == 0;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        float s = 0.0f;
-        for (int k = 0; k < parts; ++k) s += part[k * total + i];
-        const int64_t m = i / N, n = i - m * N;
-        out[m * om + n * on] = from_float<T>(s * alpha);
+        const int64_t m = total <= UINT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row, n = (i - m * per_row) * 4;
+        const float *q = part + m * ldp + n;
+        T *o = out + m * om + n * on;
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (vector && n + 4 <= N) {
+            for (int k = 0; k < parts; ++k) {
+                const float4 v = *reinterpret_cast<const float4 *>(q + k * plane);
+                s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+            }
+            T r[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = from_float<T>(s[j] * alpha);
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(o) = *reinterpret_cast<const uint4 *>(r);
+            else *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<const uint2 *>(r);
+        } else {
+            for (int j = 0; j < 4 && n + j < N; ++j) {
+                for (int k = 0; k < parts; ++k) s[j] += q[k * plane + j];
+                o[j * on] = from_float<T>(s[j] * alpha);
+            }
+        }
     }
 }
 
@@ -221,6 +297,8 @@ template <typename T> __global__ void __launch_bounds__(256) round_kernel(const 
 template <typename T> __global__ void __launch_bounds__(256) pack_kernel(const T *__restrict__ src, int64_t ld, int64_t rows, int64_t cols,
                                                                          uint16_t *__restrict__ dst, int64_t ldp, int64_t plane) {
     const int64_t per_row = ldp / 8, total = rows * per_row;
+    wait_for_previous();
+    let_next_start();
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t row = i / per_row, c = (i - row * per_row) * 8;
         const T *s = src + row * ld + c;
@@ -257,19 +335,19 @@ static __device__ int g_status;
 // ---------------------------------------------------------------------------------------------
 // plan: how a call is cut up, and where its workspace lies
 // ---------------------------------------------------------------------------------------------
-constexpr size_t PIECE_BYTES = 256ull << 20;       // workspace for G
+constexpr size_t PIECE_BYTES = 512ull << 20;       // workspace for G
 constexpr double TENSOR_PRODUCTS = 1 << 22;        // n d V from which the tensor cores take the call
 
 struct Plan {
     bool tensor;
     int planes;                                    // of an operand: 1, or 3 of bf16 for fp32
     bool pack_x, pack_w;
-    int64_t ldx, ldw, ldg;                         // rows of the operands as the tensor cores read them
+    int64_t ldx, ldw, ldg, ld_dx, ld_dw;           // rows of the operands as the tensor cores read them, of fp32 sums
     int64_t run, parts;                            // forward: class tiles per unit, parts of the class axis
     int64_t piece;                                 // backward: classes per piece
     int64_t dx_parts, dx_len, dw_parts, dw_len;    // parts of the two products' inner axes (classes of a piece, rows)
     size_t x, w;                                   // packed operands
-    size_t stats, partial;                         // forward scratch
+    size_t stats, label_score, partial, done;      // forward scratch
     size_t norm, G, dx_sum, dw_sum;                // backward scratch
     size_t bytes;
 };
@@ -278,6 +356,11 @@ static size_t place(size_t &at, size_t bytes) {
     const size_t here = at;
     at += (bytes + 255) & ~(size_t)255;
     return here;
+}
+static void place_rows(size_t &at, int64_t n, Plan *q) {
+    q->label_score = place(at, (size_t)n * sizeof(float));
+    q->partial = place(at, (size_t)ceil_div(n, (int64_t)ROWS_PER_BLOCK) * sizeof(float2));
+    q->done = place(at, sizeof(int));
 }
 // parts of an inner axis of K so that `tiles` output tiles give every SM two blocks; none shorter than `least`
 static void cut(int64_t tiles, int64_t K, int64_t least, int64_t unit, int64_t *parts, int64_t *len) {
@@ -297,39 +380,43 @@ static int cta_group(int64_t M) { return M > prod::BM ? 2 : 1; }
 
 static bool needs_packing(const void *p, int64_t ld, int dtype) { return dtype == GRWS_F32 || !aligned16(p) || ld % 8 != 0; }
 
-// Class tiles that one unit of the forward pass takes: as many as leave the SMs equally busy to a few per cent
-static void cut_runs(int64_t m_tiles, int64_t n_tiles, int64_t ctas, int64_t *run, int64_t *runs) {
+// Class tiles that one unit of the forward pass takes: as many as leave the SMs equally busy; every part is a statistic per
+// row (of two warps each) written and read at some 5 TB/s, a tile step takes about 0.4 us
+static void cut_runs(int64_t n, int64_t m_tiles, int64_t n_tiles, int64_t steps, int64_t ctas, int64_t *run, int64_t *runs) {
     int64_t best = 1;
-    double best_cost = 1e300;
+    double best_us = 1e300;
     for (int64_t r = 1; r <= n_tiles && r <= 64; ++r) {
         const int64_t k = ceil_div(n_tiles, r);
-        const double cost = (double)ceil_div(m_tiles * k, ctas) * (double)r + 0.05 * (double)k;      // a part costs a write and a read per row
-        if (cost <= best_cost) { best_cost = cost; best = r; }
+        const double us = (double)(ceil_div(m_tiles * k, ctas) * r * steps) * 0.4 + (double)(k * n) * 32.0 / 5.0e6;
+        if (us <= best_us) { best_us = us; best = r; }
     }
     *run = best;
     *runs = ceil_div(n_tiles, best);
 }
 
 // Parts of the inner axes of dx (classes of a piece) and dw (rows), which run in one launch: a unit should be short against the
-// launch, since units are dealt out round robin, but every part is one more plane of fp32 sums through memory.  In units of one
-// 64-element step of one tile: about 0.4 us of a pair of SMs.
-static void cut_products(int64_t tiles0, int64_t k0, double sums0, int64_t tiles1, int64_t k1, double sums1, int64_t ctas, int64_t *parts0, int64_t *parts1) {
-    static const int64_t tries[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128};
+// launch, since units are dealt out round robin, but every part is one more plane of fp32 sums through memory.  Costs are in
+// units of one 64-element step of one tile, about 0.4 us of a pair of SMs; a launch that adds planes up takes some 3 us.
+static double cut_products(int64_t tiles0, int64_t k0, double sums0, int64_t tiles1, int64_t k1, double sums1, int64_t ctas, int64_t *parts0, int64_t *parts1) {
+    static const int64_t tries[] = {1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 12, 14, 16, 18, 20, 24, 28, 32, 37, 48, 64, 74, 96, 128, 148};
+    const double step_us = 0.4, plane_us = 8.0 / 5.0e6;          // an fp32 number written and read at 5 TB/s
     double best = 1e300;
     for (int64_t a : tries) {
-        if (a > 1 && k0 / a < 8) break;
+        if (a > 1 && (k0 / a < 8 || tiles0 * a > 6 * ctas)) break;
         for (int64_t b : tries) {
-            if (b > 1 && k1 / b < 8) break;
-            const int64_t l0 = ceil_div(k0, a), l1 = ceil_div(k1, b), units = tiles0 * a + tiles1 * b;
-            const double all = (double)(tiles0 * k0 + tiles1 * k1) / (double)ctas;
-            const double longest = (double)(l0 > l1 ? l0 : l1);
-            const double rounds = (double)ceil_div(units, ctas) * ((double)(tiles0 * k0 + tiles1 * k1) / (double)units);
-            double cost = rounds > all ? rounds : all;
-            if (cost < longest) cost = longest;
-            cost += ((a > 1 ? (double)a * sums0 : 0.0) + (b > 1 ? (double)b * sums1 : 0.0)) * 8.0 / 6.0e12 / 0.4e-6;
+            if (b > 1 && (k1 / b < 8 || tiles1 * b > 6 * ctas)) break;
+            const int64_t l0 = ceil_div(k0, a), l1 = ceil_div(k1, b), u0 = tiles0 * a, u1 = tiles1 * b;
+            // the longer units go out first; whoever has finished its share of them starts on the others
+            const bool first1 = l1 >= l0;
+            const int64_t ua = first1 ? u1 : u0, la = first1 ? l1 : l0, lb = first1 ? l0 : l1, both = u0 + u1;
+            const int64_t rounds = ceil_div(both, ctas), long_rounds = ceil_div(ua, ctas);
+            double cost = (double)(long_rounds * la + (rounds - long_rounds) * lb);
+            if (a > 1) cost += (3.0 + (double)a * sums0 * plane_us) / step_us;
+            if (b > 1) cost += (3.0 + (double)b * sums1 * plane_us) / step_us;
             if (cost < best) { best = cost; *parts0 = a; *parts1 = b; }
         }
     }
+    return best;
 }
 
 static Plan make_plan(const Problem &p, bool backward) {
@@ -343,7 +430,7 @@ static Plan make_plan(const Problem &p, bool backward) {
             q.parts = ceil_div((int64_t)sm_count() * 2, row_tiles > 0 ? row_tiles : 1);
             if (q.parts > class_tiles) q.parts = class_tiles;
             q.stats = place(at, (size_t)q.parts * n * sizeof(float2));
-            q.partial = place(at, (size_t)ceil_div(n, (int64_t)256) * sizeof(float2));
+            place_rows(at, n, &q);
         } else {
             q.piece = (int64_t)(PIECE_BYTES / sizeof(float)) / (n > 0 ? n : 1) / TN * TN;
             if (q.piece < TN) q.piece = TN;
@@ -370,72 +457,79 @@ static Plan make_plan(const Problem &p, bool backward) {
     const int cg = cta_group(n);
     if (!backward) {
         const int64_t bn = columns_per_tile(V, cg);
-        cut_runs(ceil_div(n, (int64_t)(prod::BM * cg)), ceil_div(V, bn), sm_count() / cg, &q.run, &q.parts);
+        cut_runs(n, ceil_div(n, (int64_t)(prod::BM * cg)), ceil_div(V, bn), ceil_div(d, (int64_t)prod::BK) * (q.planes == 3 ? 6 : 1), sm_count() / cg, &q.run, &q.parts);
         q.stats = place(at, (size_t)q.parts * 2 * n * sizeof(float2));
-        q.partial = place(at, (size_t)ceil_div(n, (int64_t)256) * sizeof(float2));
+        place_rows(at, n, &q);
     } else {
-        q.piece = (int64_t)(PIECE_BYTES / (2 * q.planes)) / n / prod::BN * prod::BN;
-        if (q.piece < prod::BN) q.piece = prod::BN;
-        if (q.piece > V) q.piece = V;
-        q.ldg = ceil_div(q.piece, (int64_t)8) * 8;
+        int64_t most = (int64_t)(PIECE_BYTES / (2 * q.planes)) / n / prod::BN * prod::BN;
+        if (most < prod::BN) most = prod::BN;
         const int pg = cta_group(n > d ? n : d);
-        const int64_t rows0 = n, cols0 = d, rows1 = p.class_major ? q.piece : d, cols1 = p.class_major ? d : q.piece;
-        const int64_t tiles0 = ceil_div(rows0, (int64_t)(prod::BM * pg)) * ceil_div(cols0, (int64_t)columns_per_tile(cols0, pg));
-        const int64_t tiles1 = ceil_div(rows1, (int64_t)(prod::BM * pg)) * ceil_div(cols1, (int64_t)columns_per_tile(cols1, pg));
-        const int64_t k0 = ceil_div(q.piece, (int64_t)prod::BK), k1 = ceil_div(n, (int64_t)prod::BK);
-        cut_products(tiles0, k0, (double)rows0 * cols0, tiles1, k1, (double)rows1 * cols1, sm_count() / pg, &q.dx_parts, &q.dw_parts);
+        const int64_t k1 = ceil_div(n, (int64_t)prod::BK);
+        double best = 1e300;
+        // the largest piece, or one down to half of it whose products leave the SMs more equally busy
+        const int64_t all = ceil_div(V, (int64_t)prod::BN) * prod::BN, top = most < all ? most : all;
+        for (int64_t k = 8; k >= 4; --k) {
+            const int64_t piece = ceil_div(top * k / 8, (int64_t)prod::BN) * prod::BN;
+            const int64_t c = piece < V ? piece : V;
+            const int64_t rows1 = p.class_major ? c : d, cols1 = p.class_major ? d : c;
+            const int64_t tiles0 = ceil_div(n, (int64_t)(prod::BM * pg)) * ceil_div(d, (int64_t)columns_per_tile(d, pg));
+            const int64_t tiles1 = ceil_div(rows1, (int64_t)(prod::BM * pg)) * ceil_div(cols1, (int64_t)columns_per_tile(cols1, pg));
+            int64_t a, b;
+            const double cost = (cut_products(tiles0, ceil_div(c, (int64_t)prod::BK), (double)n * d, tiles1, k1, (double)d * c, sm_count() / pg, &a, &b) +
+                                 (c < V ? (double)n * d * 8.0 / 5.0e6 / 0.4 : 0.0)) * (double)ceil_div(V, c);
+            if (cost < best) { best = cost; q.piece = c; q.dx_parts = a; q.dw_parts = b; }
+        }
+        q.ldg = ceil_div(q.piece, (int64_t)8) * 8;
+        const int64_t k0 = ceil_div(q.piece, (int64_t)prod::BK);
         q.dx_len = ceil_div(k0, q.dx_parts);
         q.dx_parts = ceil_div(k0, q.dx_len);
         q.dw_len = ceil_div(k1, q.dw_parts);
         q.dw_parts = ceil_div(k1, q.dw_len);
+        q.ld_dx = ceil_div(d, (int64_t)4) * 4;
+        q.ld_dw = ceil_div(p.class_major ? d : q.piece, (int64_t)4) * 4;
         q.norm = place(at, sizeof(float));
         q.G = place(at, (size_t)q.planes * n * q.ldg * 2);
-        if (q.dx_parts > 1 || q.piece < V) q.dx_sum = place(at, (size_t)q.dx_parts * n * d * sizeof(float));
-        if (q.dw_parts > 1) q.dw_sum = place(at, (size_t)q.dw_parts * d * q.piece * sizeof(float));
+        if (q.dx_parts > 1 || q.piece < V) q.dx_sum = place(at, (size_t)q.dx_parts * n * q.ld_dx * sizeof(float));
+        if (q.dw_parts > 1) q.dw_sum = place(at, (size_t)q.dw_parts * (p.class_major ? q.piece : d) * q.ld_dw * sizeof(float));
     }
     q.bytes = at;
     return q;
 }
 
-template <typename T> static int launch_round(const Problem &p, const float *part, int64_t parts, int64_t M, int64_t N, float scale, void *out, int64_t om,
+template <typename T> static int launch_round(const Problem &p, const float *part, int64_t parts, int64_t M, int64_t N, int64_t ldp, float scale, void *out, int64_t om,
                                               int64_t on, cudaStream_t st) {
-    int64_t g = ceil_div(M * N, (int64_t)256);
+    int64_t g = ceil_div(M * ceil_div(N, (int64_t)4), (int64_t)256);
     const int64_t most = (int64_t)sm_count() * 8;
     if (g > most) g = most;
-    round_kernel<T><<<(unsigned)g, 256, 0, st>>>(p, part, (int)parts, M, N, scale, static_cast<T *>(out), om, on);
-    GRWS_CUDA_TRY(cudaGetLastError());
-    return GRWS_OK;
+    return launch_next(round_kernel<T>, dim3((unsigned)g), 256, 0, st, 1, p, part, (int)parts, M, N, ldp, scale, static_cast<T *>(out), om, on);
 }
 
 // ---- the tensor cores' way ----
-struct Operands { const void *x, *w; int64_t ldx, ldw, x_plane, w_plane, w_rows, w_cols; };
+// an operand as it lies in memory: [planes][rows][cols], cols contiguous
+struct View { const void *p; int64_t rows, cols, ld, plane; int planes; };
+struct Operands { View x, w; int dtype; };
 
 template <typename T> static int launch_pack(const void *src, int64_t ld, int64_t rows, int64_t cols, void *dst, int64_t ldp, cudaStream_t st) {
     int64_t g = ceil_div(rows * (ldp / 8), (int64_t)256);
     const int64_t most = (int64_t)sm_count() * 8;
     if (g > most) g = most;
-    pack_kernel<T><<<(unsigned)g, 256, 0, st>>>(static_cast<const T *>(src), ld, rows, cols, static_cast<uint16_t *>(dst), ldp, rows * ldp);
-    GRWS_CUDA_TRY(cudaGetLastError());
-    return GRWS_OK;
+    return launch_next(pack_kernel<T>, dim3((unsigned)g), 256, 0, st, 1, static_cast<const T *>(src), ld, rows, cols, static_cast<uint16_t *>(dst), ldp,
+                       rows * ldp);
 }
 
 template <typename T> static int pack_operands(const Problem &p, const Plan &q, char *scratch, Operands *o, cudaStream_t st) {
-    o->w_rows = p.class_major ? p.V : p.d;
-    o->w_cols = p.class_major ? p.d : p.V;
-    o->x = q.pack_x ? scratch + q.x : p.x;
-    o->w = q.pack_w ? scratch + q.w : p.w;
-    o->ldx = q.ldx; o->ldw = q.ldw;
-    o->x_plane = p.n * q.ldx;
-    o->w_plane = o->w_rows * q.ldw;
+    const int64_t w_rows = p.class_major ? p.V : p.d, w_cols = p.class_major ? p.d : p.V;
+    o->x = View{q.pack_x ? scratch + q.x : p.x, p.n, p.d, q.ldx, p.n * q.ldx, q.planes};
+    o->w = View{q.pack_w ? scratch + q.w : p.w, w_rows, w_cols, q.ldw, w_rows * q.ldw, q.planes};
+    o->dtype = p.dtype == GRWS_F16 ? GRWS_F16 : GRWS_BF16;
     if (q.pack_x) if (int rc = launch_pack<T>(p.x, p.ldx, p.n, p.d, scratch + q.x, q.ldx, st)) return rc;
-    if (q.pack_w) if (int rc = launch_pack<T>(p.w, p.ldw, o->w_rows, o->w_cols, scratch + q.w, q.ldw, st)) return rc;
+    if (q.pack_w) if (int rc = launch_pack<T>(p.w, p.ldw, w_rows, w_cols, scratch + q.w, q.ldw, st)) return rc;
     return GRWS_OK;
 }
 
-// sets a product up: its tile counts, and the maps of its operands ([rows][cols] in memory, cols contiguous)
-static int set_task(prod::Task *t, CUtensorMap *ma, CUtensorMap *mb, int cg, int bf16, int planes, const void *a, int64_t a_rows, int64_t a_cols, int64_t lda,
-                    int64_t a_plane, int a_outer, const void *b, int64_t b_rows, int64_t b_cols, int64_t ldb, int64_t b_plane, int b_outer, int64_t M, int64_t N,
-                    int64_t K) {
+// sets a product up: its tile counts and the maps of its operands; `outer`: the operand's rows are the inner axis
+static int set_task(prod::Task *t, CUtensorMap *ma, CUtensorMap *mb, int cg, int dtype, const View &a, int a_outer, const View &b, int b_outer, int64_t M,
+                    int64_t N, int64_t K) {
     t->M = M; t->N = N;
     t->bn = columns_per_tile(N, cg);
     t->m_tiles = (int)ceil_div(M, (int64_t)(prod::BM * cg));
@@ -444,16 +538,32 @@ static int set_task(prod::Task *t, CUtensorMap *ma, CUtensorMap *mb, int cg, int
     t->k_blocks = t->k_len = (int)ceil_div(K, (int64_t)prod::BK);
     t->group = t->m_tiles < 16 ? t->m_tiles : 16;
     t->a_outer = a_outer; t->b_outer = b_outer;
-    if (int rc = prod::encode_map(ma, a, bf16, a_cols, a_rows, lda, planes, a_plane, a_outer ? prod::BK : prod::BM)) return rc;
-    return prod::encode_map(mb, b, bf16, b_cols, b_rows, ldb, planes, b_plane, b_outer ? prod::BK : prod::BN / cg);
+    if (int rc = prod::encode_map(ma, a.p, dtype, a.cols, a.rows, a.ld, a.planes, a.plane, 64, a_outer ? prod::BK : prod::BM)) return rc;
+    return prod::encode_map(mb, b.p, dtype, b.cols, b.rows, b.ld, b.planes, b.plane, 64, b_outer ? prod::BK : prod::BN / cg);
 }
 
-static int product_params(const Problem &p, const Plan &q, prod::Params *r) {
+// where a SUM task's results go: planes of fp32 sums, or the rounded output
+static int set_sums(prod::Task *t, CUtensorMap *mc, int64_t parts, float *sum, int64_t ld, bool add) {
+    t->splits = (int)parts;
+    t->add = add;
+    return prod::encode_map(mc, sum, GRWS_F32, t->N, t->M, ld, (int)parts, t->M * ld, 32, 32);
+}
+static int set_rounded(prod::Task *t, CUtensorMap *mc, int dtype, void *out, int64_t ldo) {
+    t->rounded = 1;
+    t->out_dtype = dtype;
+    if (!aligned16(out) || ldo * (int64_t)dtype_bytes(dtype) % 16 != 0) {         // no TMA store starts at such rows
+        t->out = out;
+        t->ldo = ldo;
+        return GRWS_OK;
+    }
+    return prod::encode_map(mc, out, dtype, t->N, t->M, ldo, 1, 0, dtype == GRWS_F32 ? 32 : 64, 32);
+}
+
+static int product_params(const Problem &p, prod::Params *r) {
     void *status = nullptr;
     GRWS_CUDA_TRY(cudaGetSymbolAddress(&status, g_status));
     *r = prod::Params{};
     r->tasks = 1;
-    r->pairs = q.planes == 3 ? 6 : 1;
     r->bf16 = p.dtype != GRWS_F16;
     r->labels = p.labels; r->label_bytes = p.label_bytes; r->ignore_index = p.ignore_index; r->V = p.V;
     r->reduction = p.reduction; r->grad = p.grad; r->count = p.count; r->norm = p.norm;
@@ -464,24 +574,25 @@ static int product_params(const Problem &p, const Plan &q, prod::Params *r) {
     return GRWS_OK;
 }
 
-template <int MODE> static int launch_grouped(int cg, const prod::Maps &maps, const prod::Params &r, cudaStream_t st) {
-    return cg == 2 ? prod::launch_product<2, MODE>(maps, r, st) : prod::launch_product<1, MODE>(maps, r, st);
+template <int MODE> static int launch_product(int cg, int planes, const prod::Maps &maps, const prod::Params &r, cudaStream_t st) {
+    if (planes == 3) return cg == 2 ? prod::launch_product<2, MODE, true>(maps, r, st) : prod::launch_product<1, MODE, true>(maps, r, st);
+    return cg == 2 ? prod::launch_product<2, MODE, false>(maps, r, st) : prod::launch_product<1, MODE, false>(maps, r, st);
 }
 
-template <typename T> static int tensor_forward(const Problem &p, const Plan &q, float2 *part, float *label_score, char *scratch, cudaStream_t st) {
+template <typename T> static int tensor_forward(const Problem &p, const Plan &q, float2 *part, float *label_score, int *done, char *scratch, cudaStream_t st) {
     Operands o;
     if (int rc = pack_operands<T>(p, q, scratch, &o, st)) return rc;
     prod::Params r;
-    if (int rc = product_params(p, q, &r)) return rc;
+    if (int rc = product_params(p, &r)) return rc;
     prod::Maps maps;
     const int cg = cta_group(p.n);
-    if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, r.bf16, q.planes, o.x, p.n, p.d, o.ldx, o.x_plane, 0, o.w, o.w_rows, o.w_cols, o.ldw, o.w_plane,
-                          !p.class_major, p.n, p.V, p.d)) return rc;
+    if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, o.dtype, o.x, 0, o.w, !p.class_major, p.n, p.V, p.d)) return rc;
     r.task[0].run = (int)q.run;
     r.task[0].runs = (int)q.parts;
     r.part = part;
     r.label_score = label_score;
-    return launch_grouped<prod::STATS>(cg, maps, r, st);
+    r.done = done;
+    return launch_product<prod::STATS>(cg, q.planes, maps, r, st);
 }
 
 // G in fp16 is held as 2^12 G: |G| <= 1, and a probability of 2^-26 is still a normal number
@@ -490,121 +601,101 @@ static float stored_scale(const Problem &p) { return p.dtype == GRWS_F16 ? 4096.
 template <typename T> static int tensor_backward(const Problem &p, const Plan &q, void *dx, void *dw, char *scratch, cudaStream_t st) {
     Operands o;
     if (int rc = pack_operands<T>(p, q, scratch, &o, st)) return rc;
-    void *G = scratch + q.G;
     float *dx_sum = reinterpret_cast<float *>(scratch + q.dx_sum), *dw_sum = reinterpret_cast<float *>(scratch + q.dw_sum);
-    const int64_t g_plane = p.n * q.ldg;
-    const bool sum_dx = q.dx_parts > 1 || q.piece < p.V;
+    const bool sum_dx = q.dx_parts > 1 || q.piece < p.V, sum_dw = q.dw_parts > 1;
     for (int64_t v0 = 0; v0 < p.V; v0 += q.piece) {
         const int64_t cols = p.V - v0 < q.piece ? p.V - v0 : q.piece;
+        const View G = {scratch + q.G, p.n, cols, q.ldg, p.n * q.ldg, q.planes};
         prod::Params r;
-        if (int rc = product_params(p, q, &r)) return rc;
+        if (int rc = product_params(p, &r)) return rc;
         prod::Maps maps;
         const int cg = cta_group(p.n);
-        if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, r.bf16, q.planes, o.x, p.n, p.d, o.ldx, o.x_plane, 0, o.w, o.w_rows, o.w_cols, o.ldw,
-                              o.w_plane, !p.class_major, p.n, cols, p.d)) return rc;
+        if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, o.dtype, o.x, 0, o.w, !p.class_major, p.n, cols, p.d)) return rc;
+        if (int rc = prod::encode_map(&maps.c[0], G.p, o.dtype, cols, p.n, q.ldg, q.planes, G.plane, q.planes == 3 ? 32 : 64, 32)) return rc;
         r.task[0].b_row0 = (int)v0;
         r.v0 = v0;
-        r.label_score = const_cast<float *>(p.label_score);
         r.scale = stored_scale(p);
-        r.G = G; r.ldg = q.ldg; r.plane = g_plane;
-        if (int rc = launch_grouped<prod::GRAD>(cg, maps, r, st)) return rc;
+        if (int rc = launch_product<prod::GRAD>(cg, q.planes, maps, r, st)) return rc;
 
-        if (int rc = product_params(p, q, &r)) return rc;
+        if (int rc = product_params(p, &r)) return rc;
         r.scale = 1.0f / stored_scale(p);
         r.tasks = 0;
         const int pg = cta_group(p.n > p.d ? p.n : p.d);
-        int64_t dw_parts = 1;
-        if (dw) {
-            prod::Task *t = &r.task[r.tasks];
-            // [d, V]: x^T G; [V, d]: G^T x
-            const int64_t M = p.class_major ? cols : p.d, N = p.class_major ? p.d : cols;
+        const int64_t M = p.class_major ? cols : p.d, N = p.class_major ? p.d : cols, ldo = p.class_major ? p.d : p.V;
+        T *dw_out = static_cast<T *>(dw) + (p.class_major ? v0 * p.d : v0);
+        // the longer units first
+        for (int k = 0; k < 2; ++k) {
+            const bool is_dw = (q.dw_len >= q.dx_len) == (k == 0);
+            if (!(is_dw ? dw : dx)) continue;
+            const int i = r.tasks++;
+            prod::Task *t = &r.task[i];
             int rc;
-            if (p.class_major)
-                rc = set_task(t, &maps.a[r.tasks], &maps.b[r.tasks], pg, r.bf16, q.planes, G, p.n, cols, q.ldg, g_plane, 1, o.x, p.n, p.d, o.ldx, o.x_plane, 1, M, N, p.n);
-            else
-                rc = set_task(t, &maps.a[r.tasks], &maps.b[r.tasks], pg, r.bf16, q.planes, o.x, p.n, p.d, o.ldx, o.x_plane, 1, G, p.n, cols, q.ldg, g_plane, 1, M, N, p.n);
+            if (is_dw) {
+                // [d, V]: x^T G; [V, d]: G^T x
+                rc = p.class_major ? set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, G, 1, o.x, 1, M, N, p.n)
+                                   : set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, o.x, 1, G, 1, M, N, p.n);
+                if (rc != GRWS_OK) return rc;
+                t->k_len = (int)q.dw_len;
+                rc = sum_dw ? set_sums(t, &maps.c[i], q.dw_parts, dw_sum, q.ld_dw, false) : set_rounded(t, &maps.c[i], p.dtype, dw_out, ldo);
+            } else {
+                rc = set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, G, 0, o.w, p.class_major, p.n, p.d, cols);
+                if (rc != GRWS_OK) return rc;
+                t->b_k0 = (int)v0;
+                t->k_len = (int)q.dx_len;
+                rc = sum_dx ? set_sums(t, &maps.c[i], ceil_div((int64_t)t->k_blocks, q.dx_len), dx_sum, q.ld_dx, v0 > 0)      // (a last, shorter piece: fewer)
+                            : set_rounded(t, &maps.c[i], p.dtype, dx, p.d);
+            }
             if (rc != GRWS_OK) return rc;
-            t->k_len = (int)q.dw_len;
-            t->splits = (int)(dw_parts = q.dw_parts);
-            t->sum = dw_sum;
-            t->out_dtype = p.dtype;
-            t->ldo = p.class_major ? p.d : p.V;
-            if (dw_parts == 1) t->out = static_cast<T *>(dw) + (p.class_major ? v0 * p.d : v0);
-            ++r.tasks;
         }
-        if (dx) {
-            prod::Task *t = &r.task[r.tasks];
-            if (int rc = set_task(t, &maps.a[r.tasks], &maps.b[r.tasks], pg, r.bf16, q.planes, G, p.n, cols, q.ldg, g_plane, 0, o.w, o.w_rows, o.w_cols, o.ldw,
-                                  o.w_plane, p.class_major, p.n, p.d, cols)) return rc;
-            t->b_k0 = (int)v0;
-            t->k_len = (int)q.dx_len;
-            t->splits = (int)ceil_div((int64_t)t->k_blocks, q.dx_len);      // (a last, shorter piece has fewer)
-            t->sum = dx_sum;
-            t->add = v0 > 0;
-            t->out_dtype = p.dtype;
-            t->ldo = p.d;
-            if (!sum_dx) t->out = dx;
-            ++r.tasks;
-        }
-        if (int rc = launch_grouped<prod::SUM>(pg, maps, r, st)) return rc;
-        if (dw && dw_parts > 1) {
-            const int64_t M = p.class_major ? cols : p.d, N = p.class_major ? p.d : cols, ld = p.class_major ? p.d : p.V;
-            if (int rc = launch_round<T>(p, dw_sum, dw_parts, M, N, r.scale, static_cast<T *>(dw) + (p.class_major ? v0 * p.d : v0), ld, 1, st)) return rc;
-        }
+        if (int rc = launch_product<prod::SUM>(pg, q.planes, maps, r, st)) return rc;
+        if (dw && sum_dw) if (int rc = launch_round<T>(p, dw_sum, q.dw_parts, M, N, q.ld_dw, r.scale, dw_out, ldo, 1, st)) return rc;
     }
-    return dx && sum_dx ? launch_round<T>(p, dx_sum, q.dx_parts, p.n, p.d, 1.0f / stored_scale(p), dx, p.d, 1, st) : GRWS_OK;
+    return dx && sum_dx ? launch_round<T>(p, dx_sum, q.dx_parts, p.n, p.d, q.ld_dx, 1.0f / stored_scale(p), dx, p.d, 1, st) : GRWS_OK;
 }
 
-template <typename T> static int forward(const Problem &p, const Plan &q, float *loss, float2 *state, float *label_score, float *count, char *scratch,
-                                         cudaStream_t st) {
+template <typename T> static int forward(const Problem &p, const Plan &q, float *loss, float2 *state, float *count, char *scratch, cudaStream_t st) {
     float2 *part = reinterpret_cast<float2 *>(scratch + q.stats), *partial = reinterpret_cast<float2 *>(scratch + q.partial);
+    float *label_score = reinterpret_cast<float *>(scratch + q.label_score);
+    int *done = reinterpret_cast<int *>(scratch + q.done);
     if (q.tensor) {
-        if (int rc = tensor_forward<T>(p, q, part, label_score, scratch, st)) return rc;
+        if (int rc = tensor_forward<T>(p, q, part, label_score, done, scratch, st)) return rc;
     } else {
-        plain_stats_kernel<T><<<dim3((unsigned)ceil_div(p.n, (int64_t)TM), (unsigned)q.parts), 256, 0, st>>>(p, part, label_score);
-        GRWS_CUDA_TRY(cudaGetLastError());
+        if (int rc = launch_next(plain_stats_kernel<T>, dim3((unsigned)ceil_div(p.n, (int64_t)TM), (unsigned)q.parts), 256, 0, st, 1, p, part, label_score, done))
+            return rc;
     }
-    const int64_t blocks = ceil_div(p.n, (int64_t)256);
-    rows_kernel<<<(unsigned)blocks, 256, 0, st>>>(p, part, (int)(q.tensor ? 2 * q.parts : q.parts), label_score, state, loss, count, partial);
-    GRWS_CUDA_TRY(cudaGetLastError());
-    if (p.reduction != RED_NONE && blocks > 1) {
-        loss_sum_kernel<<<1, 512, 0, st>>>(partial, (int)blocks, p.reduction, loss, count);
-        GRWS_CUDA_TRY(cudaGetLastError());
-    }
-    return GRWS_OK;
+    return launch_next(rows_kernel, dim3((unsigned)ceil_div(p.n, (int64_t)ROWS_PER_BLOCK)), 256, 0, st, 1, p, part, (int)(q.tensor ? 2 * q.parts : q.parts),
+                       label_score, state, loss, count, partial, done);
 }
 
 template <typename T> static int backward(Problem p, const Plan &q, void *dx, void *dw, char *scratch, cudaStream_t st) {
     float *G = reinterpret_cast<float *>(scratch + q.G), *dx_sum = reinterpret_cast<float *>(scratch + q.dx_sum);
     float *dw_sum = reinterpret_cast<float *>(scratch + q.dw_sum), *norm = reinterpret_cast<float *>(scratch + q.norm);
     if (p.reduction == RED_NONE) {
-        grad_norm_kernel<<<1, 1024, 0, st>>>(p.grad, p.n, norm);
-        GRWS_CUDA_TRY(cudaGetLastError());
+        if (int rc = launch_next(grad_norm_kernel, dim3(1), 1024, 0, st, 1, p.grad, p.n, norm)) return rc;
         p.norm = norm;
     }
     if (q.tensor) return tensor_backward<T>(p, q, dx, dw, scratch, st);
-    const unsigned row_tiles = (unsigned)ceil_div(p.n, (int64_t)TM), width_tiles = (unsigned)ceil_div(p.d, (int64_t)TN);
+    const unsigned row_tiles = (unsigned)ceil_div(p.n, (int64_t)TM);
     const T *x = static_cast<const T *>(p.x), *w = static_cast<const T *>(p.w);
+    const bool sum_dx = q.dx_parts > 1 || q.piece < p.V, sum_dw = q.dw_parts > 1;
+    const int64_t ok = p.class_major ? 1 : p.V, ov = p.class_major ? p.d : 1;
     for (int64_t v0 = 0; v0 < p.V; v0 += q.piece) {
         const int64_t cols = p.V - v0 < q.piece ? p.V - v0 : q.piece;
-        const unsigned class_tiles = (unsigned)ceil_div(cols, (int64_t)TN);
-        plain_grad_kernel<T><<<dim3(row_tiles, class_tiles), 256, 0, st>>>(p, v0, cols, G, q.piece);
-        GRWS_CUDA_TRY(cudaGetLastError());
+        if (int rc = launch_next(plain_grad_kernel<T>, dim3(row_tiles, (unsigned)ceil_div(cols, (int64_t)TN)), 256, 0, st, 1, p, v0, cols, G, q.piece)) return rc;
+        PlainTask tx = {}, tw = {};
         if (dx) {
-            plain_product_kernel<float, T><<<dim3(row_tiles, width_tiles, (unsigned)q.dx_parts), 256, 0, st>>>(
-                G, q.piece, (int64_t)1, w + v0 * p.w_v(), p.w_v(), p.w_k(), p.n, p.d, cols, q.dx_len, dx_sum, v0 > 0);
-            GRWS_CUDA_TRY(cudaGetLastError());
+            tx = PlainTask{G, w + v0 * p.w_v(), q.piece, 1, p.w_v(), p.w_k(), p.n, p.d, cols, q.dx_len, (int)row_tiles, (int)ceil_div(p.d, (int64_t)TN),
+                           (int)ceil_div(cols, q.dx_len), v0 > 0, dx_sum, sum_dx ? nullptr : dx, p.d, 1};
         }
+        T *dw_out = static_cast<T *>(dw) + v0 * ov;
         if (dw) {
-            plain_product_kernel<T, float><<<dim3(width_tiles, class_tiles, (unsigned)q.dw_parts), 256, 0, st>>>(
-                x, (int64_t)1, p.ldx, G, q.piece, (int64_t)1, p.d, cols, p.n, q.dw_len, dw_sum, 0);
-            GRWS_CUDA_TRY(cudaGetLastError());
-            const int64_t ok = p.class_major ? 1 : p.V, ov = p.class_major ? p.d : 1;
-            const int rc = launch_round<T>(p, dw_sum, q.dw_parts, p.d, cols, 1.0f, static_cast<T *>(dw) + v0 * ov, ok, ov, st);
-            if (rc != GRWS_OK) return rc;
+            tw = PlainTask{x, G, 1, p.ldx, q.piece, 1, p.d, cols, p.n, q.dw_len, (int)ceil_div(p.d, (int64_t)TM), (int)ceil_div(cols, (int64_t)TN),
+                           (int)q.dw_parts, 0, dw_sum, sum_dw ? nullptr : dw_out, ok, ov};
         }
+        if (int rc = launch_next(plain_products_kernel<T>, dim3((unsigned)(tx.blocks() + tw.blocks())), 256, 0, st, 1, p, tx, tw)) return rc;
+        if (dw && sum_dw) if (int rc = launch_round<T>(p, dw_sum, q.dw_parts, p.d, cols, cols, 1.0f, dw_out, ok, ov, st)) return rc;
     }
-    return dx ? launch_round<T>(p, dx_sum, q.dx_parts, p.n, p.d, 1.0f, dx, p.d, 1, st) : GRWS_OK;
+    return dx && sum_dx ? launch_round<T>(p, dx_sum, q.dx_parts, p.n, p.d, p.d, 1.0f, dx, p.d, 1, st) : GRWS_OK;
 }
 
 static int check(const Problem &p) {
@@ -661,11 +752,10 @@ int grws_linear_ce_fwd(const void *x, int64_t ldx, const void *w, int64_t ldw, i
     if (scratch_bytes < q.bytes) return fail(GRWS_ERR_SCRATCH, "linear cross entropy scratch too small");
     char *s = static_cast<char *>(scratch);
     float2 *state2 = reinterpret_cast<float2 *>(state);
-    float *label_score = state + 2 * rows;
     switch (dtype) {
-        case GRWS_F32: return lce::forward<float>(p, q, loss, state2, label_score, count, s, st);
-        case GRWS_F16: return lce::forward<__half>(p, q, loss, state2, label_score, count, s, st);
-        default: return lce::forward<__nv_bfloat16>(p, q, loss, state2, label_score, count, s, st);
+        case GRWS_F32: return lce::forward<float>(p, q, loss, state2, count, s, st);
+        case GRWS_F16: return lce::forward<__half>(p, q, loss, state2, count, s, st);
+        default: return lce::forward<__nv_bfloat16>(p, q, loss, state2, count, s, st);
     }
 }
 
@@ -689,7 +779,6 @@ int grws_linear_ce_bwd(const void *x, int64_t ldx, const void *w, int64_t ldw, i
     const lce::Plan q = lce::make_plan(p, true);
     if (scratch_bytes < q.bytes) return fail(GRWS_ERR_SCRATCH, "linear cross entropy scratch too small");
     p.state = reinterpret_cast<const float2 *>(state);
-    p.label_score = state + 2 * rows;
     p.grad = grad_loss;
     p.count = count;
     char *s = static_cast<char *>(scratch);

@@ -1,6 +1,8 @@
 """Losses over the class axis on the library's kernels (csrc/linear_ce.cu, csrc/distill.cu): softmax cross entropy of a
 linear classifier that never keeps its scores, and distillation from a teacher's best scores.  The reference's steps take
 F.cross_entropy of the last layer's output (helper/engine.py:66-75)."""
+import contextlib
+
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
@@ -11,6 +13,7 @@ from ..core import _DT, _ptr, _scratch, _stream
 _REDUCTIONS = {'none': _native.REDUCE_NONE, 'mean': _native.REDUCE_MEAN, 'sum': _native.REDUCE_SUM}
 _INDEX_BYTES = {torch.int64: 8, torch.int32: 4}
 MAX_KEPT = 1024
+_HERE = contextlib.nullcontext()
 
 
 def _reduction(name):
@@ -44,6 +47,11 @@ def _stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _on(device):
+    """Context in which ``device`` is the current device (a guard costs time: none where it is already)."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _outputs(rows, per_row, reduction, device):
     loss = torch.empty(rows if reduction == _native.REDUCE_NONE else (), dtype=torch.float32, device=device)
     state = torch.empty(rows * per_row + 4, dtype=torch.float32, device=device)      # the last four: the count of the rows
@@ -58,10 +66,10 @@ class _LinearCrossEntropyFunction(Function):
         class_major = weight.stride(1) != 1 and weight.stride(0) == 1
         w = _rows_of(weight.t() if class_major else weight)
         (n, d), V = x.shape, weight.shape[1]
-        loss, state = _outputs(n, 3, reduction, x.device)
-        count = state.data_ptr() + 12 * n
+        loss, state = _outputs(n, 2, reduction, x.device)
+        count = state.data_ptr() + 8 * n
         args = (_ptr(x), _stride(x), _ptr(w), _stride(w), int(class_major))
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             scratch = _scratch(lib.grws_linear_ce_scratch_bytes(*args, n, d, V, _DT[x.dtype], 0), x.device)
             _native.check(lib.grws_linear_ce_fwd(*args, _ptr(labels), _INDEX_BYTES[labels.dtype], ignore_index, n, d, V, _DT[x.dtype],
                                                  reduction, loss.data_ptr(), state.data_ptr(), count, scratch.data_ptr(),
@@ -81,10 +89,10 @@ class _LinearCrossEntropyFunction(Function):
         dx = torch.empty((n, d), dtype=x.dtype, device=x.device) if ctx.needs_input_grad[0] else None
         dw = torch.empty(w.shape, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[1] else None
         args = (_ptr(x), _stride(x), _ptr(w), _stride(w), int(class_major))
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             scratch = _scratch(lib.grws_linear_ce_scratch_bytes(*args, n, d, V, _DT[x.dtype], 1), x.device)
             _native.check(lib.grws_linear_ce_bwd(*args, _ptr(labels), _INDEX_BYTES[labels.dtype], ignore_index, n, d, V, _DT[x.dtype],
-                                                 reduction, _ptr(grad_loss), state.data_ptr(), state.data_ptr() + 12 * n, _ptr(dx),
+                                                 reduction, _ptr(grad_loss), state.data_ptr(), state.data_ptr() + 8 * n, _ptr(dx),
                                                  _ptr(dw), scratch.data_ptr(), scratch.numel(), _stream(x.device)))
         return dx, dw.t() if class_major and dw is not None else dw, None, None, None
 
@@ -123,7 +131,7 @@ class _DistillationFunction(Function):
         logits, teacher, ids = _rows_of(logits), _rows_of(teacher), _rows_of(ids)
         (n, V), K = logits.shape, ids.shape[1]
         loss, state = _outputs(n, 4, reduction, logits.device)
-        with torch.cuda.device(logits.device):
+        with _on(logits.device):
             scratch = _scratch(lib.grws_distill_scratch_bytes(n, V), logits.device)
             _native.check(lib.grws_distill_fwd(
                 _ptr(logits), _stride(logits), _DT[logits.dtype], _ptr(teacher), _stride(teacher), _DT[teacher.dtype], _ptr(ids),
@@ -146,7 +154,7 @@ class _DistillationFunction(Function):
         ld = _stride(logits)
         ldo = ld if ld <= V + 16 else -(-V // 8) * 8
         dlogits = torch.empty((n, ldo), dtype=logits.dtype, device=logits.device)[:, :V]
-        with torch.cuda.device(logits.device):
+        with _on(logits.device):
             _native.check(lib.grws_distill_bwd(
                 _ptr(logits), ld, _DT[logits.dtype], _ptr(teacher), _stride(teacher), _DT[teacher.dtype], _ptr(ids), _stride(ids),
                 _INDEX_BYTES[ids.dtype], n, V, K, temperature, reduction, _ptr(grad_loss), state.data_ptr(), state.data_ptr() + 16 * n,

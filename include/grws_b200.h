@@ -272,7 +272,7 @@ int grws_layer_norm_bwd(const void *x, const void *gamma, const void *dy, const 
  *          the layers' weights) or at v * ldw + k (class_major = 1);
  *   labels [rows] integers of label_bytes (4 or 8); a row with `ignore_index` counts nothing and has
  *          no gradient, any other label outside [0, classes) makes its loss and gradients NaN;
- *   loss   [1], or [rows] without a reduction; state [3 * rows] and count [1] (with a reduction) go
+ *   loss   [1], or [rows] without a reduction; state [2 * rows] and count [1] (with a reduction) go
  *          from the forward to the backward call, 16-byte aligned state;
  *   grad_loss  gradient of `loss`, of its size;
  *   dx [rows, width] and dw (in w's order) contiguous, of `dtype`; either may be null.
