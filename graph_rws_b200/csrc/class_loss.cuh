@@ -81,16 +81,24 @@ __device__ __forceinline__ void join_stats(float &m, float &s, float m2, float s
     m = top;
 }
 
+// (up to four chains of maxima and of sums: one chain's latency would be most of the time)
 template <int N> __device__ __forceinline__ void add_values(float &m, float &s, const float (&v)[N], float c) {
-    float top = m;
+    constexpr int W = N >= 16 ? 4 : N >= 4 ? 2 : 1;
+    float top[W], t[W];
 #pragma unroll
-    for (int i = 0; i < N; ++i) top = fmaxf(top, v[i]);
-    const float safe = finite_or_zero(top);
-    if (top != m) { s *= exp2_approx((m - safe) * c); m = top; }
-    float t = 0.0f;
+    for (int j = 0; j < W; ++j) { top[j] = v[j]; t[j] = 0.0f; }
 #pragma unroll
-    for (int i = 0; i < N; ++i) t += exp2_approx((v[i] - safe) * c);
-    s += t;
+    for (int i = W; i < N; ++i) top[i % W] = fmaxf(top[i % W], v[i]);
+#pragma unroll
+    for (int j = 1; j < W; ++j) top[0] = fmaxf(top[0], top[j]);
+    top[0] = fmaxf(top[0], m);
+    const float safe = finite_or_zero(top[0]);
+    if (top[0] != m) { s *= exp2_approx((m - safe) * c); m = top[0]; }
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i % W] += exp2_approx((v[i] - safe) * c);
+#pragma unroll
+    for (int j = 1; j < W; ++j) t[0] += t[j];
+    s += t[0];
 }
 
 // Kernels of one call follow each other as programmatic dependents: the next one is launched while this one still runs, sets

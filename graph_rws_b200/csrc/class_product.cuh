@@ -103,7 +103,9 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    // (nothing but tensor memory is handed over, which tcgen05.fence orders: a release of the cluster's scope costs a
+    // memory barrier per tile and warp)
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -272,8 +274,8 @@ template <typename P> __device__ __forceinline__ float grad_alpha(const P &p) {
     return norm > 0.0f ? norm : 1.0f;
 }
 
-__device__ __forceinline__ uint32_t pack2(float a, float b, int bf16) {
-    if (bf16) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (BF16) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
@@ -479,92 +481,100 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                 const int cols = (int)min((int64_t)t.bn, t.N - col0);          // of this tile
                 const int mine = (int)max((int64_t)-1, min((int64_t)BN, label - p.v0 - col0));    // label's column, if within
                 (void)mine;
-                // 32 columns from c on, the first or second half of this warp's 64
-                auto use = [&](float (&v)[32], int c, int second) {
+                // W columns from c on: 64, for fp32 32
+                constexpr int W = SPLIT ? 32 : 64;
+                auto put16 = [&](const float (&v)[W]) {
+                    if (p.bf16) {
+#pragma unroll
+                        for (int i = 0; i < W; i += 8)
+                            put(i / 8, pack2<true>(v[i], v[i + 1]), pack2<true>(v[i + 2], v[i + 3]), pack2<true>(v[i + 4], v[i + 5]), pack2<true>(v[i + 6], v[i + 7]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < W; i += 8)
+                            put(i / 8, pack2<false>(v[i], v[i + 1]), pack2<false>(v[i + 2], v[i + 3]), pack2<false>(v[i + 4], v[i + 5]), pack2<false>(v[i + 6], v[i + 7]));
+                    }
+                };
+                auto use = [&](float (&v)[W], int c) {
                     if constexpr (MODE == STATS) {
-                        if (__any_sync(0xffffffffu, mine >= c && mine < c + 32)) {
+                        if (__any_sync(0xffffffffu, mine >= c && mine < c + W)) {
                             float score = 0.0f;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) if (mine == c + i) score = v[i];
-                            if (in && mine >= c && mine < c + 32 && mine < cols) p.label_score[row] = score;
+                            for (int i = 0; i < W; ++i) if (mine == c + i) score = v[i];
+                            if (in && mine >= c && mine < c + W && mine < cols) p.label_score[row] = score;
                         }
-                        if (c + 32 > cols) {
+                        if (c + W > cols) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) if (c + i >= cols) v[i] = NEG_INF;
+                            for (int i = 0; i < W; ++i) if (c + i >= cols) v[i] = NEG_INF;
                         }
-                        add_values<32>(m, s, v, LOG2E);
+                        add_values<W>(m, s, v, LOG2E);
                     } else if constexpr (MODE == GRAD) {
-                        const bool has = __any_sync(0xffffffffu, mine >= c && mine < c + 32);
+                        const bool has = __any_sync(0xffffffffu, mine >= c && mine < c + W);
                         if constexpr (!SPLIT) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = exp2_approx(fmaf(v[i], LOG2E, -base)) * factor;
+                            for (int i = 0; i < W; ++i) v[i] = exp2_approx(fmaf(v[i], LOG2E, -base)) * factor;
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = exp2_approx((v[i] - m) * LOG2E) * inv * factor;
+                            for (int i = 0; i < W; ++i) v[i] = exp2_approx((v[i] - m) * LOG2E) * inv * factor;
                         }
                         if (has) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) if (mine == c + i) v[i] -= factor;
+                            for (int i = 0; i < W; ++i) if (mine == c + i) v[i] -= factor;
                         }
                         if (factor == 0.0f) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+                            for (int i = 0; i < W; ++i) v[i] = 0.0f;
                         }
                         if constexpr (!SPLIT) {
-                            if (!second) box_free();
-#pragma unroll
-                            for (int i = 0; i < 32; i += 8)
-                                put(second * 4 + i / 8, pack2(v[i], v[i + 1], p.bf16), pack2(v[i + 2], v[i + 3], p.bf16), pack2(v[i + 4], v[i + 5], p.bf16),
-                                    pack2(v[i + 6], v[i + 7], p.bf16));
-                            if (second) box_out(mc, (int)col0 + c - 32, row0, 0, false);
+                            box_free();
+                            put16(v);
+                            box_out(mc, (int)col0 + c, row0, 0, false);
                         } else {
-                            // a plane of 64 columns at a time would keep all of them in registers: boxes of 32 columns here
+                            // lines of 64 bytes, not swizzled: 64 columns would keep too much in registers
 #pragma unroll
                             for (int k = 0; k < 3; ++k) {
-                                uint32_t q[16];
+                                uint32_t q[W / 2];
 #pragma unroll
-                                for (int i = 0; i < 32; i += 2) {
+                                for (int i = 0; i < W; i += 2) {
                                     float a[2], b[2], d[2];
                                     split3(v[i], a[0], b[0], d[0]);
                                     split3(v[i + 1], a[1], b[1], d[1]);
-                                    q[i / 2] = k == 0 ? pack2(a[0], a[1], 1) : k == 1 ? pack2(b[0], b[1], 1) : pack2(d[0], d[1], 1);
+                                    q[i / 2] = k == 0 ? pack2<true>(a[0], a[1]) : k == 1 ? pack2<true>(b[0], b[1]) : pack2<true>(d[0], d[1]);
                                 }
                                 box_free();
 #pragma unroll
-                                for (int j = 0; j < 4; ++j)      // lines of 64 bytes, not swizzled
-                                    st_shared16(box + lane * 64 + j * 16, q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
+                                for (int j = 0; j < W / 8; ++j) st_shared16(box + lane * 64 + j * 16, q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
                                 box_out(mc, (int)col0 + c, row0, k, false);
                             }
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] *= factor;
+                        for (int i = 0; i < W; ++i) v[i] *= factor;
                         if (!SPLIT && t.rounded && t.out_dtype != GRWS_F32) {
-                            if (!second) box_free();
-#pragma unroll
-                            for (int i = 0; i < 32; i += 8)
-                                put(second * 4 + i / 8, pack2(v[i], v[i + 1], p.bf16), pack2(v[i + 2], v[i + 3], p.bf16), pack2(v[i + 4], v[i + 5], p.bf16),
-                                    pack2(v[i + 6], v[i + 7], p.bf16));
-                            if (!second) return;
-                            if (!t.out) { box_out(mc, (int)col0 + c - 32, row0, 0, false); return; }
+                            box_free();
+                            put16(v);
+                            if (!t.out) { box_out(mc, (int)col0 + c, row0, 0, false); return; }
                             __syncwarp();
                             for (int r = 0; r < 32 && row0 + r < t.M; ++r) {
                                 const uint32_t two = ld_shared32(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-                                uint16_t *o = static_cast<uint16_t *>(t.out) + (row0 + r) * t.ldo + col0 + c - 32 + lane * 2;
-                                if (c - 32 + lane * 2 < cols) o[0] = (uint16_t)two;
-                                if (c - 32 + lane * 2 + 1 < cols) o[1] = (uint16_t)(two >> 16);
+                                uint16_t *o = static_cast<uint16_t *>(t.out) + (row0 + r) * t.ldo + col0 + c + lane * 2;
+                                if (c + lane * 2 < cols) o[0] = (uint16_t)two;
+                                if (c + lane * 2 + 1 < cols) o[1] = (uint16_t)(two >> 16);
                             }
                             __syncwarp();
-                        } else {
+                            return;
+                        }
+#pragma unroll
+                        for (int h = 0; h < W; h += 32) {
+                            if (c + h >= cols) return;
                             box_free();
 #pragma unroll
                             for (int i = 0; i < 32; i += 4)
-                                put(i / 4, __float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]));
-                            if (!t.out) { box_out(mc, (int)col0 + c, row0, w.split, t.add); return; }
+                                put(i / 4, __float_as_uint(v[h + i]), __float_as_uint(v[h + i + 1]), __float_as_uint(v[h + i + 2]), __float_as_uint(v[h + i + 3]));
+                            if (!t.out) { box_out(mc, (int)col0 + c + h, row0, w.split, t.add); continue; }
                             __syncwarp();
                             for (int r = 0; r < 32 && row0 + r < t.M; ++r) {
                                 const uint32_t one = ld_shared32(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-                                if (c + lane < cols) static_cast<float *>(t.out)[(row0 + r) * t.ldo + col0 + c + lane] = __uint_as_float(one);
+                                if (c + h + lane < cols) static_cast<float *>(t.out)[(row0 + r) * t.ldo + col0 + c + h + lane] = __uint_as_float(one);
                             }
                             __syncwarp();
                         }
@@ -577,18 +587,15 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                     if (last < 0) release_tile();
                     for (int k = 0; k <= last; ++k) {
                         const int c = half * 64 + k * 128;
-                        float v[32];
+                        float v[64];
                         uint32_t r[32], r2[32];
                         tmem_ld32(at + c, r);
                         tmem_ld32(at + c + 32, r2);
                         tmem_ld_wait();
                         if (k == last) release_tile();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-                        use(v, c, 0);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r2[i]);
-                        use(v, c + 32, 1);
+                        for (int i = 0; i < 32; ++i) { v[i] = __uint_as_float(r[i]); v[32 + i] = __uint_as_float(r2[i]); }
+                        use(v, c);
                     }
                 } else {
                     const int k0 = w.split * t.k_len, big = min(t.k_blocks, k0 + t.k_len) - k0;
@@ -615,7 +622,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const int c = half * 64 + (k >> 1) * 128 + (k & 1) * 32;
-                        if (c < cols) use(acc[k], c, k & 1);
+                        if (c < cols) use(acc[k], c);
                     }
                 }
             }

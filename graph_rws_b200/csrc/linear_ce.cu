@@ -319,9 +319,9 @@ template <typename T> __global__ void __launch_bounds__(256) pack_kernel(const T
                 float a[2], b[2], e[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) prod::split3(c + 2 * j + h < cols ? to_float(s[2 * j + h]) : 0.0f, a[h], b[h], e[h]);
-                q[0][j] = prod::pack2(a[0], a[1], 1);
-                q[1][j] = prod::pack2(b[0], b[1], 1);
-                q[2][j] = prod::pack2(e[0], e[1], 1);
+                q[0][j] = prod::pack2<true>(a[0], a[1]);
+                q[1][j] = prod::pack2<true>(b[0], b[1]);
+                q[2][j] = prod::pack2<true>(e[0], e[1]);
             }
 #pragma unroll
             for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4 *>(d + k * plane) = make_uint4(q[k][0], q[k][1], q[k][2], q[k][3]);
@@ -381,13 +381,13 @@ static int cta_group(int64_t M) { return M > prod::BM ? 2 : 1; }
 static bool needs_packing(const void *p, int64_t ld, int dtype) { return dtype == GRWS_F32 || !aligned16(p) || ld % 8 != 0; }
 
 // Class tiles that one unit of the forward pass takes: as many as leave the SMs equally busy; every part is a statistic per
-// row (of two warps each) written and read at some 5 TB/s, a tile step takes about 0.4 us
+// row (of two warps each) written and read at some 5 TB/s, and a step of the loop that joins them; a tile step takes about 0.4 us
 static void cut_runs(int64_t n, int64_t m_tiles, int64_t n_tiles, int64_t steps, int64_t ctas, int64_t *run, int64_t *runs) {
     int64_t best = 1;
     double best_us = 1e300;
     for (int64_t r = 1; r <= n_tiles && r <= 64; ++r) {
         const int64_t k = ceil_div(n_tiles, r);
-        const double us = (double)(ceil_div(m_tiles * k, ctas) * r * steps) * 0.4 + (double)(k * n) * 32.0 / 5.0e6;
+        const double us = (double)(ceil_div(m_tiles * k, ctas) * r * steps) * 0.4 + (double)(k * n) * 32.0 / 5.0e6 + 0.06 * (double)k;
         if (us <= best_us) { best_us = us; best = r; }
     }
     *run = best;
