@@ -170,10 +170,21 @@ __device__ __forceinline__ float loss_factor(const float *grad_loss, const float
     return n > 0.0f ? g / n : 0.0f;
 }
 
+// Properties of the current device, read once
+constexpr int MAX_DEVICES = 64;
+inline int current_device() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < MAX_DEVICES ? dev : -1;
+}
 inline int sm_count() {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
-        sms = 148;
+    static int known[MAX_DEVICES];
+    const int dev = current_device();
+    if (dev < 0) return 148;
+    int sms = __atomic_load_n(&known[dev], __ATOMIC_RELAXED);
+    if (sms == 0) {
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) return 148;
+        __atomic_store_n(&known[dev], sms, __ATOMIC_RELAXED);
+    }
     return sms;
 }
 

@@ -677,7 +677,13 @@ template <int CG, int MODE, bool SPLIT> static int launch_product(const Maps &ma
     int64_t units = 0;
     for (int i = 0; i < p.tasks; ++i) units += p.task[i].units();
     const int64_t clusters = units < sm_count() / CG ? units : sm_count() / CG;
-    GRWS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<CG, MODE, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<CG>::SMEM));
+    static bool allowed[MAX_DEVICES];
+    const int dev = current_device();
+    if (dev < 0) return fail(GRWS_ERR_CUDA, "no current device");
+    if (!__atomic_load_n(&allowed[dev], __ATOMIC_RELAXED)) {
+        GRWS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<CG, MODE, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<CG>::SMEM));
+        __atomic_store_n(&allowed[dev], true, __ATOMIC_RELAXED);
+    }
     return launch_next(product_kernel<CG, MODE, SPLIT>, dim3((unsigned)(clusters * CG)), THREADS, Cfg<CG>::SMEM, st, CG, maps, p);
 }
 

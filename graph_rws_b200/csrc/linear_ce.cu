@@ -559,9 +559,23 @@ static int set_rounded(prod::Task *t, CUtensorMap *mc, int dtype, void *out, int
     return prod::encode_map(mc, out, dtype, t->N, t->M, ldo, 1, 0, dtype == GRWS_F32 ? 32 : 64, 32);
 }
 
+static int status_word(int **word) {
+    static int *known[MAX_DEVICES];
+    const int dev = current_device();
+    if (dev < 0) return fail(GRWS_ERR_CUDA, "no current device");
+    *word = __atomic_load_n(&known[dev], __ATOMIC_RELAXED);
+    if (!*word) {
+        void *p = nullptr;
+        GRWS_CUDA_TRY(cudaGetSymbolAddress(&p, g_status));
+        *word = static_cast<int *>(p);
+        __atomic_store_n(&known[dev], *word, __ATOMIC_RELAXED);
+    }
+    return GRWS_OK;
+}
+
 static int product_params(const Problem &p, prod::Params *r) {
-    void *status = nullptr;
-    GRWS_CUDA_TRY(cudaGetSymbolAddress(&status, g_status));
+    int *status = nullptr;
+    if (int rc = status_word(&status)) return rc;
     *r = prod::Params{};
     r->tasks = 1;
     r->bf16 = p.dtype != GRWS_F16;
@@ -569,7 +583,7 @@ static int product_params(const Problem &p, prod::Params *r) {
     r->reduction = p.reduction; r->grad = p.grad; r->count = p.count; r->norm = p.norm;
     r->state = p.state;
     r->scale = 1.0f;
-    r->status = static_cast<int *>(status);
+    r->status = status;
     r->wait_limit = prod::WAIT_LIMIT_CYCLES;
     return GRWS_OK;
 }
@@ -791,10 +805,9 @@ int grws_linear_ce_bwd(const void *x, int64_t ldx, const void *w, int64_t ldw, i
 
 __attribute__((visibility("default")))
 int grws_linear_ce_check(void *stream) {
-    void *word = nullptr;
-    int status = 0;
+    int *word = nullptr, status = 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    GRWS_CUDA_TRY(cudaGetSymbolAddress(&word, lce::g_status));
+    if (int rc = lce::status_word(&word)) return rc;
     GRWS_CUDA_TRY(cudaMemcpyAsync(&status, word, sizeof(int), cudaMemcpyDeviceToHost, s));
     GRWS_CUDA_TRY(cudaStreamSynchronize(s));
     if (status == 0) return GRWS_OK;

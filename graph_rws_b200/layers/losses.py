@@ -2,6 +2,7 @@
 linear classifier that never keeps its scores, and distillation from a teacher's best scores.  The reference's steps take
 F.cross_entropy of the last layer's output (helper/engine.py:66-75)."""
 import contextlib
+import functools
 
 import torch
 from torch.autograd import Function
@@ -58,6 +59,17 @@ def _outputs(rows, per_row, reduction, device):
     return loss, state
 
 
+@functools.lru_cache(maxsize=256)
+def _ce_scratch_bytes(device_index, *args):
+    return _native.lib().grws_linear_ce_scratch_bytes(*args)
+
+
+def _ce_scratch(x, w, class_major, n, d, V, backward):
+    # where an operand starts matters to 16 bytes only
+    return _scratch(_ce_scratch_bytes(x.device.index, 16 + _ptr(x) % 16, _stride(x), 16 + _ptr(w) % 16, _stride(w), class_major, n, d, V,
+                                      _DT[x.dtype], backward), x.device)
+
+
 class _LinearCrossEntropyFunction(Function):
     @staticmethod
     def forward(ctx, x, weight, labels, ignore_index, reduction):
@@ -70,7 +82,7 @@ class _LinearCrossEntropyFunction(Function):
         count = state.data_ptr() + 8 * n
         args = (_ptr(x), _stride(x), _ptr(w), _stride(w), int(class_major))
         with _on(x.device):
-            scratch = _scratch(lib.grws_linear_ce_scratch_bytes(*args, n, d, V, _DT[x.dtype], 0), x.device)
+            scratch = _ce_scratch(x, w, int(class_major), n, d, V, 0)
             _native.check(lib.grws_linear_ce_fwd(*args, _ptr(labels), _INDEX_BYTES[labels.dtype], ignore_index, n, d, V, _DT[x.dtype],
                                                  reduction, loss.data_ptr(), state.data_ptr(), count, scratch.data_ptr(),
                                                  scratch.numel(), _stream(x.device)))
@@ -90,7 +102,7 @@ class _LinearCrossEntropyFunction(Function):
         dw = torch.empty(w.shape, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[1] else None
         args = (_ptr(x), _stride(x), _ptr(w), _stride(w), int(class_major))
         with _on(x.device):
-            scratch = _scratch(lib.grws_linear_ce_scratch_bytes(*args, n, d, V, _DT[x.dtype], 1), x.device)
+            scratch = _ce_scratch(x, w, int(class_major), n, d, V, 1)
             _native.check(lib.grws_linear_ce_bwd(*args, _ptr(labels), _INDEX_BYTES[labels.dtype], ignore_index, n, d, V, _DT[x.dtype],
                                                  reduction, _ptr(grad_loss), state.data_ptr(), state.data_ptr() + 8 * n, _ptr(dx),
                                                  _ptr(dw), scratch.data_ptr(), scratch.numel(), _stream(x.device)))
@@ -124,6 +136,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     return _LinearCrossEntropyFunction.apply(x, weight, labels, int(ignore_index), red)
 
 
+@functools.lru_cache(maxsize=256)
+def _distill_scratch_bytes(device_index, rows, classes):
+    return _native.lib().grws_distill_scratch_bytes(rows, classes)
+
+
 class _DistillationFunction(Function):
     @staticmethod
     def forward(ctx, logits, teacher, ids, temperature, reduction):
@@ -132,7 +149,7 @@ class _DistillationFunction(Function):
         (n, V), K = logits.shape, ids.shape[1]
         loss, state = _outputs(n, 4, reduction, logits.device)
         with _on(logits.device):
-            scratch = _scratch(lib.grws_distill_scratch_bytes(n, V), logits.device)
+            scratch = _scratch(_distill_scratch_bytes(logits.device.index, n, V), logits.device)
             _native.check(lib.grws_distill_fwd(
                 _ptr(logits), _stride(logits), _DT[logits.dtype], _ptr(teacher), _stride(teacher), _DT[teacher.dtype], _ptr(ids),
                 _stride(ids), _INDEX_BYTES[ids.dtype], n, V, K, temperature, reduction, loss.data_ptr(), state.data_ptr(),
