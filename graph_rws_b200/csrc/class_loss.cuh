@@ -2,6 +2,7 @@
 // statistics, the reduction of row losses and the factor a row's gradient gets from the loss's.
 #pragma once
 
+#include <type_traits>
 #include <utility>
 
 #include "grws_common.cuh"
@@ -24,7 +25,7 @@ template <> __device__ __forceinline__ __half from_float<__half>(float v) { retu
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // 16 bytes of a row as fp32 values and back
-template <typename T> struct Piece;
+template <typename T> struct Piece;      // `largest` of several pieces ignores NaN, as fmaxf does
 template <> struct Piece<float> {
     static constexpr int E = 4;
     static __device__ __forceinline__ void unpack(const uint4 &u, float (&v)[4]) {
@@ -65,6 +66,29 @@ template <> struct Piece<__nv_bfloat16> {
     }
 };
 
+template <typename T, int N> __device__ __forceinline__ float largest(const uint4 (&u)[N]) {
+    if constexpr (sizeof(T) == 4) {
+        float m = NEG_INF;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(u[i].x), __uint_as_float(u[i].y))), fmaxf(__uint_as_float(u[i].z), __uint_as_float(u[i].w)));
+        return m;
+    } else {
+        // two 16-bit numbers at a time: a maximum is exact in any type
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        T2 m[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const T2 *h = reinterpret_cast<const T2 *>(&u[i]);
+            m[i] = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        }
+#pragma unroll
+        for (int i = 1; i < N; ++i) m[0] = __hmax2(m[0], m[i]);
+        const float a = to_float(m[0].x), b = to_float(m[0].y);
+        return fmaxf(a, b);
+    }
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -98,6 +122,26 @@ template <int N> __device__ __forceinline__ void add_values(float &m, float &s, 
     for (int i = 0; i < N; ++i) t[i % W] += exp2_approx((v[i] - safe) * c);
 #pragma unroll
     for (int j = 1; j < W; ++j) t[0] += t[j];
+    s += t[0];
+}
+
+// the same for N pieces of a row as loaded.  (c v - c max would be one instruction instead of two, but is off by 2^-24 of
+// c max: a row masked with the type's lowest value would sum up infinities.)
+template <typename T, int N> __device__ __forceinline__ void add_pieces(float &m, float &s, const uint4 (&u)[N], float c) {
+    constexpr int E = Piece<T>::E;
+    const float top = fmaxf(m, largest<T, N>(u)), safe = finite_or_zero(top);
+    if (top != m) { s *= exp2_approx((m - safe) * c); m = top; }
+    float t[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float v[E];
+        Piece<T>::unpack(u[i], v);
+        t[i] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) t[i] += exp2_approx((v[e] - safe) * c);
+    }
+#pragma unroll
+    for (int i = 1; i < N; ++i) t[0] += t[i];
     s += t[0];
 }
 

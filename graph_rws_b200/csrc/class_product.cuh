@@ -460,7 +460,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
             const int row0 = (w.m * CG + (int)rank) * BM + quarter * 32;
             const int64_t row = row0 + lane;
             const bool in = row < t.M;
-            [[maybe_unused]] float m = NEG_INF, s = 0.0f, factor = 0.0f, base = 0.0f, inv = 0.0f;
+            [[maybe_unused]] float m = NEG_INF, s = 0.0f, factor = 0.0f, weight = 0.0f;
             [[maybe_unused]] int64_t label = -1;
             if constexpr (MODE != SUM) {
                 if (in) label = load_index(p.labels, p.label_bytes, row);
@@ -470,8 +470,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                     const float2 st = p.state[row];
                     factor = grad_row_factor(p, row, label) * p.scale;
                     m = st.x;
-                    inv = 1.0f / st.y;
-                    base = st.x * LOG2E + log2f(st.y);
+                    weight = factor / st.y;
                 }
                 if (label == p.ignore_index) label = -1;
             }
@@ -509,13 +508,8 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                         add_values<W>(m, s, v, LOG2E);
                     } else if constexpr (MODE == GRAD) {
                         const bool has = __any_sync(0xffffffffu, mine >= c && mine < c + W);
-                        if constexpr (!SPLIT) {
 #pragma unroll
-                            for (int i = 0; i < W; ++i) v[i] = exp2_approx(fmaf(v[i], LOG2E, -base)) * factor;
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < W; ++i) v[i] = exp2_approx((v[i] - m) * LOG2E) * inv * factor;
-                        }
+                        for (int i = 0; i < W; ++i) v[i] = exp2_approx((v[i] - m) * LOG2E) * weight;
                         if (has) {
 #pragma unroll
                             for (int i = 0; i < W; ++i) if (mine == c + i) v[i] -= factor;

@@ -20,7 +20,7 @@ using namespace cls;
 constexpr int MAX_KEPT = 1024;
 constexpr int THREADS = 256;
 constexpr int CTAS_PER_SM = 8;
-constexpr int SHORT_ROW = 1024;          // classes up to which a group of lanes takes a row (else a CTA)
+constexpr int SHORT_ROW = 16384;         // classes up to which a group of lanes takes a row (else a CTA), given the rows
 constexpr int SHORT_KEPT = 64;           // entries that such a group holds in shared memory
 constexpr int SPLIT_MIN = 4096;          // classes below which a row is not cut any further
 
@@ -78,66 +78,138 @@ template <typename T> struct Span {
     __device__ __forceinline__ const T *rest() const { return p + head + pieces * Piece<T>::E; }
 };
 
-// running statistics of a span by `lanes` threads
-template <typename T, int UNROLL> __device__ __forceinline__ void span_stats(const Span<T> &sp, int lane, int lanes, float c, float &m, float &s) {
-    constexpr int E = Piece<T>::E;
-    for (int i = lane; i < sp.head + sp.tail; i += lanes) {
-        const float v[1] = {to_float(i < sp.head ? sp.p[i] : sp.rest()[i - sp.head])};
-        add_values<1>(m, s, v, c);
-    }
-    const uint4 *b = sp.body();
-    int64_t k = lane;
-    for (; k + (int64_t)(UNROLL - 1) * lanes < sp.pieces; k += (int64_t)UNROLL * lanes) {
-        uint4 u[UNROLL];
+// U pieces of a span per lane, -inf behind its end
+template <typename T, int U> struct Batch { uint4 u[U]; };
+template <typename T, int U> __device__ __forceinline__ void load_batch(Batch<T, U> &b, const uint4 *body, int k, int lanes, int pieces) {
+    constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
 #pragma unroll
-        for (int i = 0; i < UNROLL; ++i) u[i] = __ldg(b + k + (int64_t)i * lanes);
-#pragma unroll
-        for (int i = 0; i < UNROLL; ++i) {
-            float v[E];
-            Piece<T>::unpack(u[i], v);
-            add_values<E>(m, s, v, c);
-        }
-    }
-    for (; k < sp.pieces; k += lanes) {
-        float v[E];
-        Piece<T>::unpack(__ldg(b + k), v);
-        add_values<E>(m, s, v, c);
-    }
+    for (int i = 0; i < U; ++i) b.u[i] = k + i * lanes < pieces ? __ldg(body + k + i * lanes) : make_uint4(none, none, none, none);
 }
 
-// The row's loss from its statistics, by L lanes that hold the same (m, s); writes the state, returns the loss in every lane.
-template <typename T, int L> __device__ __forceinline__ float row_loss(const Args &a, int64_t row, int lane, bool active, float m, float s, float &counted) {
-    const T *z = static_cast<const T *>(a.z) + row * a.ldz;
+// What a lane needs of a row before it can do anything is asked for in one go: its first pieces, its part of the elements
+// before and behind them (EDGE of them at most), its first entries.
+constexpr int HELD = 2;
+struct Entry { int64_t id; float t, z; };
+
+template <typename T> __device__ __forceinline__ void load_entry(Entry &e, const Args &a, int64_t row, int j) {
+    e.id = j < a.K ? id_at(a, row, j) : -1;
+    e.t = j < a.K ? teacher_at(a, row, j) : NEG_INF;
+}
+template <typename T> __device__ __forceinline__ void load_score(Entry &e, const Args &a, int64_t row) {
+    e.z = e.id >= 0 && e.id < a.V ? to_float(static_cast<const T *>(a.z)[row * a.ldz + e.id]) : 0.0f;
+}
+
+template <typename T, int LANES, int U> struct Front {
+    static constexpr int EDGE = (2 * (Piece<T>::E - 1) + LANES - 1) / LANES;
+    Batch<T, U> first;
+    float edge[EDGE];
+    __device__ __forceinline__ void load(const Span<T> &sp, int lane) {
+        load_batch(first, sp.body(), lane, LANES, (int)sp.pieces);
+#pragma unroll
+        for (int i = 0; i < EDGE; ++i) {
+            const int k = lane + i * LANES;
+            edge[i] = k < sp.head ? to_float(sp.p[k]) : k < sp.head + sp.tail ? to_float(sp.rest()[k - sp.head]) : NEG_INF;
+        }
+    }
+    // running statistics of the span; the next pieces are on their way while these are added
+    __device__ __forceinline__ void stats(const Span<T> &sp, int lane, float c, float &m, float &s) {
+        const int pieces = (int)sp.pieces;
+        Batch<T, U> cur = first;
+        for (int k = lane; k < pieces; k += U * LANES) {
+            Batch<T, U> next;
+            load_batch(next, sp.body(), k + U * LANES, LANES, pieces);
+            add_pieces<T, U>(m, s, cur.u, c);
+            cur = next;
+        }
+        add_values<EDGE>(m, s, edge, c);
+    }
+    // f exp((z - m) c) over the span; what the teacher's entries take off is put right behind it
+    __device__ __forceinline__ void grad(const Span<T> &sp, T *out, bool vector, int lane, float c, float m, float f) {
+        constexpr int E = Piece<T>::E;
+        const int pieces = (int)sp.pieces;
+        T *body = out + sp.head, *rest = body + sp.pieces * E;
+        Batch<T, U> cur = first;
+        for (int k = lane; k < pieces; k += U * LANES) {
+            Batch<T, U> next;
+            load_batch(next, sp.body(), k + U * LANES, LANES, pieces);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (k + i * LANES >= pieces) break;
+                float v[E];
+                Piece<T>::unpack(cur.u[i], v);
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = f * exp2_approx((v[e] - m) * c);
+                T *to = body + (int64_t)(k + i * LANES) * E;
+                if (vector) {
+                    *reinterpret_cast<uint4 *>(to) = Piece<T>::pack(v);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) to[e] = from_float<T>(v[e]);
+                }
+            }
+            cur = next;
+        }
+#pragma unroll
+        for (int i = 0; i < EDGE; ++i) {
+            const int k = lane + i * LANES;
+            const T v = from_float<T>(f * exp2_approx((edge[i] - m) * c));
+            if (k < sp.head) out[k] = v;
+            else if (k < sp.head + sp.tail) rest[k - sp.head] = v;
+        }
+    }
+};
+
+// true in every lane of a group of L if `flag` holds in one of them
+template <int L> __device__ __forceinline__ bool group_any(bool flag) {
+    const unsigned all = __ballot_sync(0xffffffffu, flag);
+    if (L == 32) return all != 0;
+    return (all >> ((threadIdx.x & 31) / L * L) & ((1u << (L & 31)) - 1u)) != 0;
+}
+
+// The row's loss from its statistics, by L lanes that hold the same (m, s) and the row's first entries; writes the state,
+// returns the loss in every lane.
+template <typename T, int L> __device__ __forceinline__ float row_loss(const Args &a, int64_t row, int lane, bool active, float m, float s,
+                                                                       const Entry (&held)[HELD], float &counted) {
+    auto entry = [&](int i) {
+        Entry e;
+        load_entry<T>(e, a, row, lane + i * L);
+        load_score<T>(e, a, row);
+        return e;
+    };
+    const int per_lane = active ? (a.K + L - 1) / L : 0;          // (the same in all lanes of the group)
     float tm = NEG_INF;
     bool any = false, bad = false;
-    if (active)
-        for (int j = lane; j < a.K; j += L) {
-            const int64_t id = id_at(a, row, j);
-            if (id < 0) continue;
-            const float t = teacher_at(a, row, j);
-            any |= t != NEG_INF;
-            bad |= id >= a.V;
-            tm = fmaxf(tm, t);
-        }
+    auto look = [&](const Entry &e) {
+        if (e.id < 0) return;
+        any |= e.t != NEG_INF;
+        bad |= e.id >= a.V;
+        tm = fmaxf(tm, e.t);
+    };
+    look(held[0]);
+    look(held[1]);
+    for (int i = HELD; i < per_lane; ++i) look(entry(i));
     tm = group_max<L>(tm);
-    any = group_max<L>(any ? 1.0f : 0.0f) > 0.0f;
-    bad = group_max<L>(bad ? 1.0f : 0.0f) > 0.0f;
+    any = group_any<L>(any);
+    bad = group_any<L>(bad);
     const float safe = finite_or_zero(tm);
     float ts = 0.0f;
-    if (active)
-        for (int j = lane; j < a.K; j += L)
-            if (id_at(a, row, j) >= 0) ts += exp2_approx((teacher_at(a, row, j) - safe) * a.c);
+    auto weigh = [&](const Entry &e) { if (e.id >= 0) ts += exp2_approx((e.t - safe) * a.c); };
+    weigh(held[0]);
+    weigh(held[1]);
+    for (int i = HELD; i < per_lane; ++i) weigh(entry(i));
     ts = group_sum<L>(ts);
     const float log_s = log2f(s), log_ts = log2f(ts);
     float l = 0.0f;
-    if (active && any && !bad)
-        for (int j = lane; j < a.K; j += L) {
-            const int64_t id = id_at(a, row, j);
-            if (id < 0) continue;
-            const float lp = (teacher_at(a, row, j) - safe) * a.c - log_ts, p = exp2_approx(lp);
-            const float lq = (to_float(z[id]) - m) * a.c - log_s;
-            if (p != 0.0f) l += p * (lp - lq);
-        }
+    auto take = [&](const Entry &e) {
+        if (e.id < 0) return;
+        const float lp = (e.t - safe) * a.c - log_ts, p = exp2_approx(lp);
+        if (p != 0.0f) l += p * (lp - ((e.z - m) * a.c - log_s));
+    };
+    if (any && !bad) {
+        take(held[0]);
+        take(held[1]);
+        for (int i = HELD; i < per_lane; ++i) take(entry(i));
+    }
     l = group_sum<L>(l) * (a.T * a.T * LN2);
     if (bad) { l = NAN; ts = NAN; }
     if (!any && !bad) ts = 0.0f;
@@ -161,14 +233,21 @@ template <typename T, int L> __global__ void __launch_bounds__(THREADS) short_fw
         const int64_t row = r0 + threadIdx.x / L;
         const bool active = row < a.n;
         float m = NEG_INF, s = 0.0f;
+        Entry held[HELD] = {{-1, NEG_INF, 0.0f}, {-1, NEG_INF, 0.0f}};
         if (active) {
-            const T *z = static_cast<const T *>(a.z) + row * a.ldz;
-            span_stats<T, 2>(Span<T>(z, 0, a.V), lane, L, a.c, m, s);
+            const Span<T> sp(static_cast<const T *>(a.z) + row * a.ldz, 0, a.V);
+            Front<T, L, L == 32 ? 4 : 2> front;
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) load_entry<T>(held[i], a, row, lane + i * L);
+            front.load(sp, lane);
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) load_score<T>(held[i], a, row);
+            front.stats(sp, lane, a.c, m, s);
         }
         const float top = group_max<L>(m);
         s = group_sum<L>(s * exp2_approx((m - finite_or_zero(top)) * a.c));
         float counted;
-        const float l = row_loss<T, L>(a, row, lane, active, top, s, counted);
+        const float l = row_loss<T, L>(a, row, lane, active, top, s, held, counted);
         if (lane == 0 && active) { sum += l; count += counted; }
     }
     if (a.reduction == RED_NONE) return;
@@ -182,63 +261,68 @@ __device__ __forceinline__ float row_factor(const Args &a, int64_t row, const fl
     return g * a.T;
 }
 
-// dz over a span: f (q - 0); what the teacher's entries take off is put right by fix_entries
-template <typename T, int UNROLL> __device__ __forceinline__ void span_grad(const Span<T> &in, T *out, bool vector, int lane, int lanes, float c,
-                                                                            float m, float f) {
-    constexpr int E = Piece<T>::E;
-    const int64_t body0 = in.head, rest0 = in.head + in.pieces * E;
-    for (int i = lane; i < in.head + in.tail; i += lanes) {
-        const int64_t at = i < in.head ? i : rest0 + (i - in.head);
-        out[at] = from_float<T>(f * exp2_approx((to_float(in.p[at]) - m) * c));
-    }
-    const uint4 *b = in.body();
-    int64_t k = lane;
-    for (; k < in.pieces; k += (int64_t)UNROLL * lanes) {
-        uint4 u[UNROLL];
+// A row's entries in shared memory, ids below 0 absent, each with its probability
+__device__ __forceinline__ void stage_entry(const Args &a, const Entry &e, int j, const float4 &st, float inv, int *ids, float *p) {
+    if (j >= a.K) return;
+    ids[j] = e.id < 0 || e.id >= a.V ? -1 : (int)e.id;
+    p[j] = e.id < 0 ? 0.0f : exp2_approx((e.t - st.z) * a.c) * inv;
+}
+
+// Class of an entry within [lo, hi): q minus the sum of all the row's entries of that class, so that an id that occurs several
+// times gets the same value from each
+template <typename T> __device__ __forceinline__ void fix_entry(const Args &a, const Entry &e, T *dz, const int *ids, const float *p, int64_t lo, int64_t hi,
+                                                                float m, float inv_s, float f) {
+    if (e.id < lo || e.id >= hi) return;          // (an absent one is below every lo)
+    float taken = 0.0f;
+    for (int i = 0; i < a.K; ++i) if (ids[i] == (int)e.id) taken += p[i];
+    dz[e.id] = from_float<T>(f * (exp2_approx((e.z - m) * a.c) * inv_s - taken));
+}
+
+// The gradient of the part [lo, hi) of a row by LANES threads; `sync` joins them.
+template <typename T, int LANES, int U, typename Sync> __device__ __forceinline__ void row_grad(const Args &a, int64_t row, int64_t lo, int64_t hi, int lane,
+                                                                                                 bool active, int *ids, float *p, Sync sync) {
+    const T *z = static_cast<const T *>(a.z) + (active ? row * a.ldz : 0);
+    T *dz = static_cast<T *>(a.dz) + (active ? row * a.ldo : 0);
+    float4 st = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
+    Entry held[HELD] = {{-1, NEG_INF, 0.0f}, {-1, NEG_INF, 0.0f}};
+    float f = 0.0f, inv_s = 0.0f;
+    bool has = false;
+    const int per_lane = (a.K + LANES - 1) / LANES;
+    auto later = [&](int i) {
+        Entry e;
+        load_entry<T>(e, a, row, lane + i * LANES);
+        load_score<T>(e, a, row);
+        return e;
+    };
+    if (active) {
+        const Span<T> sp(z + lo, 0, hi - lo);
+        Front<T, LANES, U> front;
+        st = a.state[row];
 #pragma unroll
-        for (int i = 0; i < UNROLL; ++i) if (k + (int64_t)i * lanes < in.pieces) u[i] = __ldg(b + k + (int64_t)i * lanes);
+        for (int i = 0; i < HELD; ++i) load_entry<T>(held[i], a, row, lane + i * LANES);
+        front.load(sp, lane);
 #pragma unroll
-        for (int i = 0; i < UNROLL; ++i) {
-            if (k + (int64_t)i * lanes >= in.pieces) break;
-            float v[E];
-            Piece<T>::unpack(u[i], v);
+        for (int i = 0; i < HELD; ++i) load_score<T>(held[i], a, row);
+        if (st.w != 0.0f) {
+            f = st.w != st.w ? NAN : row_factor(a, row, st);
+            inv_s = 1.0f / st.y;
+            has = st.w > 0.0f;
+            const float inv = 1.0f / st.w;
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = f * exp2_approx((v[e] - m) * c);
-            T *o = out + body0 + (k + (int64_t)i * lanes) * E;
-            if (vector) {
-                *reinterpret_cast<uint4 *>(o) = Piece<T>::pack(v);
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[e] = from_float<T>(v[e]);
-            }
+            for (int i = 0; i < HELD; ++i) stage_entry(a, held[i], lane + i * LANES, st, inv, ids, p);
+            for (int i = HELD; i < per_lane; ++i) stage_entry(a, later(i), lane + i * LANES, st, inv, ids, p);
+            front.grad(sp, dz + lo, ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15u) == 0, lane, a.c, st.x, f * inv_s);
+        } else {
+            for (int64_t i = lo + lane; i < hi; i += LANES) dz[i] = from_float<T>(0.0f);
         }
     }
-}
-
-// Classes of the teacher's entries within [lo, hi): q minus the sum of all the row's entries of that class, so that an id
-// that occurs several times gets the same value from each.  ids, p: the row's K entries in shared memory, ids below 0 absent.
-template <typename T> __device__ __forceinline__ void fix_entries(const Args &a, const T *z, T *dz, const int *ids, const float *p, int64_t lo, int64_t hi,
-                                                                  int lane, int lanes, float m, float inv_s, float f) {
-    for (int j = lane; j < a.K; j += lanes) {
-        const int id = ids[j];
-        if (id < lo || id >= hi) continue;
-        float taken = 0.0f;
-        for (int i = 0; i < a.K; ++i) if (ids[i] == id) taken += p[i];
-        dz[id] = from_float<T>(f * (exp2_approx((to_float(z[id]) - m) * a.c) * inv_s - taken));
+    sync();                                          // the stores and staged entries of all before the corrections
+    if (has) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) fix_entry<T>(a, held[i], dz, ids, p, lo, hi, st.x, inv_s, f);
+        for (int i = HELD; i < per_lane; ++i) fix_entry<T>(a, later(i), dz, ids, p, lo, hi, st.x, inv_s, f);
     }
-}
-
-__device__ __forceinline__ void stage_entries(const Args &a, int64_t row, const float4 &st, int *ids, float *p, int lane, int lanes) {
-    const float inv = 1.0f / st.w;
-    for (int j = lane; j < a.K; j += lanes) {
-        const int64_t id = id_at(a, row, j);
-        ids[j] = id < 0 || id >= a.V ? -1 : (int)id;
-        p[j] = id < 0 ? 0.0f : exp2_approx((teacher_at(a, row, j) - st.z) * a.c) * inv;
-    }
-}
-
-template <typename T> __device__ __forceinline__ bool same_offset(const T *in, const T *out) {
-    return ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+    sync();
 }
 
 template <typename T, int L> __global__ void __launch_bounds__(THREADS) short_bwd_kernel(const Args a) {
@@ -250,28 +334,7 @@ template <typename T, int L> __global__ void __launch_bounds__(THREADS) short_bw
     const int lane = threadIdx.x % L, group = threadIdx.x / L;
     for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.n; r0 += (int64_t)gridDim.x * ROWS) {
         const int64_t row = r0 + group;
-        const bool active = row < a.n;
-        const T *z = nullptr;
-        T *dz = nullptr;
-        float4 st = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
-        float f = 0.0f, inv_s = 0.0f;
-        if (active) {
-            z = static_cast<const T *>(a.z) + row * a.ldz;
-            dz = static_cast<T *>(a.dz) + row * a.ldo;
-            st = a.state[row];
-            f = row_factor(a, row, st);
-            inv_s = 1.0f / st.y;
-            if (st.w != 0.0f) {
-                if (st.w != st.w) f = NAN;
-                span_grad<T, 2>(Span<T>(z, 0, a.V), dz, same_offset(z, dz), lane, L, a.c, st.x, f * inv_s);
-                stage_entries(a, row, st, s_ids[group], s_p[group], lane, L);
-            } else {
-                for (int64_t i = lane; i < a.V; i += L) dz[i] = from_float<T>(0.0f);
-            }
-        }
-        __syncwarp();                                    // the group's stores and staged entries before its corrections
-        if (active && st.w > 0.0f) fix_entries<T>(a, z, dz, s_ids[group], s_p[group], 0, a.V, lane, L, st.x, inv_s, f);
-        __syncwarp();
+        row_grad<T, L, L == 32 ? 4 : 2>(a, row, 0, a.V, lane, row < a.n, s_ids[group], s_p[group], [] { __syncwarp(); });
     }
 }
 
@@ -289,7 +352,16 @@ template <typename T> __global__ void __launch_bounds__(THREADS) long_fwd_kernel
         const int64_t lo = split * a.part, hi = min(a.V, lo + a.part);
         float m = NEG_INF, s = 0.0f;
         const T *z = static_cast<const T *>(a.z) + row * a.ldz;
-        span_stats<T, 4>(Span<T>(z, lo, hi), threadIdx.x, THREADS, a.c, m, s);
+        Entry held[HELD] = {{-1, NEG_INF, 0.0f}, {-1, NEG_INF, 0.0f}};
+        const bool ends = warp == 0 && a.splits == 1;          // this warp takes the row's loss
+        const Span<T> sp(z, lo, hi);
+        Front<T, THREADS, 4> front;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) if (ends) load_entry<T>(held[i], a, row, lane + i * 32);
+        front.load(sp, threadIdx.x);
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) if (ends) load_score<T>(held[i], a, row);
+        front.stats(sp, threadIdx.x, a.c, m, s);
         float top = group_max<32>(m);
         s = group_sum<32>(s * exp2_approx((m - finite_or_zero(top)) * a.c));
         if (lane == 0) { red_m[warp] = top; red_s[warp] = s; }
@@ -301,7 +373,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) long_fwd_kernel
             s = group_sum<32>(s * exp2_approx((m - finite_or_zero(top)) * a.c));
             if (a.splits == 1) {
                 float counted;
-                sum += row_loss<T, 32>(a, row, lane, true, top, s, counted);
+                sum += row_loss<T, 32>(a, row, lane, true, top, s, held, counted);
                 count += counted;
             } else if (lane == 0) {
                 a.stats[(int64_t)split * a.n + row] = make_float2(top, s);
@@ -321,6 +393,9 @@ template <typename T> __global__ void __launch_bounds__(THREADS) join_fwd_kernel
     float sum = 0.0f, count = 0.0f;
     for (int64_t row = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); row < a.n; row += (int64_t)gridDim.x * (THREADS / 32)) {
         float m = NEG_INF, s = 0.0f;
+        Entry held[HELD];
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) { load_entry<T>(held[i], a, row, lane + i * 32); load_score<T>(held[i], a, row); }
         for (int i = lane; i < a.splits; i += 32) {
             const float2 p = a.stats[(int64_t)i * a.n + row];
             join_stats(m, s, p.x, p.y, a.c);
@@ -328,7 +403,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) join_fwd_kernel
         const float top = group_max<32>(m);
         s = group_sum<32>(s * exp2_approx((m - finite_or_zero(top)) * a.c));
         float counted;
-        const float l = row_loss<T, 32>(a, row, lane, true, top, s, counted);
+        const float l = row_loss<T, 32>(a, row, lane, true, top, s, held, counted);
         if (lane == 0) { sum += l; count += counted; }
     }
     if (a.reduction == RED_NONE) return;
@@ -343,33 +418,19 @@ template <typename T> __global__ void __launch_bounds__(THREADS) long_bwd_kernel
     __shared__ float s_p[MAX_KEPT];
     const int64_t items = a.n * a.splits;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t row = item / a.splits;
-        const int64_t lo = (item - row * a.splits) * a.part, hi = min(a.V, lo + a.part);
-        const T *z = static_cast<const T *>(a.z) + row * a.ldz;
-        T *dz = static_cast<T *>(a.dz) + row * a.ldo;
-        const float4 st = a.state[row];
-        const float inv_s = 1.0f / st.y;
-        float f = row_factor(a, row, st);
-        if (st.w == 0.0f) {
-            for (int64_t i = lo + threadIdx.x; i < hi; i += THREADS) dz[i] = from_float<T>(0.0f);
-        } else {
-            if (st.w != st.w) f = NAN;
-            stage_entries(a, row, st, s_ids, s_p, threadIdx.x, THREADS);
-            span_grad<T, 4>(Span<T>(z, lo, hi), dz + lo, same_offset(z, dz), threadIdx.x, THREADS, a.c, st.x, f * inv_s);
-        }
-        __syncthreads();
-        if (st.w > 0.0f) fix_entries<T>(a, z, dz, s_ids, s_p, lo, hi, threadIdx.x, THREADS, st.x, inv_s, f);
-        __syncthreads();
+        const int64_t row = item / a.splits, lo = (item - row * a.splits) * a.part;
+        row_grad<T, THREADS, 4>(a, row, lo, min(a.V, lo + a.part), threadIdx.x, true, s_ids, s_p, [] { __syncthreads(); });
     }
 }
 
 static int64_t grid_limit() { return (int64_t)sm_count() * CTAS_PER_SM; }
 
-static bool short_rows(int64_t V, int K) { return V <= SHORT_ROW && K <= SHORT_KEPT; }
-// lanes of a short row: about two 16-byte pieces each
+// A warp (or less) per row while that gives every SM 16 warps to run: no barrier, no idle warps at a row's end.
+static bool short_rows(int64_t n, int64_t V, int K) { return K <= SHORT_KEPT && (V <= 1024 || (V <= SHORT_ROW && n >= (int64_t)sm_count() * 16)); }
+// lanes of a short row: one or two 16-byte pieces each
 static int short_lanes(int64_t V, size_t es) {
     const int64_t pieces = ceil_div(V * (int64_t)es, (int64_t)16);
-    return pieces <= 8 ? 4 : pieces <= 16 ? 8 : pieces <= 32 ? 16 : 32;
+    return pieces <= 16 ? 8 : pieces <= 32 ? 16 : 32;
 }
 // Parts of a long row: as many as give every SM work, none shorter than SPLIT_MIN classes; part lengths are whole pieces.
 static void split_rows(int64_t n, int64_t V, int *splits, int64_t *part) {
@@ -402,10 +463,9 @@ template <typename T, int L> static int launch_short(const Args &a, bool fwd, in
 
 template <typename T> static int launch(Args a, bool fwd, float *loss, float *count, cudaStream_t st) {
     int64_t grid = 0;
-    if (short_rows(a.V, a.K)) {
+    if (short_rows(a.n, a.V, a.K)) {
         int rc;
         switch (short_lanes(a.V, sizeof(T))) {
-            case 4: rc = launch_short<T, 4>(a, fwd, &grid, st); break;
             case 8: rc = launch_short<T, 8>(a, fwd, &grid, st); break;
             case 16: rc = launch_short<T, 16>(a, fwd, &grid, st); break;
             default: rc = launch_short<T, 32>(a, fwd, &grid, st); break;
