@@ -22,13 +22,14 @@ constexpr int THREADS = 256;
 constexpr int CTAS_PER_SM = 8;
 constexpr int SHORT_ROW = 16384;         // classes up to which a group of lanes takes a row (else a CTA), given the rows
 constexpr int SHORT_KEPT = 64;           // entries that such a group holds in shared memory
+constexpr int LONG_HELD = 2;             // entries per lane of the warp that takes a long row's loss, loaded ahead
 constexpr int SPLIT_MIN = 4096;          // classes below which a row is not cut any further
 
 struct Args {
-    const void *z; int64_t ldz;
-    const void *t; int64_t ldt; int t_dtype;
-    const void *ids; int64_t ldi; int id_bytes;
-    int64_t n, V; int K;
+    const void *z; int ldz;              // 32-bit sizes and strides: a 64-bit product of two of them is one instruction
+    const void *t; int ldt, t_dtype;
+    const void *ids; int ldi, id_bytes;
+    int n, V, K;
     float c;                             // log2(e) / T
     float T;
     int reduction;
@@ -36,18 +37,18 @@ struct Args {
     float4 *state;                       // [n]: max z, sum exp((z - max) / T), max t, sum exp((t - max) / T); sum of t 0: no entry
     float2 *partial;                     // [grid] sums of (loss, counted rows)
     float2 *stats;                       // [splits][n] of rows cut into parts
-    int splits; int64_t part;            // parts of a row and their length
+    int splits, part;                    // parts of a row and their length
     const float *grad, *count;           // backward
-    void *dz; int64_t ldo;
+    void *dz; int ldo;
 };
 
-__device__ __forceinline__ float teacher_at(const Args &a, int64_t row, int j) {
-    const int64_t i = row * a.ldt + j;
+__device__ __forceinline__ float teacher_at(const Args &a, int row, int j) {
+    const int64_t i = (int64_t)row * a.ldt + j;
     if (a.t_dtype == GRWS_F32) return __ldg(static_cast<const float *>(a.t) + i);
     if (a.t_dtype == GRWS_F16) return to_float(static_cast<const __half *>(a.t)[i]);
     return to_float(static_cast<const __nv_bfloat16 *>(a.t)[i]);
 }
-__device__ __forceinline__ int64_t id_at(const Args &a, int64_t row, int j) { return load_index(a.ids, a.id_bytes, row * a.ldi + j); }
+__device__ __forceinline__ int64_t id_at(const Args &a, int row, int j) { return load_index(a.ids, a.id_bytes, (int64_t)row * a.ldi + j); }
 
 template <int L> __device__ __forceinline__ float group_max(float v) {
 #pragma unroll
@@ -60,19 +61,16 @@ template <int L> __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
-// The part [lo, hi) of a row that starts at p: elements before the first aligned address, whole pieces, the rest
+// `len` elements at p: those before the first aligned address, whole pieces, the rest
 template <typename T> struct Span {
     const T *p;
-    int64_t pieces;
-    int head, tail;
-    __device__ __forceinline__ Span(const T *row, int64_t lo, int64_t hi) {
+    int head, pieces, tail;
+    __device__ __forceinline__ Span(const T *start, int len) : p(start) {
         constexpr int E = Piece<T>::E;
-        p = row + lo;
-        const int64_t len = hi - lo;
-        const int off = (int)((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
-        head = (int)min((int64_t)((E - off) & (E - 1)), len);
+        const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15u) / (int)sizeof(T);
+        head = min((E - off) & (E - 1), len);
         pieces = (len - head) / E;
-        tail = (int)(len - head - pieces * E);
+        tail = len - head - pieces * E;
     }
     __device__ __forceinline__ const uint4 *body() const { return reinterpret_cast<const uint4 *>(p + head); }
     __device__ __forceinline__ const T *rest() const { return p + head + pieces * Piece<T>::E; }
@@ -86,25 +84,27 @@ template <typename T, int U> __device__ __forceinline__ void load_batch(Batch<T,
     for (int i = 0; i < U; ++i) b.u[i] = k + i * lanes < pieces ? __ldg(body + k + i * lanes) : make_uint4(none, none, none, none);
 }
 
-// What a lane needs of a row before it can do anything is asked for in one go: its first pieces, its part of the elements
-// before and behind them (EDGE of them at most), its first entries.
-constexpr int HELD = 2;
+// What a lane needs of a row before it can do anything is asked for in one go: its first U pieces, its part of the elements
+// before and behind them (EDGE of them at most), its first H entries.  Short rows are bound by their instructions (577 per
+// four rows of 47 classes when all had U = 2, EDGE = 2 and H = 2), so each size has its own.
 struct Entry { int64_t id; float t, z; };
 
-template <typename T> __device__ __forceinline__ void load_entry(Entry &e, const Args &a, int64_t row, int j) {
+template <typename T> __device__ __forceinline__ void load_entry(Entry &e, const Args &a, int row, int j) {
     e.id = j < a.K ? id_at(a, row, j) : -1;
     e.t = j < a.K ? teacher_at(a, row, j) : NEG_INF;
+    if (e.id >= a.V) e.t = NAN;          // makes the row's sum NaN, and with it its loss and gradient
 }
-template <typename T> __device__ __forceinline__ void load_score(Entry &e, const Args &a, int64_t row) {
-    e.z = e.id >= 0 && e.id < a.V ? to_float(static_cast<const T *>(a.z)[row * a.ldz + e.id]) : 0.0f;
+template <typename T> __device__ __forceinline__ void load_score(Entry &e, const Args &a, int row) {
+    e.z = e.id >= 0 && e.id < a.V ? to_float(static_cast<const T *>(a.z)[(int64_t)row * a.ldz + e.id]) : 0.0f;
 }
 
-template <typename T, int LANES, int U> struct Front {
-    static constexpr int EDGE = (2 * (Piece<T>::E - 1) + LANES - 1) / LANES;
+template <typename T> constexpr int edge_elements(int lanes, bool aligned) { return ((aligned ? 1 : 2) * (Piece<T>::E - 1) + lanes - 1) / lanes; }
+
+template <typename T, int LANES, int U, int EDGE> struct Front {
     Batch<T, U> first;
     float edge[EDGE];
     __device__ __forceinline__ void load(const Span<T> &sp, int lane) {
-        load_batch(first, sp.body(), lane, LANES, (int)sp.pieces);
+        load_batch(first, sp.body(), lane, LANES, sp.pieces);
 #pragma unroll
         for (int i = 0; i < EDGE; ++i) {
             const int k = lane + i * LANES;
@@ -113,11 +113,12 @@ template <typename T, int LANES, int U> struct Front {
     }
     // running statistics of the span; the next pieces are on their way while these are added
     __device__ __forceinline__ void stats(const Span<T> &sp, int lane, float c, float &m, float &s) {
-        const int pieces = (int)sp.pieces;
+        const int pieces = sp.pieces;
         Batch<T, U> cur = first;
-        for (int k = lane; k < pieces; k += U * LANES) {
+        for (int k = lane; k < pieces;) {
             Batch<T, U> next;
-            load_batch(next, sp.body(), k + U * LANES, LANES, pieces);
+            k += U * LANES;
+            if (LANES >= 32 || k < pieces) load_batch(next, sp.body(), k, LANES, pieces);
             add_pieces<T, U>(m, s, cur.u, c);
             cur = next;
         }
@@ -126,12 +127,12 @@ template <typename T, int LANES, int U> struct Front {
     // f exp((z - m) c) over the span; what the teacher's entries take off is put right behind it
     __device__ __forceinline__ void grad(const Span<T> &sp, T *out, bool vector, int lane, float c, float m, float f) {
         constexpr int E = Piece<T>::E;
-        const int pieces = (int)sp.pieces;
-        T *body = out + sp.head, *rest = body + sp.pieces * E;
+        const int pieces = sp.pieces;
+        T *body = out + sp.head, *rest = body + pieces * E;
         Batch<T, U> cur = first;
         for (int k = lane; k < pieces; k += U * LANES) {
             Batch<T, U> next;
-            load_batch(next, sp.body(), k + U * LANES, LANES, pieces);
+            if (LANES >= 32 || k + U * LANES < pieces) load_batch(next, sp.body(), k + U * LANES, LANES, pieces);
 #pragma unroll
             for (int i = 0; i < U; ++i) {
                 if (k + i * LANES >= pieces) break;
@@ -139,7 +140,7 @@ template <typename T, int LANES, int U> struct Front {
                 Piece<T>::unpack(cur.u[i], v);
 #pragma unroll
                 for (int e = 0; e < E; ++e) v[e] = f * exp2_approx((v[e] - m) * c);
-                T *to = body + (int64_t)(k + i * LANES) * E;
+                T *to = body + (k + i * LANES) * E;
                 if (vector) {
                     *reinterpret_cast<uint4 *>(to) = Piece<T>::pack(v);
                 } else {
@@ -159,17 +160,10 @@ template <typename T, int LANES, int U> struct Front {
     }
 };
 
-// true in every lane of a group of L if `flag` holds in one of them
-template <int L> __device__ __forceinline__ bool group_any(bool flag) {
-    const unsigned all = __ballot_sync(0xffffffffu, flag);
-    if (L == 32) return all != 0;
-    return (all >> ((threadIdx.x & 31) / L * L) & ((1u << (L & 31)) - 1u)) != 0;
-}
-
 // The row's loss from its statistics, by L lanes that hold the same (m, s) and the row's first entries; writes the state,
 // returns the loss in every lane.
-template <typename T, int L> __device__ __forceinline__ float row_loss(const Args &a, int64_t row, int lane, bool active, float m, float s,
-                                                                       const Entry (&held)[HELD], float &counted) {
+template <typename T, int L, int H> __device__ __forceinline__ float row_loss(const Args &a, int row, int lane, bool active, float m, float s,
+                                                                       const Entry (&held)[H], float &counted) {
     auto entry = [&](int i) {
         Entry e;
         load_entry<T>(e, a, row, lane + i * L);
@@ -178,25 +172,17 @@ template <typename T, int L> __device__ __forceinline__ float row_loss(const Arg
     };
     const int per_lane = active ? (a.K + L - 1) / L : 0;          // (the same in all lanes of the group)
     float tm = NEG_INF;
-    bool any = false, bad = false;
-    auto look = [&](const Entry &e) {
-        if (e.id < 0) return;
-        any |= e.t != NEG_INF;
-        bad |= e.id >= a.V;
-        tm = fmaxf(tm, e.t);
-    };
-    look(held[0]);
-    look(held[1]);
-    for (int i = HELD; i < per_lane; ++i) look(entry(i));
+    auto look = [&](const Entry &e) { if (e.id >= 0) tm = fmaxf(tm, e.t); };
+#pragma unroll
+    for (int i = 0; i < H; ++i) look(held[i]);
+    for (int i = H; i < per_lane; ++i) look(entry(i));
     tm = group_max<L>(tm);
-    any = group_any<L>(any);
-    bad = group_any<L>(bad);
     const float safe = finite_or_zero(tm);
     float ts = 0.0f;
     auto weigh = [&](const Entry &e) { if (e.id >= 0) ts += exp2_approx((e.t - safe) * a.c); };
-    weigh(held[0]);
-    weigh(held[1]);
-    for (int i = HELD; i < per_lane; ++i) weigh(entry(i));
+#pragma unroll
+    for (int i = 0; i < H; ++i) weigh(held[i]);
+    for (int i = H; i < per_lane; ++i) weigh(entry(i));
     ts = group_sum<L>(ts);
     const float log_s = log2f(s), log_ts = log2f(ts);
     float l = 0.0f;
@@ -205,15 +191,13 @@ template <typename T, int L> __device__ __forceinline__ float row_loss(const Arg
         const float lp = (e.t - safe) * a.c - log_ts, p = exp2_approx(lp);
         if (p != 0.0f) l += p * (lp - ((e.z - m) * a.c - log_s));
     };
-    if (any && !bad) {
-        take(held[0]);
-        take(held[1]);
-        for (int i = HELD; i < per_lane; ++i) take(entry(i));
+    if (ts != 0.0f) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) take(held[i]);
+        for (int i = H; i < per_lane; ++i) take(entry(i));
     }
     l = group_sum<L>(l) * (a.T * a.T * LN2);
-    if (bad) { l = NAN; ts = NAN; }
-    if (!any && !bad) ts = 0.0f;
-    counted = any || bad ? 1.0f : 0.0f;
+    counted = ts != 0.0f ? 1.0f : 0.0f;          // no entry, or none of any weight: the sum is 0
     if (active && lane == 0) {
         a.state[row] = make_float4(m, s, safe, ts);
         if (a.reduction == RED_NONE) a.loss[row] = l;
@@ -222,7 +206,7 @@ template <typename T, int L> __device__ __forceinline__ float row_loss(const Arg
 }
 
 // ---- rows of up to SHORT_ROW classes: L lanes a row, the losses of a block's rows summed ----
-template <typename T, int L> __global__ void __launch_bounds__(THREADS) short_fwd_kernel(const Args a) {
+template <typename T, int L, int U, int EDGE, int H> __global__ void __launch_bounds__(THREADS) short_fwd_kernel(const Args a) {
     wait_for_previous();
     let_next_start();
     __shared__ float red[64];
@@ -230,24 +214,26 @@ template <typename T, int L> __global__ void __launch_bounds__(THREADS) short_fw
     constexpr int ROWS = THREADS / L;
     float sum = 0.0f, count = 0.0f;
     for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.n; r0 += (int64_t)gridDim.x * ROWS) {
-        const int64_t row = r0 + threadIdx.x / L;
-        const bool active = row < a.n;
+        const bool active = r0 + threadIdx.x / L < a.n;
+        const int row = (int)r0 + threadIdx.x / L;
         float m = NEG_INF, s = 0.0f;
-        Entry held[HELD] = {{-1, NEG_INF, 0.0f}, {-1, NEG_INF, 0.0f}};
-        if (active) {
-            const Span<T> sp(static_cast<const T *>(a.z) + row * a.ldz, 0, a.V);
-            Front<T, L, L == 32 ? 4 : 2> front;
+        Entry held[H];
 #pragma unroll
-            for (int i = 0; i < HELD; ++i) load_entry<T>(held[i], a, row, lane + i * L);
+        for (int i = 0; i < H; ++i) held[i] = {-1, NEG_INF, 0.0f};
+        if (active) {
+            const Span<T> sp(static_cast<const T *>(a.z) + (int64_t)row * a.ldz, a.V);
+            Front<T, L, U, EDGE> front;
+#pragma unroll
+            for (int i = 0; i < H; ++i) load_entry<T>(held[i], a, row, lane + i * L);
             front.load(sp, lane);
 #pragma unroll
-            for (int i = 0; i < HELD; ++i) load_score<T>(held[i], a, row);
+            for (int i = 0; i < H; ++i) load_score<T>(held[i], a, row);
             front.stats(sp, lane, a.c, m, s);
         }
         const float top = group_max<L>(m);
         s = group_sum<L>(s * exp2_approx((m - finite_or_zero(top)) * a.c));
         float counted;
-        const float l = row_loss<T, L>(a, row, lane, active, top, s, held, counted);
+        const float l = row_loss<T, L, H>(a, row, lane, active, top, s, held, counted);
         if (lane == 0 && active) { sum += l; count += counted; }
     }
     if (a.reduction == RED_NONE) return;
@@ -255,7 +241,7 @@ template <typename T, int L> __global__ void __launch_bounds__(THREADS) short_fw
     if (threadIdx.x == 0) a.partial[blockIdx.x] = make_float2(sum, count);
 }
 
-__device__ __forceinline__ float row_factor(const Args &a, int64_t row, const float4 &st) {
+__device__ __forceinline__ float row_factor(const Args &a, int row, const float4 &st) {
     if (st.w == 0.0f) return 0.0f;
     const float g = a.reduction == RED_NONE ? __ldg(a.grad + row) : loss_factor(a.grad, a.count, a.reduction);
     return g * a.T;
@@ -270,7 +256,7 @@ __device__ __forceinline__ void stage_entry(const Args &a, const Entry &e, int j
 
 // Class of an entry within [lo, hi): q minus the sum of all the row's entries of that class, so that an id that occurs several
 // times gets the same value from each
-template <typename T> __device__ __forceinline__ void fix_entry(const Args &a, const Entry &e, T *dz, const int *ids, const float *p, int64_t lo, int64_t hi,
+template <typename T> __device__ __forceinline__ void fix_entry(const Args &a, const Entry &e, T *dz, const int *ids, const float *p, int lo, int hi,
                                                                 float m, float inv_s, float f) {
     if (e.id < lo || e.id >= hi) return;          // (an absent one is below every lo)
     float taken = 0.0f;
@@ -279,12 +265,14 @@ template <typename T> __device__ __forceinline__ void fix_entry(const Args &a, c
 }
 
 // The gradient of the part [lo, hi) of a row by LANES threads; `sync` joins them.
-template <typename T, int LANES, int U, typename Sync> __device__ __forceinline__ void row_grad(const Args &a, int64_t row, int64_t lo, int64_t hi, int lane,
+template <typename T, int LANES, int U, int EDGE, int H, typename Sync> __device__ __forceinline__ void row_grad(const Args &a, int row, int lo, int hi, int lane,
                                                                                                  bool active, int *ids, float *p, Sync sync) {
-    const T *z = static_cast<const T *>(a.z) + (active ? row * a.ldz : 0);
-    T *dz = static_cast<T *>(a.dz) + (active ? row * a.ldo : 0);
+    const T *z = static_cast<const T *>(a.z) + (active ? (int64_t)row * a.ldz : 0);
+    T *dz = static_cast<T *>(a.dz) + (active ? (int64_t)row * a.ldo : 0);
     float4 st = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
-    Entry held[HELD] = {{-1, NEG_INF, 0.0f}, {-1, NEG_INF, 0.0f}};
+    Entry held[H];
+#pragma unroll
+    for (int i = 0; i < H; ++i) held[i] = {-1, NEG_INF, 0.0f};
     float f = 0.0f, inv_s = 0.0f;
     bool has = false;
     const int per_lane = (a.K + LANES - 1) / LANES;
@@ -295,37 +283,37 @@ template <typename T, int LANES, int U, typename Sync> __device__ __forceinline_
         return e;
     };
     if (active) {
-        const Span<T> sp(z + lo, 0, hi - lo);
-        Front<T, LANES, U> front;
+        const Span<T> sp(z + lo, hi - lo);
+        Front<T, LANES, U, EDGE> front;
         st = a.state[row];
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) load_entry<T>(held[i], a, row, lane + i * LANES);
+        for (int i = 0; i < H; ++i) load_entry<T>(held[i], a, row, lane + i * LANES);
         front.load(sp, lane);
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) load_score<T>(held[i], a, row);
+        for (int i = 0; i < H; ++i) load_score<T>(held[i], a, row);
         if (st.w != 0.0f) {
             f = st.w != st.w ? NAN : row_factor(a, row, st);
             inv_s = 1.0f / st.y;
             has = st.w > 0.0f;
             const float inv = 1.0f / st.w;
 #pragma unroll
-            for (int i = 0; i < HELD; ++i) stage_entry(a, held[i], lane + i * LANES, st, inv, ids, p);
-            for (int i = HELD; i < per_lane; ++i) stage_entry(a, later(i), lane + i * LANES, st, inv, ids, p);
+            for (int i = 0; i < H; ++i) stage_entry(a, held[i], lane + i * LANES, st, inv, ids, p);
+            for (int i = H; i < per_lane; ++i) stage_entry(a, later(i), lane + i * LANES, st, inv, ids, p);
             front.grad(sp, dz + lo, ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15u) == 0, lane, a.c, st.x, f * inv_s);
         } else {
-            for (int64_t i = lo + lane; i < hi; i += LANES) dz[i] = from_float<T>(0.0f);
+            for (int i = lo + lane; i < hi; i += LANES) dz[i] = from_float<T>(0.0f);
         }
     }
     sync();                                          // the stores and staged entries of all before the corrections
     if (has) {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) fix_entry<T>(a, held[i], dz, ids, p, lo, hi, st.x, inv_s, f);
-        for (int i = HELD; i < per_lane; ++i) fix_entry<T>(a, later(i), dz, ids, p, lo, hi, st.x, inv_s, f);
+        for (int i = 0; i < H; ++i) fix_entry<T>(a, held[i], dz, ids, p, lo, hi, st.x, inv_s, f);
+        for (int i = H; i < per_lane; ++i) fix_entry<T>(a, later(i), dz, ids, p, lo, hi, st.x, inv_s, f);
     }
     sync();
 }
 
-template <typename T, int L> __global__ void __launch_bounds__(THREADS) short_bwd_kernel(const Args a) {
+template <typename T, int L, int U, int EDGE, int H> __global__ void __launch_bounds__(THREADS) short_bwd_kernel(const Args a) {
     wait_for_previous();
     let_next_start();
     constexpr int ROWS = THREADS / L;
@@ -333,8 +321,9 @@ template <typename T, int L> __global__ void __launch_bounds__(THREADS) short_bw
     __shared__ float s_p[ROWS][SHORT_KEPT];
     const int lane = threadIdx.x % L, group = threadIdx.x / L;
     for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.n; r0 += (int64_t)gridDim.x * ROWS) {
-        const int64_t row = r0 + group;
-        row_grad<T, L, L == 32 ? 4 : 2>(a, row, 0, a.V, lane, row < a.n, s_ids[group], s_p[group], [] { __syncwarp(); });
+        const bool active = r0 + group < a.n;
+        const int row = (int)r0 + group;
+        row_grad<T, L, U, EDGE, H>(a, row, 0, a.V, lane, active, s_ids[group], s_p[group], [] { __syncwarp(); });
     }
 }
 
@@ -345,22 +334,26 @@ template <typename T> __global__ void __launch_bounds__(THREADS) long_fwd_kernel
     __shared__ float red_m[THREADS / 32], red_s[THREADS / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     float sum = 0.0f, count = 0.0f;
-    const int64_t items = a.n * a.splits;
+    const int64_t items = (int64_t)a.n * a.splits;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t row = item / a.splits;
-        const int split = (int)(item - row * a.splits);
-        const int64_t lo = split * a.part, hi = min(a.V, lo + a.part);
+        const int row = (int)(item / a.splits);
+        const int split = (int)(item - (int64_t)row * a.splits);
+        const int lo = split * a.part, hi = min(a.V, lo + a.part);
         float m = NEG_INF, s = 0.0f;
-        const T *z = static_cast<const T *>(a.z) + row * a.ldz;
-        Entry held[HELD] = {{-1, NEG_INF, 0.0f}, {-1, NEG_INF, 0.0f}};
+        const T *z = static_cast<const T *>(a.z) + (int64_t)row * a.ldz;
+        Entry held[LONG_HELD];
         const bool ends = warp == 0 && a.splits == 1;          // this warp takes the row's loss
-        const Span<T> sp(z, lo, hi);
-        Front<T, THREADS, 4> front;
+        const Span<T> sp(z + lo, hi - lo);
+        Front<T, THREADS, 4, 1> front;
+        if (ends) {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) if (ends) load_entry<T>(held[i], a, row, lane + i * 32);
+            for (int i = 0; i < LONG_HELD; ++i) load_entry<T>(held[i], a, row, lane + i * 32);
+        }
         front.load(sp, threadIdx.x);
+        if (ends) {
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) if (ends) load_score<T>(held[i], a, row);
+            for (int i = 0; i < LONG_HELD; ++i) load_score<T>(held[i], a, row);
+        }
         front.stats(sp, threadIdx.x, a.c, m, s);
         float top = group_max<32>(m);
         s = group_sum<32>(s * exp2_approx((m - finite_or_zero(top)) * a.c));
@@ -373,7 +366,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) long_fwd_kernel
             s = group_sum<32>(s * exp2_approx((m - finite_or_zero(top)) * a.c));
             if (a.splits == 1) {
                 float counted;
-                sum += row_loss<T, 32>(a, row, lane, true, top, s, held, counted);
+                sum += row_loss<T, 32, LONG_HELD>(a, row, lane, true, top, s, held, counted);
                 count += counted;
             } else if (lane == 0) {
                 a.stats[(int64_t)split * a.n + row] = make_float2(top, s);
@@ -391,11 +384,12 @@ template <typename T> __global__ void __launch_bounds__(THREADS) join_fwd_kernel
     __shared__ float red[64];
     const int lane = threadIdx.x & 31;
     float sum = 0.0f, count = 0.0f;
-    for (int64_t row = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); row < a.n; row += (int64_t)gridDim.x * (THREADS / 32)) {
+    for (int64_t r = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); r < a.n; r += (int64_t)gridDim.x * (THREADS / 32)) {
+        const int row = (int)r;
         float m = NEG_INF, s = 0.0f;
-        Entry held[HELD];
+        Entry held[LONG_HELD];
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) { load_entry<T>(held[i], a, row, lane + i * 32); load_score<T>(held[i], a, row); }
+        for (int i = 0; i < LONG_HELD; ++i) { load_entry<T>(held[i], a, row, lane + i * 32); load_score<T>(held[i], a, row); }
         for (int i = lane; i < a.splits; i += 32) {
             const float2 p = a.stats[(int64_t)i * a.n + row];
             join_stats(m, s, p.x, p.y, a.c);
@@ -403,7 +397,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) join_fwd_kernel
         const float top = group_max<32>(m);
         s = group_sum<32>(s * exp2_approx((m - finite_or_zero(top)) * a.c));
         float counted;
-        const float l = row_loss<T, 32>(a, row, lane, true, top, s, held, counted);
+        const float l = row_loss<T, 32, LONG_HELD>(a, row, lane, true, top, s, held, counted);
         if (lane == 0) { sum += l; count += counted; }
     }
     if (a.reduction == RED_NONE) return;
@@ -416,10 +410,11 @@ template <typename T> __global__ void __launch_bounds__(THREADS) long_bwd_kernel
     let_next_start();
     __shared__ int s_ids[MAX_KEPT];
     __shared__ float s_p[MAX_KEPT];
-    const int64_t items = a.n * a.splits;
+    const int64_t items = (int64_t)a.n * a.splits;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t row = item / a.splits, lo = (item - row * a.splits) * a.part;
-        row_grad<T, THREADS, 4>(a, row, lo, min(a.V, lo + a.part), threadIdx.x, true, s_ids, s_p, [] { __syncthreads(); });
+        const int row = (int)(item / a.splits);
+        const int lo = (int)(item - (int64_t)row * a.splits) * a.part;
+        row_grad<T, THREADS, 4, 1, 1>(a, row, lo, min(a.V, lo + a.part), threadIdx.x, true, s_ids, s_p, [] { __syncthreads(); });
     }
 }
 
@@ -427,25 +422,20 @@ static int64_t grid_limit() { return (int64_t)sm_count() * CTAS_PER_SM; }
 
 // A warp (or less) per row while that gives every SM 16 warps to run: no barrier, no idle warps at a row's end.
 static bool short_rows(int64_t n, int64_t V, int K) { return K <= SHORT_KEPT && (V <= 1024 || (V <= SHORT_ROW && n >= (int64_t)sm_count() * 16)); }
-// lanes of a short row: one or two 16-byte pieces each
-static int short_lanes(int64_t V, size_t es) {
-    const int64_t pieces = ceil_div(V * (int64_t)es, (int64_t)16);
-    return pieces <= 16 ? 8 : pieces <= 32 ? 16 : 32;
-}
 // Parts of a long row: as many as give every SM work, none shorter than SPLIT_MIN classes; part lengths are whole pieces.
-static void split_rows(int64_t n, int64_t V, int *splits, int64_t *part) {
+static void split_rows(int64_t n, int64_t V, int *splits, int *part) {
     int64_t s = ceil_div(grid_limit() / 2, n > 0 ? n : 1);
     const int64_t most = V / SPLIT_MIN;
     if (s > most) s = most;
     if (s < 1) s = 1;
-    *part = ceil_div(ceil_div(V, s), (int64_t)64) * 64;
-    *splits = (int)ceil_div(V, *part);
+    const int64_t p = ceil_div(ceil_div(V, s), (int64_t)64) * 64;
+    *part = (int)(p < V ? p : V);
+    *splits = (int)ceil_div(V, p);
 }
 
 struct Layout { size_t partial, stats, bytes; };
 static Layout layout(int64_t n, int64_t V) {
-    int splits;
-    int64_t part;
+    int splits, part;
     split_rows(n, V, &splits, &part);
     Layout l;
     l.partial = 0;
@@ -454,29 +444,35 @@ static Layout layout(int64_t n, int64_t V) {
     return l;
 }
 
-template <typename T, int L> static int launch_short(const Args &a, bool fwd, int64_t *grid, cudaStream_t st) {
-    int64_t g = ceil_div(a.n, (int64_t)(THREADS / L));
+template <typename T, int L, int U, int EDGE> static int launch_short(const Args &a, bool fwd, int64_t *grid, cudaStream_t st) {
+    int64_t g = ceil_div((int64_t)a.n, (int64_t)(THREADS / L));
     if (g > grid_limit()) g = grid_limit();
     *grid = g;
-    return launch_next(fwd ? short_fwd_kernel<T, L> : short_bwd_kernel<T, L>, dim3((unsigned)g), THREADS, 0, st, 1, a);
+    void (*kernel)(const Args) = a.K <= L ? (fwd ? short_fwd_kernel<T, L, U, EDGE, 1> : short_bwd_kernel<T, L, U, EDGE, 1>)
+                                          : (fwd ? short_fwd_kernel<T, L, U, EDGE, 2> : short_bwd_kernel<T, L, U, EDGE, 2>);
+    return launch_next(kernel, dim3((unsigned)g), THREADS, 0, st, 1, a);
+}
+
+// lanes of a short row: one or two 16-byte pieces each, four at a time for a warp
+template <typename T> static int launch_short_rows(const Args &a, bool fwd, int64_t *grid, cudaStream_t st) {
+    const int64_t pieces = ceil_div(a.V * (int64_t)sizeof(T), (int64_t)16);
+    const bool aligned = aligned16(a.z) && a.ldz * (int64_t)sizeof(T) % 16 == 0;
+    if (pieces <= 8) return aligned ? launch_short<T, 8, 1, edge_elements<T>(8, true)>(a, fwd, grid, st) : launch_short<T, 8, 1, edge_elements<T>(8, false)>(a, fwd, grid, st);
+    if (pieces <= 16) return aligned ? launch_short<T, 8, 2, edge_elements<T>(8, true)>(a, fwd, grid, st) : launch_short<T, 8, 2, edge_elements<T>(8, false)>(a, fwd, grid, st);
+    if (pieces <= 32) return launch_short<T, 16, 2, 1>(a, fwd, grid, st);
+    return launch_short<T, 32, 4, 1>(a, fwd, grid, st);
 }
 
 template <typename T> static int launch(Args a, bool fwd, float *loss, float *count, cudaStream_t st) {
     int64_t grid = 0;
     if (short_rows(a.n, a.V, a.K)) {
-        int rc;
-        switch (short_lanes(a.V, sizeof(T))) {
-            case 8: rc = launch_short<T, 8>(a, fwd, &grid, st); break;
-            case 16: rc = launch_short<T, 16>(a, fwd, &grid, st); break;
-            default: rc = launch_short<T, 32>(a, fwd, &grid, st); break;
-        }
-        if (rc != GRWS_OK) return rc;
+        if (int rc = launch_short_rows<T>(a, fwd, &grid, st)) return rc;
     } else {
         split_rows(a.n, a.V, &a.splits, &a.part);
-        grid = a.n * a.splits < grid_limit() ? a.n * a.splits : grid_limit();
+        grid = (int64_t)a.n * a.splits < grid_limit() ? (int64_t)a.n * a.splits : grid_limit();
         if (int rc = launch_next(fwd ? long_fwd_kernel<T> : long_bwd_kernel<T>, dim3((unsigned)grid), THREADS, 0, st, 1, a)) return rc;
         if (fwd && a.splits > 1) {
-            grid = ceil_div(a.n, (int64_t)(THREADS / 32));
+            grid = ceil_div((int64_t)a.n, (int64_t)(THREADS / 32));
             if (grid > grid_limit()) grid = grid_limit();
             if (int rc = launch_next(join_fwd_kernel<T>, dim3((unsigned)grid), THREADS, 0, st, 1, a)) return rc;
         }
@@ -489,7 +485,7 @@ template <typename T> static int launch(Args a, bool fwd, float *loss, float *co
 
 static int check(int64_t n, int64_t V, int64_t K, int64_t ldz, int64_t ldt, int64_t ldi, int dtype, int t_dtype, int id_bytes, float T, int reduction) {
     GRWS_REQUIRE(n >= 0 && V > 0 && K > 0, "bad size (rows = %lld, classes = %lld, kept = %lld)", (long long)n, (long long)V, (long long)K);
-    GRWS_REQUIRE(V <= INT32_MAX && n <= INT32_MAX, "rows and classes must fit 31 bits");
+    GRWS_REQUIRE(V <= INT32_MAX && n <= INT32_MAX && ldz <= INT32_MAX && ldt <= INT32_MAX && ldi <= INT32_MAX, "rows, classes and strides must fit 31 bits");
     if (K > MAX_KEPT) return fail(GRWS_ERR_UNSUPPORTED, "at most %d teacher entries per row (kept = %lld)", MAX_KEPT, (long long)K);
     GRWS_REQUIRE(ldz >= V && ldt >= K && ldi >= K, "leading dimension smaller than the row");
     if (dtype < GRWS_F32 || dtype > GRWS_BF16) return fail(GRWS_ERR_UNSUPPORTED, "bad dtype %d", dtype);
@@ -532,9 +528,9 @@ int grws_distill_fwd(const void *logits, int64_t ldz, int dtype, const void *tea
     const distill::Layout l = distill::layout(rows, classes);
     if (scratch_bytes < l.bytes) return fail(GRWS_ERR_SCRATCH, "distillation scratch too small");
     distill::Args a = {};
-    a.z = logits; a.ldz = ldz; a.t = teacher; a.ldt = ldt; a.t_dtype = teacher_dtype; a.ids = ids; a.ldi = ldi; a.id_bytes = id_bytes;
-    a.n = rows; a.V = classes; a.K = (int)kept; a.T = temperature; a.c = cls::LOG2E / temperature; a.reduction = reduction;
-    a.loss = loss; a.state = reinterpret_cast<float4 *>(state); a.splits = 1; a.part = classes;
+    a.z = logits; a.ldz = (int)ldz; a.t = teacher; a.ldt = (int)ldt; a.t_dtype = teacher_dtype; a.ids = ids; a.ldi = (int)ldi; a.id_bytes = id_bytes;
+    a.n = (int)rows; a.V = (int)classes; a.K = (int)kept; a.T = temperature; a.c = cls::LOG2E / temperature; a.reduction = reduction;
+    a.loss = loss; a.state = reinterpret_cast<float4 *>(state); a.splits = 1; a.part = (int)classes;
     a.partial = reinterpret_cast<float2 *>(static_cast<char *>(scratch) + l.partial);
     a.stats = reinterpret_cast<float2 *>(static_cast<char *>(scratch) + l.stats);
     switch (dtype) {
@@ -550,16 +546,16 @@ int grws_distill_bwd(const void *logits, int64_t ldz, int dtype, const void *tea
                      const float *grad_loss, const float *state, const float *count, void *dlogits, int64_t ldo, void *stream) {
     int rc = distill::check(rows, classes, kept, ldz, ldt, ldi, dtype, teacher_dtype, id_bytes, temperature, reduction);
     if (rc != GRWS_OK) return rc;
-    GRWS_REQUIRE(ldo >= classes, "leading dimension smaller than the row");
+    GRWS_REQUIRE(ldo >= classes && ldo <= INT32_MAX, "leading dimension smaller than the row");
     if (rows == 0) return GRWS_OK;
     GRWS_REQUIRE(logits && teacher && ids && grad_loss && state && dlogits, "null pointer");
     GRWS_REQUIRE(reduction != cls::RED_MEAN || count, "null pointer");
     GRWS_REQUIRE(aligned16(state), "state must be 16-byte aligned");
     distill::Args a = {};
-    a.z = logits; a.ldz = ldz; a.t = teacher; a.ldt = ldt; a.t_dtype = teacher_dtype; a.ids = ids; a.ldi = ldi; a.id_bytes = id_bytes;
-    a.n = rows; a.V = classes; a.K = (int)kept; a.T = temperature; a.c = cls::LOG2E / temperature; a.reduction = reduction;
-    a.state = reinterpret_cast<float4 *>(const_cast<float *>(state)); a.splits = 1; a.part = classes;
-    a.grad = grad_loss; a.count = count; a.dz = dlogits; a.ldo = ldo;
+    a.z = logits; a.ldz = (int)ldz; a.t = teacher; a.ldt = (int)ldt; a.t_dtype = teacher_dtype; a.ids = ids; a.ldi = (int)ldi; a.id_bytes = id_bytes;
+    a.n = (int)rows; a.V = (int)classes; a.K = (int)kept; a.T = temperature; a.c = cls::LOG2E / temperature; a.reduction = reduction;
+    a.state = reinterpret_cast<float4 *>(const_cast<float *>(state)); a.splits = 1; a.part = (int)classes;
+    a.grad = grad_loss; a.count = count; a.dz = dlogits; a.ldo = (int)ldo;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (dtype) {
         case GRWS_F32: return distill::launch<float>(a, false, nullptr, nullptr, st);
