@@ -95,6 +95,30 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
+// Two fp32 numbers per instruction
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// exp2((a - m) c), exp2((b - m) c) with minus_m = (-m, -m) and cc = (c, c)
+__device__ __forceinline__ uint64_t exp2_pair(float a, float b, uint64_t minus_m, uint64_t cc) {
+    float x, y;
+    unpair2(mul2(add2(pair2(a, b), minus_m), cc), x, y);
+    return pair2(exp2_approx(x), exp2_approx(y));
+}
+
 // Running maximum m and sum s = sum exp(scale * (x - m)) of a part of a row, scale * ln 2 in `c`.  A part without entries,
 // or of entries that are all -inf, is (-inf, 0); subtracting 0 instead of -inf keeps its exponentials at 0.
 __device__ __forceinline__ float finite_or_zero(float m) { return m == NEG_INF ? 0.0f : m; }
@@ -107,22 +131,32 @@ __device__ __forceinline__ void join_stats(float &m, float &s, float m2, float s
 
 // (up to four chains of maxima and of sums: one chain's latency would be most of the time)
 template <int N> __device__ __forceinline__ void add_values(float &m, float &s, const float (&v)[N], float c) {
-    constexpr int W = N >= 16 ? 4 : N >= 4 ? 2 : 1;
-    float top[W], t[W];
+    if constexpr (N < 16) {
+        float top = m, t = 0.0f;
 #pragma unroll
-    for (int j = 0; j < W; ++j) { top[j] = v[j]; t[j] = 0.0f; }
+        for (int i = 0; i < N; ++i) top = fmaxf(top, v[i]);
+        const float safe = finite_or_zero(top);
+        if (top != m) { s *= exp2_approx((m - safe) * c); m = top; }
 #pragma unroll
-    for (int i = W; i < N; ++i) top[i % W] = fmaxf(top[i % W], v[i]);
+        for (int i = 0; i < N; ++i) t += exp2_approx((v[i] - safe) * c);
+        s += t;
+    } else {
+        float top[4];
+        uint64_t t[4];
 #pragma unroll
-    for (int j = 1; j < W; ++j) top[0] = fmaxf(top[0], top[j]);
-    top[0] = fmaxf(top[0], m);
-    const float safe = finite_or_zero(top[0]);
-    if (top[0] != m) { s *= exp2_approx((m - safe) * c); m = top[0]; }
+        for (int j = 0; j < 4; ++j) { top[j] = v[j]; t[j] = 0; }
 #pragma unroll
-    for (int i = 0; i < N; ++i) t[i % W] += exp2_approx((v[i] - safe) * c);
+        for (int i = 4; i < N; ++i) top[i % 4] = fmaxf(top[i % 4], v[i]);
+        top[0] = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), m);
+        const float safe = finite_or_zero(top[0]);
+        if (top[0] != m) { s *= exp2_approx((m - safe) * c); m = top[0]; }
+        const uint64_t minus = pair2(-safe, -safe), cc = pair2(c, c);
 #pragma unroll
-    for (int j = 1; j < W; ++j) t[0] += t[j];
-    s += t[0];
+        for (int i = 0; i < N; i += 2) t[i / 2 % 4] = add2(t[i / 2 % 4], exp2_pair(v[i], v[i + 1], minus, cc));
+        float a, b;
+        unpair2(add2(add2(t[0], t[1]), add2(t[2], t[3])), a, b);
+        s += a + b;
+    }
 }
 
 // the same for N pieces of a row as loaded.  (c v - c max would be one instruction instead of two, but is off by 2^-24 of
@@ -131,18 +165,21 @@ template <typename T, int N> __device__ __forceinline__ void add_pieces(float &m
     constexpr int E = Piece<T>::E;
     const float top = fmaxf(m, largest<T, N>(u)), safe = finite_or_zero(top);
     if (top != m) { s *= exp2_approx((m - safe) * c); m = top; }
-    float t[N];
+    const uint64_t minus = pair2(-safe, -safe), cc = pair2(c, c);
+    uint64_t t[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         float v[E];
         Piece<T>::unpack(u[i], v);
-        t[i] = 0.0f;
+        t[i] = exp2_pair(v[0], v[1], minus, cc);
 #pragma unroll
-        for (int e = 0; e < E; ++e) t[i] += exp2_approx((v[e] - safe) * c);
+        for (int e = 2; e < E; e += 2) t[i] = add2(t[i], exp2_pair(v[e], v[e + 1], minus, cc));
     }
 #pragma unroll
-    for (int i = 1; i < N; ++i) t[0] += t[i];
-    s += t[0];
+    for (int i = 1; i < N; ++i) t[0] = add2(t[0], t[i]);
+    float x, y;
+    unpair2(t[0], x, y);
+    s += x + y;
 }
 
 // Kernels of one call follow each other as programmatic dependents: the next one is launched while this one still runs, sets

@@ -21,6 +21,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <limits.h>
 
 #include "class_loss.cuh"
 
@@ -33,6 +34,7 @@ constexpr int BM = 128, BN = 256, BK = 64;          // rows per CTA, columns per
 constexpr int EPILOGUE_WARPS = 8, TMA_WARP = 8, MMA_WARP = 9, THREADS = 320;
 constexpr long long WAIT_LIMIT_CYCLES = 3000000000ll;   // about 1.5 to 2.5 s of SM clocks
 constexpr int MAX_TASKS = 2;
+constexpr int PIECE_BYTES = 64 * BK * 2;                // 64 of the outer axis of an operand: what one copy brings of B
 constexpr int BOX_BYTES = 32 * 128;                     // what a warp stores at once: 32 rows of 64 16-bit or 32 fp32 numbers
 constexpr int SUB_STAGES = 2;                           // fp32: stages of the big pair that are summed in tensor memory
 
@@ -50,14 +52,14 @@ enum : int { WAIT_OPERANDS = 1, WAIT_STAGE = 2, WAIT_ACCUMULATOR = 3, WAIT_TILE 
 struct Task {
     int m_tiles, n_tiles, run, runs;      // a unit is one m tile and `run` n tiles
     int splits, k_blocks, k_len;          // parts of the inner axis, 64-element blocks in all and per part
-    int bn;                               // columns per tile (a multiple of 32 CG)
+    int bn;                               // columns per tile: a multiple of 64, or all of them in 32s
     int group;                            // m tiles side by side in the order of the units
     int a_outer, b_outer;                 // operand's outer axis contiguous
     int b_row0, b_k0;                     // first column / inner element of B within its tensor map
     int64_t M, N;
-    // SUM: partial sums [splits][M][] in fp32 (added to what is there if `add`), or the rounded output, through the map of
-    // the outputs; `out` with rows of ldo where its rows are no multiple of 16 bytes apart
-    int rounded, add, out_dtype;
+    // SUM: partial sums [splits][M][] in fp32 (added to what is there if `add`), or the output rounded to the operands' type,
+    // through the map of the outputs; or to `out` with rows of ldo, where these are no multiple of 16 bytes apart
+    int rounded, add;
     void *out; int64_t ldo;
     __host__ __device__ int units() const { return m_tiles * runs * splits; }
 };
@@ -65,6 +67,7 @@ struct Task {
 struct Params {
     Task task[MAX_TASKS];
     int tasks;
+    int deal, deal_less, deal_more;       // see Walk
     int bf16;
     // STATS, GRAD
     const void *labels; int label_bytes;
@@ -151,6 +154,7 @@ template <int CG> __device__ __forceinline__ void tma_load(uint32_t dst, const C
         asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];"
                      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 // box of shared memory to its place in the output (what lies outside is dropped), or added to it
 __device__ __forceinline__ void tma_store(const CUtensorMap *map, uint32_t src, int x, int y, int z) {
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
@@ -231,6 +235,10 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, int outer) {
 // order of the units: groups of `group` m tiles, within a group the n runs one after the other, so that the CTAs at work share
 // the columns of B; parts of the inner axis outermost
 // ---------------------------------------------------------------------------------------------
+// columns that the MMA computes of a tile: the last one's in 32s (other tiles are multiples of 64, so that no box of 64 reaches
+// into the next tile)
+__device__ __forceinline__ int tile_columns(const Task &t, int n) { return (int)min((int64_t)t.bn, (t.N - (int64_t)n * t.bn + 31) & ~(int64_t)31); }
+
 struct Unit { int task, m, n0, n1, split; };
 __device__ __forceinline__ Unit unit_at(const Params &p, int u) {
     Unit r;
@@ -248,6 +256,35 @@ __device__ __forceinline__ Unit unit_at(const Params &p, int u) {
     r.n1 = min(t.n_tiles, r.n0 + t.run);
     return r;
 }
+
+// The units of one CTA (pair) in order: every `ctas`-th one; or, where `deal` is set, every ctas-th of the first task and then
+// of the second as many as leave all busy equally long: CTAs with one unit less of the first start on them `early` rounds sooner.
+struct Walk {
+    int u, step, left, end, phase, units, ctas, cta, many, early, rounds, second;
+    __device__ __forceinline__ Walk(const Params &p, int all, int first, int n) : u(first - n), step(n), left(INT_MAX), end(all), phase(2), units(all), ctas(n),
+                                                                                 cta(first), many(0), early(0), rounds(0), second(0) {
+        if (!p.deal) return;
+        end = second = p.task[0].units();
+        phase = 0;
+        many = end % n;                                     // CTAs that have one unit more of the first task
+        early = p.deal_more - p.deal_less;
+        rounds = p.deal_less;
+    }
+    __device__ __forceinline__ bool next() {
+        for (;;) {
+            if (left > 0) {
+                --left;
+                u += step;
+                if (u < end) return true;
+            }
+            if (phase == 2) return false;
+            const int others = ctas - many;
+            if (phase++ == 0) { step = others; left = cta >= many ? early : 0; u = second + cta - many - step; }
+            else { step = ctas; left = rounds; u = second + early * others + cta - step; }
+            end = units;
+        }
+    }
+};
 
 struct Shared {
     uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
@@ -308,6 +345,10 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
         for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&ss->acc_full[i]), 1); mbar_init(smem_u32(&ss->acc_empty[i]), EPILOGUE_WARPS * CG); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == TMA_WARP && lane < p.tasks) {
+        prefetch_map(&maps.a[lane]);
+        prefetch_map(&maps.b[lane]);
+    }
     if (warp == MMA_WARP) {
         tmem_alloc<CG>(smem_u32(&ss->tmem));
         tmem_relinquish<CG>();
@@ -323,36 +364,45 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
 
     if (warp == TMA_WARP) {
         if (elect_one()) {
-            // the pair's copies all count on the barrier of its first CTA, whose MMA warp issues for both
+            // the pair's copies all count on the barriers of its first CTA, whose MMA warp issues for both.  (This thread's
+            // instructions between a stage's release and its copies are time in which nothing is on the way.)
             int stage = 0, issued = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int u = first; ok && u < units; u += stride) {
-                const Unit w = unit_at(p, u);
+            uint32_t full0 = smem_u32(&ss->full[0]);
+            if constexpr (CG == 2) full0 = map_to_rank(full0, 0);
+            constexpr int B_PIECES = BN / CG / 64;
+            for (Walk walk(p, units, first, stride); ok && walk.next();) {
+                const Unit w = unit_at(p, walk.u);
                 const Task &t = p.task[w.task];
                 const CUtensorMap *ma = &maps.a[w.task], *mb = &maps.b[w.task];
-                const int k0 = w.split * t.k_len, k1 = min(t.k_blocks, k0 + t.k_len);
+                const int k0 = w.split * t.k_len, k1 = min(t.k_blocks, k0 + t.k_len), b_k0 = t.b_k0;
                 const int a_row = (w.m * CG + (int)rank) * BM;
+                const bool a_outer = t.a_outer, b_outer = t.b_outer;
                 for (int n = w.n0; ok && n < w.n1; ++n) {
-                    const int b_row = t.b_row0 + n * t.bn + (int)rank * (t.bn / CG);
+                    const int cols = tile_columns(t, n) / CG, b_row = t.b_row0 + n * t.bn + (int)rank * cols;
+                    const int pieces = b_outer ? (cols + 63) >> 6 : B_PIECES;
+                    const uint32_t bytes = CG * (C::A_BYTES + pieces * PIECE_BYTES);
                     for (int pair = SPLIT ? 0 : 5; ok && pair < 6; ++pair) {
                         const int pa = pair == 0 ? 2 : pair == 2 || pair == 3 ? 1 : 0, pb = pair == 1 ? 2 : pair == 2 || pair == 4 ? 1 : 0;
                         for (int kb = k0; kb < k1; ++kb) {
                             if (!mbar_wait(smem_u32(&ss->empty[stage]), phase ^ 1u, abort_flag, limit)) { give_up(ss, p, WAIT_STAGE); ok = false; break; }
-                            uint32_t bar = smem_u32(&ss->full[stage]);
-                            if (rank == 0) mbar_expect_tx(bar, CG * C::STAGE_BYTES);
-                            if constexpr (CG == 2) bar = map_to_rank(bar, 0);
-                            const uint32_t a = ring + stage * C::STAGE_BYTES, b = a + C::A_BYTES;
-                            const int ka = kb * BK, kB = t.b_k0 + kb * BK;
-                            if (t.a_outer) {
-                                for (int j = 0; j < BM / 64; ++j) tma_load<CG>(a + j * (64 * BK * 2), ma, bar, a_row + j * 64, ka, pa);
+                            const uint32_t bar = full0 + stage * 8, a = ring + stage * C::STAGE_BYTES, b = a + C::A_BYTES;
+                            const int ka = kb * BK, kB = b_k0 + ka;
+                            if (rank == 0) mbar_expect_tx(smem_u32(&ss->full[stage]), bytes);
+                            if (a_outer) {
+#pragma unroll
+                                for (int j = 0; j < BM / 64; ++j) tma_load<CG>(a + j * PIECE_BYTES, ma, bar, a_row + j * 64, ka, pa);
                             } else {
                                 tma_load<CG>(a, ma, bar, ka, a_row, pa);
                             }
-                            if (t.b_outer) {
-                                for (int j = 0; j < BN / CG / 64; ++j) tma_load<CG>(b + j * (64 * BK * 2), mb, bar, b_row + j * 64, kB, pb);
-                            } else {
+                            if (!b_outer) {
                                 tma_load<CG>(b, mb, bar, kB, b_row, pb);
+                            } else if (pieces == B_PIECES) {
+#pragma unroll
+                                for (int j = 0; j < B_PIECES; ++j) tma_load<CG>(b + j * PIECE_BYTES, mb, bar, b_row + j * 64, kB, pb);
+                            } else {
+                                for (int j = 0; j < pieces; ++j) tma_load<CG>(b + j * PIECE_BYTES, mb, bar, b_row + j * 64, kB, pb);
                             }
                             ++issued;
                             if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
@@ -377,15 +427,16 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
             int stage = 0;
             uint32_t phase = 0, tile = 0;
             bool ok = true;
-            for (int u = first; ok && u < units; u += stride) {
-                const Unit w = unit_at(p, u);
+            for (Walk walk(p, units, first, stride); ok && walk.next();) {
+                const Unit w = unit_at(p, walk.u);
                 const Task &t = p.task[w.task];
                 const int k0 = w.split * t.k_len, steps = (min(t.k_blocks, k0 + t.k_len) - k0) * (SPLIT ? 6 : 1);
-                const uint32_t idesc = (1u << 4) | ((uint32_t)p.bf16 << 7) | ((uint32_t)p.bf16 << 10) | ((uint32_t)t.a_outer << 15) |
-                                       ((uint32_t)t.b_outer << 16) | ((uint32_t)(t.bn >> 3) << 17) | ((uint32_t)(BM * CG >> 4) << 24);
+                const uint32_t idesc0 = (1u << 4) | ((uint32_t)p.bf16 << 7) | ((uint32_t)p.bf16 << 10) | ((uint32_t)t.a_outer << 15) |
+                                        ((uint32_t)t.b_outer << 16) | ((uint32_t)(BM * CG >> 4) << 24);
                 const uint64_t a_step = t.a_outer ? 2048 >> 4 : 32 >> 4, b_step = t.b_outer ? 2048 >> 4 : 32 >> 4;
                 const int small = SPLIT ? steps / 6 * 5 : 0;
                 for (int n = w.n0; ok && n < w.n1; ++n) {
+                    const uint32_t idesc = idesc0 | ((uint32_t)(tile_columns(t, n) >> 3) << 17);
                     // sums of the tile: all steps, or for fp32 the small pairs' and SUB_STAGES steps each of the big one's
                     for (int k0s = 0; ok && k0s < steps; ++tile) {
                         const int k1s = !SPLIT ? steps : k0s < small ? small : min(steps, k0s + SUB_STAGES);
@@ -453,8 +504,9 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                 bulk_commit();
             }
         };
-        for (int u = first; ok && u < units; u += stride) {
-            const Unit w = unit_at(p, u);
+        [[maybe_unused]] const float alpha = MODE == SUM ? grad_alpha(p) * p.scale : 0.0f;
+        for (Walk walk(p, units, first, stride); ok && walk.next();) {
+            const Unit w = unit_at(p, walk.u);
             const Task &t = p.task[w.task];
             const CUtensorMap *mc = &maps.c[w.task];
             const int row0 = (w.m * CG + (int)rank) * BM + quarter * 32;
@@ -474,23 +526,25 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                 }
                 if (label == p.ignore_index) label = -1;
             }
-            if constexpr (MODE == SUM) factor = t.rounded ? grad_alpha(p) * p.scale : 1.0f;
+            if constexpr (MODE == SUM) factor = t.rounded ? alpha : 1.0f;
             for (int n = w.n0; ok && n < w.n1; ++n) {
                 const int64_t col0 = (int64_t)n * t.bn;
                 const int cols = (int)min((int64_t)t.bn, t.N - col0);          // of this tile
                 const int mine = (int)max((int64_t)-1, min((int64_t)BN, label - p.v0 - col0));    // label's column, if within
                 (void)mine;
-                // W columns from c on: 64, for fp32 32
-                constexpr int W = SPLIT ? 32 : 64;
-                auto put16 = [&](const float (&v)[W]) {
+                // W columns from c on: 64, for fp32 16
+                constexpr int W = SPLIT ? 16 : 64;
+                auto put16 = [&](const float (&v)[W], uint32_t mask) {
                     if (p.bf16) {
 #pragma unroll
                         for (int i = 0; i < W; i += 8)
-                            put(i / 8, pack2<true>(v[i], v[i + 1]), pack2<true>(v[i + 2], v[i + 3]), pack2<true>(v[i + 4], v[i + 5]), pack2<true>(v[i + 6], v[i + 7]));
+                            put(i / 8, pack2<true>(v[i], v[i + 1]) & mask, pack2<true>(v[i + 2], v[i + 3]) & mask, pack2<true>(v[i + 4], v[i + 5]) & mask,
+                                pack2<true>(v[i + 6], v[i + 7]) & mask);
                     } else {
 #pragma unroll
                         for (int i = 0; i < W; i += 8)
-                            put(i / 8, pack2<false>(v[i], v[i + 1]), pack2<false>(v[i + 2], v[i + 3]), pack2<false>(v[i + 4], v[i + 5]), pack2<false>(v[i + 6], v[i + 7]));
+                            put(i / 8, pack2<false>(v[i], v[i + 1]) & mask, pack2<false>(v[i + 2], v[i + 3]) & mask, pack2<false>(v[i + 4], v[i + 5]) & mask,
+                                pack2<false>(v[i + 6], v[i + 7]) & mask);
                     }
                 };
                 auto use = [&](float (&v)[W], int c) {
@@ -508,67 +562,85 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                         add_values<W>(m, s, v, LOG2E);
                     } else if constexpr (MODE == GRAD) {
                         const bool has = __any_sync(0xffffffffu, mine >= c && mine < c + W);
+                        const uint64_t minus = pair2(-m, -m), cc = pair2(LOG2E, LOG2E), ww = pair2(weight, weight);
 #pragma unroll
-                        for (int i = 0; i < W; ++i) v[i] = exp2_approx((v[i] - m) * LOG2E) * weight;
+                        for (int i = 0; i < W; i += 2) unpair2(mul2(exp2_pair(v[i], v[i + 1], minus, cc), ww), v[i], v[i + 1]);
                         if (has) {
 #pragma unroll
                             for (int i = 0; i < W; ++i) if (mine == c + i) v[i] -= factor;
                         }
-                        if (factor == 0.0f) {
-#pragma unroll
-                            for (int i = 0; i < W; ++i) v[i] = 0.0f;
-                        }
+                        box_free();
                         if constexpr (!SPLIT) {
-                            box_free();
-                            put16(v);
+                            put16(v, factor == 0.0f ? 0u : ~0u);
                             box_out(mc, (int)col0 + c, row0, 0, false);
                         } else {
-                            // lines of 64 bytes, not swizzled: 64 columns would keep too much in registers
+                            // the three planes of 16 columns: boxes of 32-byte lines
+                            if (factor == 0.0f) {
 #pragma unroll
-                            for (int k = 0; k < 3; ++k) {
-                                uint32_t q[W / 2];
+                                for (int i = 0; i < W; ++i) v[i] = 0.0f;
+                            }
 #pragma unroll
-                                for (int i = 0; i < W; i += 2) {
+                            for (int i = 0; i < W; i += 8) {
+                                uint32_t q[3][4];
+#pragma unroll
+                                for (int j = 0; j < 8; j += 2) {
                                     float a[2], b[2], d[2];
-                                    split3(v[i], a[0], b[0], d[0]);
-                                    split3(v[i + 1], a[1], b[1], d[1]);
-                                    q[i / 2] = k == 0 ? pack2<true>(a[0], a[1]) : k == 1 ? pack2<true>(b[0], b[1]) : pack2<true>(d[0], d[1]);
+                                    split3(v[i + j], a[0], b[0], d[0]);
+                                    split3(v[i + j + 1], a[1], b[1], d[1]);
+                                    q[0][j / 2] = pack2<true>(a[0], a[1]);
+                                    q[1][j / 2] = pack2<true>(b[0], b[1]);
+                                    q[2][j / 2] = pack2<true>(d[0], d[1]);
                                 }
-                                box_free();
 #pragma unroll
-                                for (int j = 0; j < W / 8; ++j) st_shared16(box + lane * 64 + j * 16, q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
-                                box_out(mc, (int)col0 + c, row0, k, false);
+                                for (int k = 0; k < 3; ++k) st_shared16(box + k * 1024 + lane * 32 + i * 2, q[k][0], q[k][1], q[k][2], q[k][3]);
+                            }
+                            fence_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+#pragma unroll
+                                for (int k = 0; k < 3; ++k) tma_store(mc, box + k * 1024, (int)col0 + c, row0, k);
+                                bulk_commit();
                             }
                         }
                     } else {
 #pragma unroll
                         for (int i = 0; i < W; ++i) v[i] *= factor;
-                        if (!SPLIT && t.rounded && t.out_dtype != GRWS_F32) {
-                            box_free();
-                            put16(v);
-                            if (!t.out) { box_out(mc, (int)col0 + c, row0, 0, false); return; }
-                            __syncwarp();
-                            for (int r = 0; r < 32 && row0 + r < t.M; ++r) {
-                                const uint32_t two = ld_shared32(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-                                uint16_t *o = static_cast<uint16_t *>(t.out) + (row0 + r) * t.ldo + col0 + c + lane * 2;
-                                if (c + lane * 2 < cols) o[0] = (uint16_t)two;
-                                if (c + lane * 2 + 1 < cols) o[1] = (uint16_t)(two >> 16);
+                        if constexpr (!SPLIT) {
+                            if (t.rounded) {
+                                box_free();
+                                put16(v, ~0u);
+                                if (!t.out) { box_out(mc, (int)col0 + c, row0, 0, false); return; }
+                                __syncwarp();
+                                for (int r = 0; r < 32 && row0 + r < t.M; ++r) {
+                                    const uint32_t two = ld_shared32(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                                    uint16_t *o = static_cast<uint16_t *>(t.out) + (row0 + r) * t.ldo + col0 + c + lane * 2;
+                                    if (c + lane * 2 < cols) o[0] = (uint16_t)two;
+                                    if (c + lane * 2 + 1 < cols) o[1] = (uint16_t)(two >> 16);
+                                }
+                                __syncwarp();
+                                return;
                             }
-                            __syncwarp();
-                            return;
-                        }
 #pragma unroll
-                        for (int h = 0; h < W; h += 32) {
-                            if (c + h >= cols) return;
+                            for (int h = 0; h < W; h += 32) {
+                                if (c + h >= cols) return;
+                                box_free();
+#pragma unroll
+                                for (int i = 0; i < 32; i += 4)
+                                    put(i / 4, __float_as_uint(v[h + i]), __float_as_uint(v[h + i + 1]), __float_as_uint(v[h + i + 2]), __float_as_uint(v[h + i + 3]));
+                                box_out(mc, (int)col0 + c + h, row0, w.split, t.add);
+                            }
+                        } else {
+                            // 16 fp32 columns: lines of 64 bytes
                             box_free();
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4)
-                                put(i / 4, __float_as_uint(v[h + i]), __float_as_uint(v[h + i + 1]), __float_as_uint(v[h + i + 2]), __float_as_uint(v[h + i + 3]));
-                            if (!t.out) { box_out(mc, (int)col0 + c + h, row0, w.split, t.add); continue; }
+                            for (int i = 0; i < W; i += 4)
+                                st_shared16(box + lane * 64 + i * 4, __float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]));
+                            if (!t.out) { box_out(mc, (int)col0 + c, row0, w.split, t.add); return; }
                             __syncwarp();
-                            for (int r = 0; r < 32 && row0 + r < t.M; ++r) {
-                                const uint32_t one = ld_shared32(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-                                if (c + h + lane < cols) static_cast<float *>(t.out)[(row0 + r) * t.ldo + col0 + c + h + lane] = __uint_as_float(one);
+                            for (int r = 0; r < 32 && row0 + r < t.M; r += 2) {
+                                const int rr = r + (lane >> 4), cc = lane & 15;
+                                if (row0 + rr < t.M && c + cc < cols)
+                                    static_cast<float *>(t.out)[(row0 + rr) * t.ldo + col0 + c + cc] = __uint_as_float(ld_shared32(box + rr * 64 + cc * 4));
                             }
                             __syncwarp();
                         }
@@ -593,29 +665,26 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                     }
                 } else {
                     const int k0 = w.split * t.k_len, big = min(t.k_blocks, k0 + t.k_len) - k0;
-                    float acc[4][32];
+                    float acc[8][W];
                     for (int sub = 0; ok && sub <= (big + SUB_STAGES - 1) / SUB_STAGES; ++sub) {
                         const uint32_t at = wait_tile();
                         if (!ok) break;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int c = half * 64 + (k >> 1) * 128 + (k & 1) * 32;
+                        for (int k = 0; k < 8; ++k) {
+                            const int c = half * 64 + (k >> 2) * 128 + (k & 3) * 16;
                             if (c >= cols) continue;
+                            uint32_t r[16];
+                            tmem_ld16(at + c, r);
+                            tmem_ld_wait();
 #pragma unroll
-                            for (int h = 0; h < 32; h += 16) {
-                                uint32_t r[16];
-                                tmem_ld16(at + c + h, r);
-                                tmem_ld_wait();
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) acc[k][h + i] = sub ? acc[k][h + i] + __uint_as_float(r[i]) : __uint_as_float(r[i]);
-                            }
+                            for (int i = 0; i < 16; ++i) acc[k][i] = sub ? acc[k][i] + __uint_as_float(r[i]) : __uint_as_float(r[i]);
                         }
                         release_tile();
                     }
                     if (!ok) break;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int c = half * 64 + (k >> 1) * 128 + (k & 1) * 32;
+                    for (int k = 0; k < 8; ++k) {
+                        const int c = half * 64 + (k >> 2) * 128 + (k & 3) * 16;
                         if (c < cols) use(acc[k], c);
                     }
                 }

@@ -129,6 +129,7 @@ template <typename T, int LANES, int U, int EDGE> struct Front {
         constexpr int E = Piece<T>::E;
         const int pieces = sp.pieces;
         T *body = out + sp.head, *rest = body + pieces * E;
+        const uint64_t minus = pair2(-m, -m), cc = pair2(c, c), ff = pair2(f, f);
         Batch<T, U> cur = first;
         for (int k = lane; k < pieces; k += U * LANES) {
             Batch<T, U> next;
@@ -139,7 +140,7 @@ template <typename T, int LANES, int U, int EDGE> struct Front {
                 float v[E];
                 Piece<T>::unpack(cur.u[i], v);
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = f * exp2_approx((v[e] - m) * c);
+                for (int e = 0; e < E; e += 2) unpair2(mul2(exp2_pair(v[e], v[e + 1], minus, cc), ff), v[e], v[e + 1]);
                 T *to = body + (k + i * LANES) * E;
                 if (vector) {
                     *reinterpret_cast<uint4 *>(to) = Piece<T>::pack(v);

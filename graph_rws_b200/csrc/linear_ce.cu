@@ -371,48 +371,66 @@ static void cut(int64_t tiles, int64_t K, int64_t least, int64_t unit, int64_t *
     *parts = ceil_div(K > 0 ? K : 1, *len);
 }
 
-static int columns_per_tile(int64_t N, int cg) {
+static int64_t in_32s(int64_t N) { return ceil_div(N, (int64_t)32) * 32; }
+static int columns_per_tile(int64_t N) {
     const int64_t tiles = ceil_div(N, (int64_t)prod::BN);
-    return (int)(ceil_div(ceil_div(N, tiles), (int64_t)(32 * cg)) * 32 * cg);
+    return (int)(tiles == 1 ? in_32s(N) : ceil_div(ceil_div(N, tiles), (int64_t)64) * 64);
 }
+static int64_t tiles_of(int64_t M, int64_t N, int cg) { return ceil_div(M, (int64_t)(prod::BM * cg)) * ceil_div(N, (int64_t)prod::BN); }
 // CTAs that share a tile: pairs where there are more rows than one CTA's
 static int cta_group(int64_t M) { return M > prod::BM ? 2 : 1; }
 
 static bool needs_packing(const void *p, int64_t ld, int dtype) { return dtype == GRWS_F32 || !aligned16(p) || ld % 8 != 0; }
 
-// Class tiles that one unit of the forward pass takes: as many as leave the SMs equally busy; every part is a statistic per
-// row (of two warps each) written and read at some 5 TB/s, and a step of the loop that joins them; a tile step takes about 0.4 us
-static void cut_runs(int64_t n, int64_t m_tiles, int64_t n_tiles, int64_t steps, int64_t ctas, int64_t *run, int64_t *runs) {
+// Class tiles that one unit of the scores takes: as many as leave the SMs equally busy.  A tile step takes about 0.4 us; a unit
+// costs the latency of its rows' data (0.8 us) and, forward, a statistic per row (of two warps each) written and read at some
+// 5 TB/s and a step of the loop that joins them.
+static void cut_runs(int64_t n, int64_t m_tiles, int64_t n_tiles, int64_t steps, int64_t ctas, bool forward, int64_t *run, int64_t *runs) {
     int64_t best = 1;
     double best_us = 1e300;
     for (int64_t r = 1; r <= n_tiles && r <= 64; ++r) {
         const int64_t k = ceil_div(n_tiles, r);
-        const double us = (double)(ceil_div(m_tiles * k, ctas) * r * steps) * 0.4 + (double)(k * n) * 32.0 / 5.0e6 + 0.06 * (double)k;
+        const double us = (double)ceil_div(m_tiles * k, ctas) * ((double)(r * steps) * 0.4 + 0.8) + (forward ? (double)(k * n) * 32.0 / 5.0e6 + 0.06 * (double)k : 0.0);
         if (us <= best_us) { best_us = us; best = r; }
     }
     *run = best;
     *runs = ceil_div(n_tiles, best);
 }
 
-// Parts of the inner axes of dx (classes of a piece) and dw (rows), which run in one launch: a unit should be short against the
-// launch, since units are dealt out round robin, but every part is one more plane of fp32 sums through memory.  Costs are in
-// units of one 64-element step of one tile, about 0.4 us of a pair of SMs; a launch that adds planes up takes some 3 us.
+// What a unit of `steps` takes, in steps: a tile's sums need about six to leave
+static int64_t unit_time(int64_t steps) { return steps > 6 ? steps : 6; }
+
+// Units of the second task for the CTAs that have one unit more (less) of the first, whose units are the longer ones, so that
+// all are done at about the same time; returns that time in steps.
+static int64_t deal_units(int64_t u0, int64_t l0, int64_t u1, int64_t l1, int64_t ctas, int *less, int *more) {
+    const int64_t each = u0 / ctas, many = u0 % ctas;
+    for (int64_t t = ceil_div(u0 * l0 + u1 * l1, ctas);; t += 1 + l1 / 16) {
+        const int64_t left = t - (each + 1) * l0, right = t - each * l0;
+        const int64_t a = left > 0 ? left / l1 : 0, b = right > 0 ? right / l1 : 0;
+        if (many * a + (ctas - many) * b < u1) continue;
+        if (less) *less = (int)a;
+        if (more) *more = (int)b;
+        const int64_t longest = (each + (many > 0)) * l0;
+        return t > longest ? t : longest;
+    }
+}
+
+// Parts of the inner axes of dx (classes of a piece) and dw (rows), which run in one launch: short units leave the CTAs equally
+// busy, but every part is one more plane of fp32 sums through memory.  Costs are in
+// units of one 64-element step of one tile, about 0.4 us of a pair of SMs; a launch that adds planes up takes some 6 us.
 static double cut_products(int64_t tiles0, int64_t k0, double sums0, int64_t tiles1, int64_t k1, double sums1, int64_t ctas, int64_t *parts0, int64_t *parts1) {
     static const int64_t tries[] = {1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 12, 14, 16, 18, 20, 24, 28, 32, 37, 48, 64, 74, 96, 128, 148};
-    const double step_us = 0.4, plane_us = 8.0 / 5.0e6;          // an fp32 number written and read at 5 TB/s
+    const double step_us = 0.4, plane_us = 8.0 / 2.5e6;          // an fp32 number written and read at 2.5 TB/s
     double best = 1e300;
     for (int64_t a : tries) {
         if (a > 1 && (k0 / a < 8 || tiles0 * a > 6 * ctas)) break;
         for (int64_t b : tries) {
             if (b > 1 && (k1 / b < 8 || tiles1 * b > 6 * ctas)) break;
             const int64_t l0 = ceil_div(k0, a), l1 = ceil_div(k1, b), u0 = tiles0 * a, u1 = tiles1 * b;
-            // the longer units go out first; whoever has finished its share of them starts on the others
-            const bool first1 = l1 >= l0;
-            const int64_t ua = first1 ? u1 : u0, la = first1 ? l1 : l0, lb = first1 ? l0 : l1, both = u0 + u1;
-            const int64_t rounds = ceil_div(both, ctas), long_rounds = ceil_div(ua, ctas);
-            double cost = (double)(long_rounds * la + (rounds - long_rounds) * lb);
-            if (a > 1) cost += (3.0 + (double)a * sums0 * plane_us) / step_us;
-            if (b > 1) cost += (3.0 + (double)b * sums1 * plane_us) / step_us;
+            const int64_t t0 = unit_time(l0), t1 = unit_time(l1);
+            double cost = (double)(l1 >= l0 ? deal_units(u1, t1, u0, t0, ctas, nullptr, nullptr) : deal_units(u0, t0, u1, t1, ctas, nullptr, nullptr));
+            if (a > 1) cost += (6.0 + (double)a * sums0 * plane_us) / step_us;
+            if (b > 1) cost += (6.0 + (double)b * sums1 * plane_us) / step_us;
             if (cost < best) { best = cost; *parts0 = a; *parts1 = b; }
         }
     }
@@ -456,8 +474,8 @@ static Plan make_plan(const Problem &p, bool backward) {
     if (q.pack_w) q.w = place(at, (size_t)q.planes * w_rows * q.ldw * 2);
     const int cg = cta_group(n);
     if (!backward) {
-        const int64_t bn = columns_per_tile(V, cg);
-        cut_runs(n, ceil_div(n, (int64_t)(prod::BM * cg)), ceil_div(V, bn), ceil_div(d, (int64_t)prod::BK) * (q.planes == 3 ? 6 : 1), sm_count() / cg, &q.run, &q.parts);
+        const int64_t bn = columns_per_tile(V);
+        cut_runs(n, ceil_div(n, (int64_t)(prod::BM * cg)), ceil_div(V, bn), ceil_div(d, (int64_t)prod::BK) * (q.planes == 3 ? 6 : 1), sm_count() / cg, true, &q.run, &q.parts);
         q.stats = place(at, (size_t)q.parts * 2 * n * sizeof(float2));
         place_rows(at, n, &q);
     } else {
@@ -471,9 +489,7 @@ static Plan make_plan(const Problem &p, bool backward) {
         for (int64_t k = 8; k >= 4; --k) {
             const int64_t piece = ceil_div(top * k / 8, (int64_t)prod::BN) * prod::BN;
             const int64_t c = piece < V ? piece : V;
-            const int64_t rows1 = p.class_major ? c : d, cols1 = p.class_major ? d : c;
-            const int64_t tiles0 = ceil_div(n, (int64_t)(prod::BM * pg)) * ceil_div(d, (int64_t)columns_per_tile(d, pg));
-            const int64_t tiles1 = ceil_div(rows1, (int64_t)(prod::BM * pg)) * ceil_div(cols1, (int64_t)columns_per_tile(cols1, pg));
+            const int64_t tiles0 = tiles_of(n, d, pg), tiles1 = p.class_major ? tiles_of(c, d, pg) : tiles_of(d, c, pg);
             int64_t a, b;
             const double cost = (cut_products(tiles0, ceil_div(c, (int64_t)prod::BK), (double)n * d, tiles1, k1, (double)d * c, sm_count() / pg, &a, &b) +
                                  (c < V ? (double)n * d * 8.0 / 5.0e6 / 0.4 : 0.0)) * (double)ceil_div(V, c);
@@ -531,7 +547,7 @@ template <typename T> static int pack_operands(const Problem &p, const Plan &q, 
 static int set_task(prod::Task *t, CUtensorMap *ma, CUtensorMap *mb, int cg, int dtype, const View &a, int a_outer, const View &b, int b_outer, int64_t M,
                     int64_t N, int64_t K) {
     t->M = M; t->N = N;
-    t->bn = columns_per_tile(N, cg);
+    t->bn = columns_per_tile(N);
     t->m_tiles = (int)ceil_div(M, (int64_t)(prod::BM * cg));
     t->n_tiles = (int)ceil_div(N, (int64_t)t->bn);
     t->run = 1; t->runs = t->n_tiles; t->splits = 1;
@@ -543,20 +559,19 @@ static int set_task(prod::Task *t, CUtensorMap *ma, CUtensorMap *mb, int cg, int
 }
 
 // where a SUM task's results go: planes of fp32 sums, or the rounded output
-static int set_sums(prod::Task *t, CUtensorMap *mc, int64_t parts, float *sum, int64_t ld, bool add) {
+static int set_sums(prod::Task *t, CUtensorMap *mc, int planes, int64_t parts, float *sum, int64_t ld, bool add) {
     t->splits = (int)parts;
     t->add = add;
-    return prod::encode_map(mc, sum, GRWS_F32, t->N, t->M, ld, (int)parts, t->M * ld, 32, 32);
+    return prod::encode_map(mc, sum, GRWS_F32, t->N, t->M, ld, (int)parts, t->M * ld, planes == 3 ? 16 : 32, 32);
 }
 static int set_rounded(prod::Task *t, CUtensorMap *mc, int dtype, void *out, int64_t ldo) {
     t->rounded = 1;
-    t->out_dtype = dtype;
     if (!aligned16(out) || ldo * (int64_t)dtype_bytes(dtype) % 16 != 0) {         // no TMA store starts at such rows
         t->out = out;
         t->ldo = ldo;
         return GRWS_OK;
     }
-    return prod::encode_map(mc, out, dtype, t->N, t->M, ldo, 1, 0, dtype == GRWS_F32 ? 32 : 64, 32);
+    return prod::encode_map(mc, out, dtype, t->N, t->M, ldo, 1, 0, dtype == GRWS_F32 ? 16 : 64, 32);
 }
 
 static int status_word(int **word) {
@@ -625,7 +640,11 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
         prod::Maps maps;
         const int cg = cta_group(p.n);
         if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, o.dtype, o.x, 0, o.w, !p.class_major, p.n, cols, p.d)) return rc;
-        if (int rc = prod::encode_map(&maps.c[0], G.p, o.dtype, cols, p.n, q.ldg, q.planes, G.plane, q.planes == 3 ? 32 : 64, 32)) return rc;
+        if (int rc = prod::encode_map(&maps.c[0], G.p, o.dtype, cols, p.n, q.ldg, q.planes, G.plane, q.planes == 3 ? 16 : 64, 32)) return rc;
+        int64_t run, runs;
+        cut_runs(p.n, r.task[0].m_tiles, r.task[0].n_tiles, r.task[0].k_blocks * (q.planes == 3 ? 6 : 1), sm_count() / cg, false, &run, &runs);
+        r.task[0].run = (int)run;
+        r.task[0].runs = (int)runs;
         r.task[0].b_row0 = (int)v0;
         r.v0 = v0;
         r.scale = stored_scale(p);
@@ -650,16 +669,22 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
                                    : set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, o.x, 1, G, 1, M, N, p.n);
                 if (rc != GRWS_OK) return rc;
                 t->k_len = (int)q.dw_len;
-                rc = sum_dw ? set_sums(t, &maps.c[i], q.dw_parts, dw_sum, q.ld_dw, false) : set_rounded(t, &maps.c[i], p.dtype, dw_out, ldo);
+                rc = sum_dw ? set_sums(t, &maps.c[i], q.planes, q.dw_parts, dw_sum, q.ld_dw, false) : set_rounded(t, &maps.c[i], p.dtype, dw_out, ldo);
             } else {
                 rc = set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, G, 0, o.w, p.class_major, p.n, p.d, cols);
                 if (rc != GRWS_OK) return rc;
                 t->b_k0 = (int)v0;
                 t->k_len = (int)q.dx_len;
-                rc = sum_dx ? set_sums(t, &maps.c[i], ceil_div((int64_t)t->k_blocks, q.dx_len), dx_sum, q.ld_dx, v0 > 0)      // (a last, shorter piece: fewer)
+                rc = sum_dx ? set_sums(t, &maps.c[i], q.planes, ceil_div((int64_t)t->k_blocks, q.dx_len), dx_sum, q.ld_dx, v0 > 0)      // (a last, shorter piece: fewer)
                             : set_rounded(t, &maps.c[i], p.dtype, dx, p.d);
             }
             if (rc != GRWS_OK) return rc;
+        }
+        const int64_t ctas = sm_count() / pg, units = r.task[0].units() + (r.tasks > 1 ? r.task[1].units() : 0);
+        // few units per CTA: dealt out by length (many: in order, so that those at work at a time share operands in L2)
+        if (r.tasks > 1 && units <= 12 * ctas) {
+            r.deal = 1;
+            deal_units(r.task[0].units(), unit_time(r.task[0].k_len), r.task[1].units(), unit_time(r.task[1].k_len), units < ctas ? units : ctas, &r.deal_less, &r.deal_more);
         }
         if (int rc = launch_product<prod::SUM>(pg, q.planes, maps, r, st)) return rc;
         if (dw && sum_dw) if (int rc = launch_round<T>(p, dw_sum, q.dw_parts, M, N, q.ld_dw, r.scale, dw_out, ldo, 1, st)) return rc;
