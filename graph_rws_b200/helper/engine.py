@@ -14,6 +14,8 @@ import torch
 import torch.distributed as dist
 import torch.nn.functional as F
 
+from ..layers.losses import distillation_loss
+
 
 class _FlatGrads:
     """All gradients of a model as views into one flat buffer, so that the data-parallel all-reduce
@@ -81,12 +83,52 @@ def _allreduce_grads(model, group=None, average=True):
         off += g.numel()
 
 
-def train_step_full(model, graph, features, labels, train_idx, optimizer):
-    """One full-graph epoch (= one step); returns the loss tensor (no host sync)."""
+class Distillation:
+    """What a step learns from a teacher: its ``kept`` best scores of every node and their classes, at which
+    temperature, and how much of the loss they are (the rest is the labels')."""
+
+    def __init__(self, scores, ids, temperature: float = 2.0, weight: float = 0.5):
+        if scores.shape != ids.shape or scores.dim() != 2:
+            raise RuntimeError(f"scores {tuple(scores.shape)} and ids {tuple(ids.shape)} must both be [nodes, kept]")
+        if not 0.0 <= weight <= 1.0:
+            raise ValueError(f"weight must lie between 0 and 1, got {weight}")
+        self.scores, self.ids, self.temperature, self.weight = scores, ids, float(temperature), float(weight)
+
+    @classmethod
+    def from_logits(cls, logits, kept: int, temperature: float = 2.0, weight: float = 0.5):
+        """From a teacher's scores of all nodes (``GCN_BCSR.inference``), of which only the best are kept."""
+        scores, ids = logits.detach().topk(min(int(kept), logits.shape[1]), dim=1)
+        return cls(scores, ids.int(), temperature, weight)
+
+
+def _loss(model, graphs, x, rows, nodes, labels, fused_loss, distill):
+    """Mean loss of a step over the rows ``rows`` of the model's output, which are the nodes ``nodes``."""
+    if fused_loss:
+        if distill is not None:
+            raise ValueError("distillation compares class scores: it needs fused_loss=False")
+        return model.loss(graphs, x, labels[nodes], rows=rows)
+    logits = model(graphs, x)[rows]
+    loss = F.cross_entropy(logits.float(), labels[nodes])
+    if distill is None:
+        return loss
+    soft = distillation_loss(logits, distill.scores[nodes], distill.ids[nodes], temperature=distill.temperature)
+    return (1.0 - distill.weight) * loss + distill.weight * soft
+
+
+def _loss_sum(model, graph, features, train_idx, labels, fused_loss):
+    if fused_loss:
+        return model.loss(graph, features, labels[train_idx], rows=train_idx, reduction='sum')
+    return F.cross_entropy(model(graph, features)[train_idx].float(), labels[train_idx], reduction='sum')
+
+
+def train_step_full(model, graph, features, labels, train_idx, optimizer, fused_loss=False, distill=None):
+    """One full-graph epoch (= one step); returns the loss tensor (no host sync).
+
+    ``fused_loss``: the loss without the matrix of class scores (``GCN_BCSR.loss``), for many classes;
+    ``distill``: a ``Distillation`` to learn from as well."""
     model.train()
     _zero_grads(model, optimizer)
-    logits = model(graph, features)
-    loss = F.cross_entropy(logits[train_idx].float(), labels[train_idx])
+    loss = _loss(model, graph, features, train_idx, train_idx, labels, fused_loss, distill)
     loss.backward()
     _allreduce_grads(model)
     torch.nn.utils.clip_grad_norm_(model.parameters(), max_norm=1.0)
@@ -94,14 +136,14 @@ def train_step_full(model, graph, features, labels, train_idx, optimizer):
     return loss.detach()
 
 
-def train_step_full_sharded(model, graph, features_local, labels_local, train_idx_local, num_train, optimizer):
+def train_step_full_sharded(model, graph, features_local, labels_local, train_idx_local, num_train, optimizer, fused_loss=False):
     """One full-graph epoch with the rows of the graph, features and labels sharded over the ranks
     (``graph`` is a parallel.RowShardedGraph).  The loss is the global mean over ``num_train``
-    training rows: every rank sums its own rows' terms, so the weight gradients ADD across ranks."""
+    training rows: every rank sums its own rows' terms, so the weight gradients ADD across ranks.
+    ``fused_loss`` as in ``train_step_full``."""
     model.train()
     _zero_grads(model, optimizer)
-    logits = model(graph, features_local)
-    loss = F.cross_entropy(logits[train_idx_local].float(), labels_local[train_idx_local], reduction='sum') / num_train
+    loss = _loss_sum(model, graph, features_local, train_idx_local, labels_local, fused_loss) / num_train
     loss.backward()
     _allreduce_grads(model, average=False)
     torch.nn.utils.clip_grad_norm_(model.parameters(), max_norm=1.0)
@@ -139,16 +181,16 @@ def layer0_inputs(blocks, features, fetch_rows=None):
     return [g0] + list(blocks[1:]), features
 
 
-def train_step_sampled(model, sampler, graph, features, labels, seeds, optimizer, fetch_rows=None):
+def train_step_sampled(model, sampler, graph, features, labels, seeds, optimizer, fetch_rows=None, fused_loss=False, distill=None):
     """One mini-batch step: sample the blocks for ``seeds``, gather the input rows, train.
 
     ``fetch_rows(node_ids)`` supplies feature rows when they are sharded across ranks
-    (parallel.exchange_rows); by default they are indexed from the local ``features``."""
+    (parallel.exchange_rows); by default they are indexed from the local ``features``.
+    ``fused_loss`` and ``distill`` as in ``train_step_full``."""
     model.train()
     blocks, x = layer0_inputs(sampler.sample_layers(graph, seeds), features, fetch_rows)
     _zero_grads(model, optimizer)
-    logits = model(blocks, x)[:seeds.numel()]
-    loss = F.cross_entropy(logits.float(), labels[seeds.long()])
+    loss = _loss(model, blocks, x, slice(0, seeds.numel()), seeds.long(), labels, fused_loss, distill)
     loss.backward()
     _allreduce_grads(model)
     torch.nn.utils.clip_grad_norm_(model.parameters(), max_norm=1.0)
@@ -203,7 +245,7 @@ def _block_tensors(blocks):
 
 
 def graphed_sampled_step(model, sampler, graph, features, labels, optimizer, num_seeds, fetch_rows=None, warmup=3,
-                         pipelined=False):
+                         pipelined=False, fused_loss=False, distill=None):
     """``step(seeds, step_index) -> loss`` for sampled training, as one CUDA graph per step.
 
     ``pipelined=True`` overlaps the sampler with the training: the graph of a step has two branches,
@@ -213,7 +255,7 @@ def graphed_sampled_step(model, sampler, graph, features, labels, optimizer, num
     GPU runs the sampler's small kernels in the gaps of the training's).  ``step`` then returns the
     loss of the batch given to the PREVIOUS call; ``step.prime(seeds, step_index)`` samples the
     first batch.  Results per batch are the same as without pipelining: sampling depends on the
-    seeds and the step index only."""
+    seeds and the step index only.  ``fused_loss`` and ``distill`` as in ``train_step_full``."""
     device = labels.device
     seeds_buf = torch.zeros(num_seeds, dtype=torch.int32, device=device)
     seed_dev = torch.zeros(1, dtype=torch.int64, device=device)          # the Philox seed, read by the sampling kernels
@@ -222,8 +264,7 @@ def graphed_sampled_step(model, sampler, graph, features, labels, optimizer, num
     def train_on(blocks, seeds):
         blocks, x = layer0_inputs(blocks, features, fetch_rows)
         _zero_grads(model, optimizer)
-        logits = model(blocks, x)[:num_seeds]
-        loss = F.cross_entropy(logits.float(), labels[seeds.long()])
+        loss = _loss(model, blocks, x, slice(0, num_seeds), seeds.long(), labels, fused_loss, distill)
         loss.backward()
         _allreduce_grads(model)
         torch.nn.utils.clip_grad_norm_(model.parameters(), max_norm=1.0)
@@ -286,19 +327,22 @@ def graphed_sampled_step(model, sampler, graph, features, labels, optimizer, num
     return step
 
 
-def graphed_full_step(model, graph, features, labels, train_idx, optimizer, num_train=None, warmup=3):
+def graphed_full_step(model, graph, features, labels, train_idx, optimizer, num_train=None, warmup=3, fused_loss=False,
+                      distill=None):
     """``step() -> loss`` for full-graph training (one GPU, or a row shard with ``num_train`` = the
-    global number of training rows) as one CUDA graph per epoch."""
+    global number of training rows) as one CUDA graph per epoch.  ``fused_loss`` and (one GPU) ``distill``
+    as in ``train_step_full``."""
     device = labels.device
     sharded = num_train is not None
+    if sharded and distill is not None:
+        raise ValueError("distillation of row shards is not built")
 
     def body():
         _zero_grads(model, optimizer)
-        logits = model(graph, features)
         if sharded:
-            loss = F.cross_entropy(logits[train_idx].float(), labels[train_idx], reduction='sum') / num_train
+            loss = _loss_sum(model, graph, features, train_idx, labels, fused_loss) / num_train
         else:
-            loss = F.cross_entropy(logits[train_idx].float(), labels[train_idx])
+            loss = _loss(model, graph, features, train_idx, train_idx, labels, fused_loss, distill)
         loss.backward()
         _allreduce_grads(model, average=not sharded)
         torch.nn.utils.clip_grad_norm_(model.parameters(), max_norm=1.0)
@@ -326,13 +370,15 @@ def _record_stream(obj, stream):
 
 
 def train_epoch_node_sampling(model, graph, features, labels, train_idx, optimizer, sampler,
-                              batch_size: int = 1024, pipeline: bool = True, fetch_rows=None, max_batches=None):
+                              batch_size: int = 1024, pipeline: bool = True, fetch_rows=None, max_batches=None,
+                              fused_loss=False, distill=None):
     """One epoch of mini-batch training over ``train_idx`` (helper/engine.py:86-256).
 
     With ``pipeline`` a producer thread samples the blocks of batch i+1 and gathers its input rows
     on a side stream while the main thread trains on batch i (the reference's producer / consumer
     pair with a queue of one, helper/engine.py:118-153); the hand-over is a CUDA event, so neither
-    thread synchronises the device.  Returns (mean loss tensor, number of seeds trained on)."""
+    thread synchronises the device.  Returns (mean loss tensor, number of seeds trained on).
+    ``fused_loss`` and ``distill`` as in ``train_step_full``."""
     device = labels.device
     n = train_idx.numel()
     starts = list(range(0, n, batch_size))
@@ -358,8 +404,7 @@ def train_epoch_node_sampling(model, graph, features, labels, train_idx, optimiz
 
     def train_on(seeds, blocks, x):
         _zero_grads(model, optimizer)
-        logits = model(blocks, x)[:seeds.numel()]
-        loss = F.cross_entropy(logits.float(), labels[seeds.long()])
+        loss = _loss(model, blocks, x, slice(0, seeds.numel()), seeds.long(), labels, fused_loss, distill)
         loss.backward()
         _allreduce_grads(model)
         torch.nn.utils.clip_grad_norm_(model.parameters(), max_norm=1.0)

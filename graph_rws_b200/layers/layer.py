@@ -90,6 +90,22 @@ class BCSRAggregateFirstFunction(Function):
         return None, None, grad_weight, None
 
 
+class BCSRAggregateFunction(Function):
+    """``A @ X`` alone; backward is the same product on the graph's cached transposed BCSR."""
+
+    @staticmethod
+    def forward(ctx, graph, features):
+        ctx.graph, ctx.rows = graph, features.shape[0]
+        record_spmm_time(0.0)
+        return _spmm_graph(graph, features)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        grad_output = grad_output.contiguous()
+        g_t = ctx.graph.transposed(ctx.rows, dtype=grad_output.dtype)
+        return None, _spmm_graph(g_t, grad_output)[:ctx.rows]
+
+
 class BCSRGraphConv(nn.Module):
     """Aggregation only; activation, normalisation and dropout live in the model."""
 
@@ -141,3 +157,17 @@ class BCSRGraphConv(nn.Module):
             h_neigh = F.pad(h_neigh, (0, 0, 0, h_self.shape[0] - h_neigh.shape[0]))
         out = h_neigh + h_self
         return out[:, :self.out_feats] if pad else out
+
+    def classifier(self, graph, features: torch.Tensor, features_target: torch.Tensor = None, rows=None):
+        """``(x, weight)`` such that ``x @ weight`` are the rows ``rows`` (an index or a slice; all by default) of
+        ``forward(graph, features, features_target)``: ``A (X W_neigh) + X_target W_self = [A X, X_target] [W_neigh; W_self]``.
+        The product with the graph runs at the input width, whatever the number of classes, and a loss
+        that takes ``x`` and ``weight`` apart (``linear_cross_entropy``) needs no row of class scores."""
+        h_neigh = BCSRAggregateFunction.apply(graph, features)
+        h_self = features_target if features_target is not None else features[:h_neigh.shape[0]]
+        n = h_neigh.shape[0] if features_target is None else h_self.shape[0]
+        h_neigh, h_self = (h[:n] if h.shape[0] >= n else F.pad(h, (0, 0, 0, n - h.shape[0])) for h in (h_neigh, h_self))
+        if rows is not None:
+            h_neigh, h_self = h_neigh[rows], h_self[rows]
+        x = torch.cat((h_neigh, h_self), dim=1)
+        return x, torch.cat((self.weight_neigh, self.weight_self), dim=0).to(x.dtype)

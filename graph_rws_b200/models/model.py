@@ -27,6 +27,7 @@ from torch.utils.checkpoint import checkpoint
 from .. import core
 from ..data import BCSRGraph
 from ..layers import BCSRGraphConv
+from ..layers.losses import linear_cross_entropy
 from ..layers.norm import act_layer_norm
 
 _ACTIVATIONS = {'relu': F.relu, 'elu': F.elu, 'gelu': F.gelu}
@@ -134,40 +135,65 @@ class GCN_BCSR(nn.Module):
             return F.pad(h_in, (0, 0, 0, target_rows - h_in.shape[0]))
         return h_in[:target_rows]          # target nodes come first
 
+    def _layer_inputs(self, l, graph_list, h):
+        """(graph, previous graph, rows of the self path) of layer ``l``."""
+        g, prev_g = graph_list[l], graph_list[l - 1] if l > 0 else None
+        self._sanitize_and_reindex(l, g, prev_g, h.shape)     # edits the graph: outside checkpoint
+        return g, prev_g, self._get_residual(l, g, prev_g, h, g.num_rows)
+
+    def _run_layer(self, l, graph_list, h):
+        g, prev_g, h_target = self._layer_inputs(l, graph_list, h)
+
+        def run_curr_layer(h_curr, layer=self.layers[l], g=g, h_tgt=h_target):
+            return layer(g, h_curr, features_target=h_tgt)
+
+        if self.use_checkpoint and self.training and h.requires_grad:
+            h_out = checkpoint(run_curr_layer, h, use_reentrant=False)
+        else:
+            h_out = run_curr_layer(h)
+
+        if self.residual and l < len(self.layers) - 1:
+            h_res = h
+            if self.residual_projs is not None and self.residual_projs[l] is not None:
+                h_res = self.residual_projs[l](h_res)
+            h_out = h_out + self._get_residual(l, g, prev_g, h_res, h_out.shape[0])
+        h = h_out
+        if l < len(self.layers) - 1:
+            if self.norms:
+                # activation and normalisation in one pass over the rows when the activation is ReLU
+                relu = self.activation is F.relu
+                h = act_layer_norm(h if relu else self.activation(h), self.norms[l], relu)
+            else:
+                h = self.activation(h)
+            if self.dropout_layer is not None:
+                h = self.dropout_layer(h)
+        return h
+
     def forward(self, graphs: Union[BCSRGraph, List[BCSRGraph]], features: torch.Tensor) -> torch.Tensor:
         if features.device.type != 'cuda':
             features = features.to('cuda', non_blocking=True)
         graph_list = self._ensure_graph_list(graphs)
         h = features
-        for l, (layer, g) in enumerate(zip(self.layers, graph_list)):
-            prev_g = graph_list[l - 1] if l > 0 else None
-            self._sanitize_and_reindex(l, g, prev_g, h.shape)     # edits the graph: outside checkpoint
-            h_target = self._get_residual(l, g, prev_g, h, g.num_rows)
-
-            def run_curr_layer(h_curr, layer=layer, g=g, h_tgt=h_target):
-                return layer(g, h_curr, features_target=h_tgt)
-
-            if self.use_checkpoint and self.training and h.requires_grad:
-                h_out = checkpoint(run_curr_layer, h, use_reentrant=False)
-            else:
-                h_out = run_curr_layer(h)
-
-            if self.residual and l < len(self.layers) - 1:
-                h_res = h
-                if self.residual_projs is not None and self.residual_projs[l] is not None:
-                    h_res = self.residual_projs[l](h_res)
-                h_out = h_out + self._get_residual(l, g, prev_g, h_res, h_out.shape[0])
-            h = h_out
-            if l < len(self.layers) - 1:
-                if self.norms:
-                    # activation and normalisation in one pass over the rows when the activation is ReLU
-                    relu = self.activation is F.relu
-                    h = act_layer_norm(h if relu else self.activation(h), self.norms[l], relu)
-                else:
-                    h = self.activation(h)
-                if self.dropout_layer is not None:
-                    h = self.dropout_layer(h)
+        for l in range(len(self.layers)):
+            h = self._run_layer(l, graph_list, h)
         return h
+
+    def loss(self, graphs: Union[BCSRGraph, List[BCSRGraph]], features: torch.Tensor, labels: torch.Tensor, rows=None,
+             ignore_index: int = -100, reduction: str = 'mean') -> torch.Tensor:
+        """Cross entropy of the scores that ``forward`` returns, of the rows ``rows`` (an index or a slice; all by
+        default) against their ``labels``, without computing the scores as a matrix: the last layer aggregates its
+        input at the hidden width, and ``linear_cross_entropy`` goes over the classes piece by piece.  For
+        many classes: forward multiplies the graph at class width and keeps rows x classes for backward."""
+        if features.device.type != 'cuda':
+            features = features.to('cuda', non_blocking=True)
+        graph_list = self._ensure_graph_list(graphs)
+        h = features
+        last = len(self.layers) - 1
+        for l in range(last):
+            h = self._run_layer(l, graph_list, h)
+        g, _, h_target = self._layer_inputs(last, graph_list, h)
+        x, weight = self.layers[last].classifier(g, h, features_target=h_target, rows=rows)
+        return linear_cross_entropy(x, weight, labels, ignore_index=ignore_index, reduction=reduction)
 
     def inference(self, graph: BCSRGraph, features: torch.Tensor, batch_size: int = 0) -> torch.Tensor:
         if features.device.type != 'cuda':
