@@ -109,14 +109,13 @@ __global__ void __launch_bounds__(256) rows_kernel(const Problem p, const float2
 }
 
 // ---------------------------------------------------------------------------------------------
-// fp32 arithmetic on the general cores: any stride, any size.  64 x 64 tiles, 16 deep, 4 x 4 a thread.
+// Small fp32 calls, in fp32 arithmetic on the general cores: 64 x 64 tiles, 16 deep, 4 x 4 a thread.
 // ---------------------------------------------------------------------------------------------
 constexpr int TM = 64, TN = 64, TK = 16, PAD = 4;
 
 struct Tiles { float a[TK][TM + PAD], b[TK][TN + PAD]; };
 
-template <typename TA, typename TB>
-__device__ __forceinline__ void tile_product(const TA *A, int64_t am, int64_t ak, const TB *B, int64_t bk, int64_t bn, int64_t M, int64_t N,
+__device__ __forceinline__ void tile_product(const float *A, int64_t am, int64_t ak, const float *B, int64_t bk, int64_t bn, int64_t M, int64_t N,
                                              int64_t m0, int64_t n0, int64_t k0, int64_t k1, Tiles &t, float (&acc)[4][4]) {
     const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
 #pragma unroll
@@ -131,8 +130,8 @@ __device__ __forceinline__ void tile_product(const TA *A, int64_t am, int64_t ak
             const int am_i = ak == 1 ? e >> 4 : e & 63, ak_i = ak == 1 ? e & 15 : e >> 6;
             const int bn_i = bk == 1 ? e >> 4 : e & 63, bk_i = bk == 1 ? e & 15 : e >> 6;
             const int64_t ma = m0 + am_i, ka = k + ak_i, nb = n0 + bn_i, kb = k + bk_i;
-            t.a[ak_i][am_i] = ma < M && ka < k1 ? to_float(A[ma * am + ka * ak]) : 0.0f;
-            t.b[bk_i][bn_i] = nb < N && kb < k1 ? to_float(B[kb * bk + nb * bn]) : 0.0f;
+            t.a[ak_i][am_i] = ma < M && ka < k1 ? A[ma * am + ka * ak] : 0.0f;
+            t.b[bk_i][bn_i] = nb < N && kb < k1 ? B[kb * bk + nb * bn] : 0.0f;
         }
         __syncthreads();
 #pragma unroll
@@ -149,7 +148,7 @@ __device__ __forceinline__ void tile_product(const TA *A, int64_t am, int64_t ak
 }
 
 // statistics of 64 rows over the class tiles blockIdx.y, + gridDim.y, ...
-template <typename T> __global__ void __launch_bounds__(256) plain_stats_kernel(const Problem p, float2 *__restrict__ part, float *__restrict__ label_score,
+__global__ void __launch_bounds__(256) plain_stats_kernel(const Problem p, float2 *__restrict__ part, float *__restrict__ label_score,
                                                                                int *__restrict__ done) {
     __shared__ __align__(16) Tiles t;
     wait_for_previous();
@@ -168,7 +167,7 @@ template <typename T> __global__ void __launch_bounds__(256) plain_stats_kernel(
     const int64_t tiles = (p.V + TN - 1) / TN;
     for (int64_t tile = blockIdx.y; tile < tiles; tile += gridDim.y) {
         const int64_t n0 = tile * TN;
-        tile_product(static_cast<const T *>(p.x), p.ldx, (int64_t)1, static_cast<const T *>(p.w), p.w_k(), p.w_v(), p.n, p.V, m0, n0, 0, p.d, t, acc);
+        tile_product(static_cast<const float *>(p.x), p.ldx, 1, static_cast<const float *>(p.w), p.w_k(), p.w_v(), p.n, p.V, m0, n0, 0, p.d, t, acc);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -190,14 +189,14 @@ template <typename T> __global__ void __launch_bounds__(256) plain_stats_kernel(
 }
 
 // G of the classes [v0, v0 + cols), fp32, rows of ldg
-template <typename T> __global__ void __launch_bounds__(256) plain_grad_kernel(const Problem p, int64_t v0, int64_t cols, float *__restrict__ G, int64_t ldg) {
+__global__ void __launch_bounds__(256) plain_grad_kernel(const Problem p, int64_t v0, int64_t cols, float *__restrict__ G, int64_t ldg) {
     __shared__ __align__(16) Tiles t;
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
     const int64_t m0 = (int64_t)blockIdx.x * TM, n0 = (int64_t)blockIdx.y * TN;
     float acc[4][4];
     wait_for_previous();
     let_next_start();
-    tile_product(static_cast<const T *>(p.x), p.ldx, (int64_t)1, static_cast<const T *>(p.w) + v0 * p.w_v(), p.w_k(), p.w_v(), p.n, cols, m0, n0, 0, p.d, t, acc);
+    tile_product(static_cast<const float *>(p.x), p.ldx, 1, static_cast<const float *>(p.w) + v0 * p.w_v(), p.w_k(), p.w_v(), p.n, cols, m0, n0, 0, p.d, t, acc);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t row = m0 + ty * 4 + i;
@@ -219,17 +218,16 @@ template <typename T> __global__ void __launch_bounds__(256) plain_grad_kernel(c
 // A product A [M, K] B [K, N] in parts of K: element strides, tiles, and its plane of fp32 partial sums [parts][M][N], or (one
 // part) the output itself at m * om + n * on
 struct PlainTask {
-    const void *a, *b;
+    const float *a, *b;
     int64_t am, ak, bk, bn, M, N, K, k_part;
     int m_tiles, n_tiles, parts, add;
-    float *sum;
-    void *out;
+    float *sum, *out;
     int64_t om, on;
     __host__ __device__ int blocks() const { return m_tiles * n_tiles * parts; }
 };
 
 // dx = G w^T (task 0) and dw = x^T G (task 1) of one piece
-template <typename T> __global__ void __launch_bounds__(256) plain_products_kernel(const Problem p, const PlainTask dx, const PlainTask dw) {
+__global__ void __launch_bounds__(256) plain_products_kernel(const Problem p, const PlainTask dx, const PlainTask dw) {
     __shared__ __align__(16) Tiles t;
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
     wait_for_previous();
@@ -241,8 +239,7 @@ template <typename T> __global__ void __launch_bounds__(256) plain_products_kern
     const int part = i / (q.m_tiles * q.n_tiles), tile = i - part * (q.m_tiles * q.n_tiles);
     const int64_t m0 = (int64_t)(tile % q.m_tiles) * TM, n0 = (int64_t)(tile / q.m_tiles) * TN, k0 = part * q.k_part, k1 = min(q.K, k0 + q.k_part);
     float acc[4][4];
-    if (second) tile_product(static_cast<const T *>(q.a), q.am, q.ak, static_cast<const float *>(q.b), q.bk, q.bn, q.M, q.N, m0, n0, k0, k1, t, acc);
-    else tile_product(static_cast<const float *>(q.a), q.am, q.ak, static_cast<const T *>(q.b), q.bk, q.bn, q.M, q.N, m0, n0, k0, k1, t, acc);
+    tile_product(q.a, q.am, q.ak, q.b, q.bk, q.bn, q.M, q.N, m0, n0, k0, k1, t, acc);
     const float alpha = q.out ? prod::grad_alpha(p) : 1.0f;
 #pragma unroll
     for (int a = 0; a < 4; ++a)
@@ -251,7 +248,7 @@ template <typename T> __global__ void __launch_bounds__(256) plain_products_kern
             const int64_t m = m0 + ty * 4 + a, n = n0 + tx * 4 + b;
             if (m >= q.M || n >= q.N) continue;
             if (q.out) {
-                static_cast<T *>(q.out)[m * q.om + n * q.on] = from_float<T>(acc[a][b] * alpha);
+                q.out[m * q.om + n * q.on] = acc[a][b] * alpha;
             } else {
                 float *o = q.sum + ((int64_t)part * q.M + m) * q.N + n;
                 *o = q.add ? *o + acc[a][b] : acc[a][b];
@@ -336,7 +333,6 @@ static __device__ int g_status;
 // plan: how a call is cut up, and where its workspace lies
 // ---------------------------------------------------------------------------------------------
 constexpr size_t PIECE_BYTES = 512ull << 20;       // workspace for G
-constexpr double TENSOR_PRODUCTS = 1 << 22;        // n d V from which the tensor cores take the call
 
 struct Plan {
     bool tensor;
@@ -437,10 +433,18 @@ static double cut_products(int64_t tiles0, int64_t k0, double sums0, int64_t til
     return best;
 }
 
+// 16-bit operands always go to the tensor cores (140 x 32 x 7: 20.7 us against 24.7 on the general cores, 300 x 256 x 40: 23
+// against 66).  fp32 costs them six products of packed planes: 35 against 25 us and 48 against 68; narrow rows, where a tile's
+// sums are over after a step or two, stay on the general cores for longer (170,000 x 16 x 7: 310 against 189).
+static bool on_tensor_cores(int64_t n, int64_t d, int64_t V, int dtype) {
+    const double products = (double)n * (double)d * (double)V;
+    return dtype != GRWS_F32 || products >= (double)(1 << 26) || (d >= 192 && products >= (double)(1 << 21));
+}
+
 static Plan make_plan(const Problem &p, bool backward) {
     Plan q = {};
     const int64_t n = p.n, d = p.d, V = p.V;
-    q.tensor = (double)n * (double)d * (double)V >= TENSOR_PRODUCTS;
+    q.tensor = on_tensor_cores(n, d, V, p.dtype);
     size_t at = 0;
     if (!q.tensor) {
         const int64_t row_tiles = ceil_div(n, (int64_t)TM), class_tiles = ceil_div(V, (int64_t)TN), width_tiles = ceil_div(d, (int64_t)TN);
@@ -696,45 +700,45 @@ template <typename T> static int forward(const Problem &p, const Plan &q, float 
     float2 *part = reinterpret_cast<float2 *>(scratch + q.stats), *partial = reinterpret_cast<float2 *>(scratch + q.partial);
     float *label_score = reinterpret_cast<float *>(scratch + q.label_score);
     int *done = reinterpret_cast<int *>(scratch + q.done);
-    if (q.tensor) {
-        if (int rc = tensor_forward<T>(p, q, part, label_score, done, scratch, st)) return rc;
-    } else {
-        if (int rc = launch_next(plain_stats_kernel<T>, dim3((unsigned)ceil_div(p.n, (int64_t)TM), (unsigned)q.parts), 256, 0, st, 1, p, part, label_score, done))
-            return rc;
-    }
+    if (int rc = q.tensor ? tensor_forward<T>(p, q, part, label_score, done, scratch, st)
+                          : launch_next(plain_stats_kernel, dim3((unsigned)ceil_div(p.n, (int64_t)TM), (unsigned)q.parts), 256, 0, st, 1, p, part, label_score, done))
+        return rc;
     return launch_next(rows_kernel, dim3((unsigned)ceil_div(p.n, (int64_t)ROWS_PER_BLOCK)), 256, 0, st, 1, p, part, (int)(q.tensor ? 2 * q.parts : q.parts),
                        label_score, state, loss, count, partial, done);
 }
 
-template <typename T> static int backward(Problem p, const Plan &q, void *dx, void *dw, char *scratch, cudaStream_t st) {
-    float *G = reinterpret_cast<float *>(scratch + q.G), *dx_sum = reinterpret_cast<float *>(scratch + q.dx_sum);
-    float *dw_sum = reinterpret_cast<float *>(scratch + q.dw_sum), *norm = reinterpret_cast<float *>(scratch + q.norm);
-    if (p.reduction == RED_NONE) {
-        if (int rc = launch_next(grad_norm_kernel, dim3(1), 1024, 0, st, 1, p.grad, p.n, norm)) return rc;
-        p.norm = norm;
-    }
-    if (q.tensor) return tensor_backward<T>(p, q, dx, dw, scratch, st);
+static int plain_backward(const Problem &p, const Plan &q, float *dx, float *dw, char *scratch, cudaStream_t st) {
+    float *G = reinterpret_cast<float *>(scratch + q.G), *dx_sum = reinterpret_cast<float *>(scratch + q.dx_sum), *dw_sum = reinterpret_cast<float *>(scratch + q.dw_sum);
     const unsigned row_tiles = (unsigned)ceil_div(p.n, (int64_t)TM);
-    const T *x = static_cast<const T *>(p.x), *w = static_cast<const T *>(p.w);
+    const float *x = static_cast<const float *>(p.x), *w = static_cast<const float *>(p.w);
     const bool sum_dx = q.dx_parts > 1 || q.piece < p.V, sum_dw = q.dw_parts > 1;
     const int64_t ok = p.class_major ? 1 : p.V, ov = p.class_major ? p.d : 1;
     for (int64_t v0 = 0; v0 < p.V; v0 += q.piece) {
         const int64_t cols = p.V - v0 < q.piece ? p.V - v0 : q.piece;
-        if (int rc = launch_next(plain_grad_kernel<T>, dim3(row_tiles, (unsigned)ceil_div(cols, (int64_t)TN)), 256, 0, st, 1, p, v0, cols, G, q.piece)) return rc;
+        if (int rc = launch_next(plain_grad_kernel, dim3(row_tiles, (unsigned)ceil_div(cols, (int64_t)TN)), 256, 0, st, 1, p, v0, cols, G, q.piece)) return rc;
         PlainTask tx = {}, tw = {};
         if (dx) {
             tx = PlainTask{G, w + v0 * p.w_v(), q.piece, 1, p.w_v(), p.w_k(), p.n, p.d, cols, q.dx_len, (int)row_tiles, (int)ceil_div(p.d, (int64_t)TN),
                            (int)ceil_div(cols, q.dx_len), v0 > 0, dx_sum, sum_dx ? nullptr : dx, p.d, 1};
         }
-        T *dw_out = static_cast<T *>(dw) + v0 * ov;
+        float *dw_out = dw + v0 * ov;
         if (dw) {
             tw = PlainTask{x, G, 1, p.ldx, q.piece, 1, p.d, cols, p.n, q.dw_len, (int)ceil_div(p.d, (int64_t)TM), (int)ceil_div(cols, (int64_t)TN),
                            (int)q.dw_parts, 0, dw_sum, sum_dw ? nullptr : dw_out, ok, ov};
         }
-        if (int rc = launch_next(plain_products_kernel<T>, dim3((unsigned)(tx.blocks() + tw.blocks())), 256, 0, st, 1, p, tx, tw)) return rc;
-        if (dw && sum_dw) if (int rc = launch_round<T>(p, dw_sum, q.dw_parts, p.d, cols, cols, 1.0f, dw_out, ok, ov, st)) return rc;
+        if (int rc = launch_next(plain_products_kernel, dim3((unsigned)(tx.blocks() + tw.blocks())), 256, 0, st, 1, p, tx, tw)) return rc;
+        if (dw && sum_dw) if (int rc = launch_round<float>(p, dw_sum, q.dw_parts, p.d, cols, cols, 1.0f, dw_out, ok, ov, st)) return rc;
     }
-    return dx && sum_dx ? launch_round<T>(p, dx_sum, q.dx_parts, p.n, p.d, p.d, 1.0f, dx, p.d, 1, st) : GRWS_OK;
+    return dx && sum_dx ? launch_round<float>(p, dx_sum, q.dx_parts, p.n, p.d, p.d, 1.0f, dx, p.d, 1, st) : GRWS_OK;
+}
+
+template <typename T> static int backward(Problem p, const Plan &q, void *dx, void *dw, char *scratch, cudaStream_t st) {
+    if (p.reduction == RED_NONE) {
+        float *norm = reinterpret_cast<float *>(scratch + q.norm);
+        if (int rc = launch_next(grad_norm_kernel, dim3(1), 1024, 0, st, 1, p.grad, p.n, norm)) return rc;
+        p.norm = norm;
+    }
+    return q.tensor ? tensor_backward<T>(p, q, dx, dw, scratch, st) : plain_backward(p, q, static_cast<float *>(dx), static_cast<float *>(dw), scratch, st);
 }
 
 static int check(const Problem &p) {
