@@ -54,6 +54,7 @@ def _on(device):
 
 
 def _outputs(rows, per_row, reduction, device):
+    """The loss and the state that goes to the backward call."""
     loss = torch.empty(rows if reduction == _native.REDUCE_NONE else (), dtype=torch.float32, device=device)
     state = torch.empty(rows * per_row + 4, dtype=torch.float32, device=device)      # the last four: the count of the rows
     return loss, state
