@@ -744,6 +744,7 @@ template <typename T> static int backward(Problem p, const Plan &q, void *dx, vo
 static int check(const Problem &p) {
     GRWS_REQUIRE(p.n >= 0 && p.d > 0 && p.V > 0, "bad size (rows = %lld, width = %lld, classes = %lld)", (long long)p.n, (long long)p.d, (long long)p.V);
     GRWS_REQUIRE(p.n <= INT32_MAX && p.d <= INT32_MAX && p.V <= INT32_MAX, "rows, width and classes must fit 31 bits");
+    GRWS_REQUIRE((double)p.n * (double)p.V < 3.0e13, "rows x classes must stay below 3e13");      // tiles are numbered in 31 bits
     GRWS_REQUIRE(p.ldx >= p.d && p.ldw >= (p.class_major ? p.d : p.V), "leading dimension smaller than the row");
     GRWS_REQUIRE(p.class_major == 0 || p.class_major == 1, "bad weight order %d", p.class_major);
     if (p.dtype < GRWS_F32 || p.dtype > GRWS_BF16) return fail(GRWS_ERR_UNSUPPORTED, "bad dtype %d", p.dtype);

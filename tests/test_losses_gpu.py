@@ -129,6 +129,12 @@ def test_cross_entropy_against_differences():
         assert abs(float(slope - got)) <= 1e-5 * float((dx.double() * u).abs().sum() + (dw.double() * v).abs().sum())
 
 
+@pytest.mark.parametrize("dtype,class_major", [(torch.float32, False), (torch.float16, True), (torch.bfloat16, False)])
+def test_cross_entropy_in_pieces_of_the_classes(dtype, class_major):
+    """So many rows that the workspace of the backward pass holds a part of the classes at a time."""
+    check_ce(*ce_inputs(70001, 24, 4501, dtype, class_major, ignored=0.2))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_cross_entropy_strides(dtype):
     """Operands cut from wider ones, at odd offsets, and orders that need a copy."""
@@ -404,6 +410,42 @@ def test_two_streams_at_once():
     for i in (0, 1):
         for r in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+def test_another_stream_than_the_operands_and_another_device():
+    x, w, y = ce_inputs(130, 64, 500, torch.bfloat16)
+    want = run_ce(x, w, y, "mean")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got = run_ce(x, w, y, "mean")
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    if torch.cuda.device_count() > 1:
+        from graph_rws_b200.layers import linear_cross_entropy
+        a, b = (t.to("cuda:1").requires_grad_(True) for t in (x, w))
+        assert torch.cuda.current_device() == 0
+        loss = linear_cross_entropy(a, b, y.to("cuda:1"))
+        grads = torch.autograd.grad(loss, (a, b))
+        assert loss.device.index == 1 and torch.equal(grads[0].cpu(), want[1].cpu()) and torch.equal(grads[1].cpu(), want[2].cpu())
+
+
+def test_broadcast_inputs_and_shared_weights():
+    """Gradients of a row used by all rows, and of a weight used twice, are sums."""
+    from graph_rws_b200.layers import distillation_loss, linear_cross_entropy
+    x, w, y = ce_inputs(60, 32, 90, torch.float32)
+    row = x[:1].detach().requires_grad_(True)
+    w1 = w.detach().requires_grad_(True)
+    loss = linear_cross_entropy(row.expand(60, 32), w1, y) + linear_cross_entropy(x, w1, y)
+    got = torch.autograd.grad(loss, (row, w1))
+    rd, wd = row.detach().double().requires_grad_(True), w.double().requires_grad_(True)
+    ref = torch.nn.functional.cross_entropy(rd.expand(60, 32) @ wd, y) + torch.nn.functional.cross_entropy(x.double() @ wd, y)
+    for a, b in zip(got, torch.autograd.grad(ref, (rd, wd))):
+        assert float((a - b).abs().max()) <= 1e-5 * float(b.abs().max())
+    z, t, ids = distill_inputs(40, 77, 5, torch.float32)
+    zr = z[:1].detach().clone().requires_grad_(True)
+    dz, = torch.autograd.grad(distillation_loss(zr.expand(40, 77), t, ids, temperature=2.0, reduction="sum"), zr)
+    _, _, dz64, _, _ = distill_reference(z[:1].expand(40, 77), t, ids, 2.0, torch.ones(40, device="cuda"))
+    assert dz.shape == (1, 77) and float((dz.double() - dz64.sum(0)).abs().max()) <= 1e-5 * float(dz64.sum(0).abs().max())
 
 
 def test_captured_step_replays_on_new_inputs():
