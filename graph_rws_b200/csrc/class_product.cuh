@@ -6,10 +6,12 @@
 // swizzled rows of 64 elements of K; of one whose outer axis is contiguous, 64 x 64 pieces of 64 outer elements a line.  Both
 // are read by the MMA as they are, so that no operand is ever transposed in memory.
 //
-// fp32 operands come as three bf16 planes (x = hi + mid + lo exactly to 24 bits), the inner axis is walked once per pair
-// of planes, the smallest products first: lo hi, hi lo, mid mid, mid hi, hi mid, hi hi.  What is left out (mid lo and below)
-// is 2^-24 of a product.  The tensor cores cut every sum off towards zero, so these sums are kept short: the five small pairs
-// are one of them, the big pair one for every two stages, and the epilogue adds them up in registers, rounding to nearest.
+// fp32 operands come as three bf16 planes (x = hi + mid + lo exactly to 24 bits): six products, hi hi, hi mid, mid hi, mid mid,
+// hi lo, lo hi.  What is left out (mid lo and below) is 2^-24 of a product.  The tensor cores cut every sum off towards zero,
+// so these sums are kept short: the five small pairs have an accumulator of their own, hi hi one for every two steps of the
+// inner axis, and the epilogue adds them up in registers, rounding to nearest.  Tiles have 128 columns, so that two of each
+// accumulator fit and a thread's 64 sums stay in registers; a stage is one plane of both operands, which all products that
+// need it read from where it lies.
 //
 // A persistent CTA (or a pair of CTAs that share the tile's columns, CG = 2) owns output tiles of 128 CG x up to 256; two
 // accumulators alternate, so the epilogue of one tile runs under the MMAs of the next.  Warps: 0-7 epilogue (warp % 4
@@ -30,18 +32,22 @@ namespace prod {
 
 using namespace cls;
 
-constexpr int BM = 128, BN = 256, BK = 64;          // rows per CTA, columns per tile at most, inner elements per stage
+constexpr int BM = 128, BK = 64;                    // rows per CTA, inner elements per stage
+constexpr int tile_width(int planes) { return planes == 3 ? 128 : 256; }            // columns per tile at most
+constexpr int MAX_STAGES = 8;
 constexpr int EPILOGUE_WARPS = 8, TMA_WARP = 8, MMA_WARP = 9, THREADS = 320;
 constexpr long long WAIT_LIMIT_CYCLES = 3000000000ll;   // about 1.5 to 2.5 s of SM clocks
 constexpr int MAX_TASKS = 2;
 constexpr int PIECE_BYTES = 64 * BK * 2;                // 64 of the outer axis of an operand: what one copy brings of B
 constexpr int BOX_BYTES = 32 * 128;                     // what a warp stores at once: 32 rows of 64 16-bit or 32 fp32 numbers
-constexpr int SUB_STAGES = 2;                           // fp32: stages of the big pair that are summed in tensor memory
+constexpr int SUB_STEPS = 2;                            // fp32: steps of 64 inner elements whose hi hi is summed in tensor memory
 
-template <int CG> struct Cfg {
+template <int CG, bool SPLIT> struct Cfg {
+    static constexpr int BN = tile_width(SPLIT ? 3 : 1);
     static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN / CG * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES = CG == 2 ? 6 : 4;
+    static constexpr int STAGES = 196608 / STAGE_BYTES;           // 192 KB: 4 to 8
     static constexpr int SMEM = STAGES * STAGE_BYTES + EPILOGUE_WARPS * BOX_BYTES + 1024;      // + alignment of the first stage
+    static_assert(STAGES <= MAX_STAGES && STAGES >= 4, "stages");
 };
 
 enum Mode : int { STATS = 0, GRAD = 1, SUM = 2 };
@@ -215,12 +221,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
                    "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(taddr) : "memory");
-}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // shared-memory matrix descriptor, 128-byte swizzle.  Inner axis contiguous: 8-row groups 1,024 bytes apart, a step of 16
@@ -287,7 +287,7 @@ struct Walk {
 };
 
 struct Shared {
-    uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
+    uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2], big_full[2], big_empty[2];
     uint32_t tmem;
     int abort_flag;
 };
@@ -326,7 +326,7 @@ __device__ __forceinline__ void split3(float v, float &a, float &b, float &c) {
 }
 
 template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
-    using C = Cfg<CG>;
+    using C = Cfg<CG, SPLIT>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Shared shared;
     Shared *ss = &shared;
@@ -342,7 +342,10 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
     if (threadIdx.x == 0) {
         ss->abort_flag = 0;
         for (int i = 0; i < C::STAGES; ++i) { mbar_init(smem_u32(&ss->full[i]), 1); mbar_init(smem_u32(&ss->empty[i]), 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&ss->acc_full[i]), 1); mbar_init(smem_u32(&ss->acc_empty[i]), EPILOGUE_WARPS * CG); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&ss->acc_full[i]), 1); mbar_init(smem_u32(&ss->acc_empty[i]), EPILOGUE_WARPS * CG);
+            mbar_init(smem_u32(&ss->big_full[i]), 1); mbar_init(smem_u32(&ss->big_empty[i]), EPILOGUE_WARPS * CG);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == TMA_WARP && lane < p.tasks) {
@@ -371,7 +374,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
             bool ok = true;
             uint32_t full0 = smem_u32(&ss->full[0]);
             if constexpr (CG == 2) full0 = map_to_rank(full0, 0);
-            constexpr int B_PIECES = BN / CG / 64;
+            constexpr int B_PIECES = C::BN / CG / 64, PLANES = SPLIT ? 3 : 1;
             for (Walk walk(p, units, first, stride); ok && walk.next();) {
                 const Unit w = unit_at(p, walk.u);
                 const Task &t = p.task[w.task];
@@ -383,26 +386,25 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                     const int cols = tile_columns(t, n) / CG, b_row = t.b_row0 + n * t.bn + (int)rank * cols;
                     const int pieces = b_outer ? (cols + 63) >> 6 : B_PIECES;
                     const uint32_t bytes = CG * (C::A_BYTES + pieces * PIECE_BYTES);
-                    for (int pair = SPLIT ? 0 : 5; ok && pair < 6; ++pair) {
-                        const int pa = pair == 0 ? 2 : pair == 2 || pair == 3 ? 1 : 0, pb = pair == 1 ? 2 : pair == 2 || pair == 4 ? 1 : 0;
-                        for (int kb = k0; kb < k1; ++kb) {
+                    for (int kb = k0; ok && kb < k1; ++kb) {
+                        for (int plane = 0; plane < PLANES; ++plane) {
                             if (!mbar_wait(smem_u32(&ss->empty[stage]), phase ^ 1u, abort_flag, limit)) { give_up(ss, p, WAIT_STAGE); ok = false; break; }
                             const uint32_t bar = full0 + stage * 8, a = ring + stage * C::STAGE_BYTES, b = a + C::A_BYTES;
                             const int ka = kb * BK, kB = b_k0 + ka;
                             if (rank == 0) mbar_expect_tx(smem_u32(&ss->full[stage]), bytes);
                             if (a_outer) {
 #pragma unroll
-                                for (int j = 0; j < BM / 64; ++j) tma_load<CG>(a + j * PIECE_BYTES, ma, bar, a_row + j * 64, ka, pa);
+                                for (int j = 0; j < BM / 64; ++j) tma_load<CG>(a + j * PIECE_BYTES, ma, bar, a_row + j * 64, ka, plane);
                             } else {
-                                tma_load<CG>(a, ma, bar, ka, a_row, pa);
+                                tma_load<CG>(a, ma, bar, ka, a_row, plane);
                             }
                             if (!b_outer) {
-                                tma_load<CG>(b, mb, bar, kB, b_row, pb);
+                                tma_load<CG>(b, mb, bar, kB, b_row, plane);
                             } else if (pieces == B_PIECES) {
 #pragma unroll
-                                for (int j = 0; j < B_PIECES; ++j) tma_load<CG>(b + j * PIECE_BYTES, mb, bar, b_row + j * 64, kB, pb);
+                                for (int j = 0; j < B_PIECES; ++j) tma_load<CG>(b + j * PIECE_BYTES, mb, bar, b_row + j * 64, kB, plane);
                             } else {
-                                for (int j = 0; j < pieces; ++j) tma_load<CG>(b + j * PIECE_BYTES, mb, bar, b_row + j * 64, kB, pb);
+                                for (int j = 0; j < pieces; ++j) tma_load<CG>(b + j * PIECE_BYTES, mb, bar, b_row + j * 64, kB, plane);
                             }
                             ++issued;
                             if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
@@ -426,36 +428,66 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
         if (rank == 0 && elect_one()) {
             int stage = 0;
             uint32_t phase = 0, tile = 0;
+            [[maybe_unused]] uint32_t chain = 0;
             bool ok = true;
             for (Walk walk(p, units, first, stride); ok && walk.next();) {
                 const Unit w = unit_at(p, walk.u);
                 const Task &t = p.task[w.task];
-                const int k0 = w.split * t.k_len, steps = (min(t.k_blocks, k0 + t.k_len) - k0) * (SPLIT ? 6 : 1);
+                const int k0 = w.split * t.k_len, steps = min(t.k_blocks, k0 + t.k_len) - k0;
                 const uint32_t idesc0 = (1u << 4) | ((uint32_t)p.bf16 << 7) | ((uint32_t)p.bf16 << 10) | ((uint32_t)t.a_outer << 15) |
                                         ((uint32_t)t.b_outer << 16) | ((uint32_t)(BM * CG >> 4) << 24);
                 const uint64_t a_step = t.a_outer ? 2048 >> 4 : 32 >> 4, b_step = t.b_outer ? 2048 >> 4 : 32 >> 4;
-                const int small = SPLIT ? steps / 6 * 5 : 0;
-                for (int n = w.n0; ok && n < w.n1; ++n) {
-                    const uint32_t idesc = idesc0 | ((uint32_t)(tile_columns(t, n) >> 3) << 17);
-                    // sums of the tile: all steps, or for fp32 the small pairs' and SUB_STAGES steps each of the big one's
-                    for (int k0s = 0; ok && k0s < steps; ++tile) {
-                        const int k1s = !SPLIT ? steps : k0s < small ? small : min(steps, k0s + SUB_STAGES);
-                        const uint32_t buf = tile & 1u, d = tmem + buf * BN;
-                        if (!mbar_wait(smem_u32(&ss->acc_empty[buf]), ((tile >> 1) & 1u) ^ 1u, abort_flag, limit)) { give_up(ss, p, WAIT_ACCUMULATOR); ok = false; break; }
-                        tc_fence_after();
-                        for (int k = k0s; k < k1s; ++k) {
-                            if (!mbar_wait(smem_u32(&ss->full[stage]), phase, abort_flag, limit)) { give_up(ss, p, WAIT_OPERANDS); ok = false; break; }
-                            tc_fence_after();
-                            const uint32_t a = ring + stage * C::STAGE_BYTES;
-                            const uint64_t ad = smem_desc(a, t.a_outer), bd = smem_desc(a + C::A_BYTES, t.b_outer);
+                auto advance = [&]() { if (++stage == C::STAGES) { stage = 0; phase ^= 1u; } };
+                auto wait_stage = [&](int at, uint32_t parity) {
+                    if (mbar_wait(smem_u32(&ss->full[at]), parity, abort_flag, limit)) { tc_fence_after(); return true; }
+                    give_up(ss, p, WAIT_OPERANDS);
+                    return false;
+                };
+                auto wait_empty = [&](uint64_t *bar, uint32_t use) {
+                    if (mbar_wait(smem_u32(&bar[use & 1u]), ((use >> 1) & 1u) ^ 1u, abort_flag, limit)) { tc_fence_after(); return true; }
+                    give_up(ss, p, WAIT_ACCUMULATOR);
+                    return false;
+                };
+                for (int n = w.n0; ok && n < w.n1; ++n, ++tile) {
+                    const uint32_t idesc = idesc0 | ((uint32_t)(tile_columns(t, n) >> 3) << 17), d = tmem + (tile & 1u) * C::BN;
+                    // the product of stage i's A and stage j's B; `add`: onto what is there
+                    auto multiply = [&](uint32_t to, int i, int j, bool add) {
+                        const uint64_t ad = smem_desc(ring + i * C::STAGE_BYTES, t.a_outer), bd = smem_desc(ring + j * C::STAGE_BYTES + C::A_BYTES, t.b_outer);
 #pragma unroll
-                            for (int i = 0; i < BK / 16; ++i) umma<CG>(d, ad + i * a_step, bd + i * b_step, idesc, k > k0s || i > 0);
+                        for (int k = 0; k < BK / 16; ++k) umma<CG>(to, ad + k * a_step, bd + k * b_step, idesc, add || k > 0);
+                    };
+                    ok = wait_empty(ss->acc_empty, tile);
+                    for (int k = 0; ok && k < steps; ++k) {
+                        if constexpr (!SPLIT) {
+                            if (!(ok = wait_stage(stage, phase))) break;
+                            multiply(d, stage, stage, k > 0);
                             umma_commit<CG>(smem_u32(&ss->empty[stage]));
-                            if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                            advance();
+                        } else {
+                            const uint32_t db = tmem + 2 * C::BN + (chain & 1u) * C::BN;
+                            const int hi = stage;
+                            if (k % SUB_STEPS == 0 && !(ok = wait_empty(ss->big_empty, chain))) break;
+                            if (!(ok = wait_stage(stage, phase))) break;
+                            multiply(db, hi, hi, k % SUB_STEPS != 0);
+                            advance();
+                            const int mid = stage;
+                            if (!(ok = wait_stage(stage, phase))) break;
+                            multiply(d, hi, mid, k > 0);
+                            multiply(d, mid, hi, true);
+                            multiply(d, mid, mid, true);
+                            advance();
+                            const int lo = stage;
+                            if (!(ok = wait_stage(stage, phase))) break;
+                            multiply(d, hi, lo, true);
+                            multiply(d, lo, hi, true);
+                            advance();
+                            umma_commit<CG>(smem_u32(&ss->empty[hi]));
+                            umma_commit<CG>(smem_u32(&ss->empty[mid]));
+                            umma_commit<CG>(smem_u32(&ss->empty[lo]));
+                            if (k % SUB_STEPS == SUB_STEPS - 1 || k == steps - 1) { umma_commit<CG>(smem_u32(&ss->big_full[chain & 1u])); ++chain; }
                         }
-                        if (ok) umma_commit<CG>(smem_u32(&ss->acc_full[buf]));
-                        k0s = k1s;
                     }
+                    if (ok) umma_commit<CG>(smem_u32(&ss->acc_full[tile & 1u]));
                 }
             }
         }
@@ -464,29 +496,23 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
         const int quarter = warp & 3, half = warp >> 2;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t box = ring + C::STAGES * C::STAGE_BYTES + warp * BOX_BYTES;
-        uint32_t acc_empty[2];
-        for (int i = 0; i < 2; ++i) {
-            acc_empty[i] = smem_u32(&ss->acc_empty[i]);
-            if constexpr (CG == 2) acc_empty[i] = map_to_rank(acc_empty[i], 0);
-        }
         uint32_t tile = 0;
+        [[maybe_unused]] uint32_t chain = 0;
         bool ok = true;
-        auto wait_tile = [&]() {
-            const uint32_t buf = tile & 1u;
-            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&ss->acc_full[buf]), (tile >> 1) & 1u, abort_flag, limit));
+        // waits for an accumulator's `use`-th sum, and gives it back
+        auto wait_sum = [&](uint64_t *full, uint32_t use) {
+            ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[use & 1u]), (use >> 1) & 1u, abort_flag, limit));
             if (!ok) give_up(ss, p, WAIT_TILE);
             tc_fence_after();
-            return tmem + buf * BN + lanes;
         };
-        auto release_tile = [&]() {
-            const uint32_t buf = tile & 1u;
+        auto release_sum = [&](uint64_t *empty, uint32_t use) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                if constexpr (CG == 2) mbar_arrive_cluster(acc_empty[buf]);
-                else mbar_arrive(acc_empty[buf]);
+                const uint32_t bar = smem_u32(&empty[use & 1u]);
+                if constexpr (CG == 2) mbar_arrive_cluster(map_to_rank(bar, 0));
+                else mbar_arrive(bar);
             }
-            ++tile;
         };
         // 16 bytes of this lane's row of the box, swizzled as the store expects them
         auto put = [&](int piece, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -530,7 +556,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
             for (int n = w.n0; ok && n < w.n1; ++n) {
                 const int64_t col0 = (int64_t)n * t.bn;
                 const int cols = (int)min((int64_t)t.bn, t.N - col0);          // of this tile
-                const int mine = (int)max((int64_t)-1, min((int64_t)BN, label - p.v0 - col0));    // label's column, if within
+                const int mine = (int)max((int64_t)-1, min((int64_t)C::BN, label - p.v0 - col0));    // label's column, if within
                 (void)mine;
                 // W columns from c on: 64, for fp32 16
                 constexpr int W = SPLIT ? 16 : 64;
@@ -646,11 +672,12 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                         }
                     }
                 };
+                const uint32_t at = tmem + (tile & 1u) * C::BN + lanes;
                 if constexpr (!SPLIT) {
-                    const uint32_t at = wait_tile();
+                    wait_sum(ss->acc_full, tile);
                     if (!ok) break;
                     const int last = (cols - 1 - half * 64) >> 7;          // 64-column pieces of this warp, less one (-1: none)
-                    if (last < 0) release_tile();
+                    if (last < 0) release_sum(ss->acc_empty, tile);
                     for (int k = 0; k <= last; ++k) {
                         const int c = half * 64 + k * 128;
                         float v[64];
@@ -658,36 +685,45 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                         tmem_ld32(at + c, r);
                         tmem_ld32(at + c + 32, r2);
                         tmem_ld_wait();
-                        if (k == last) release_tile();
+                        if (k == last) release_sum(ss->acc_empty, tile);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) { v[i] = __uint_as_float(r[i]); v[32 + i] = __uint_as_float(r2[i]); }
                         use(v, c);
                     }
                 } else {
-                    const int k0 = w.split * t.k_len, big = min(t.k_blocks, k0 + t.k_len) - k0;
-                    float acc[8][W];
-                    for (int sub = 0; ok && sub <= (big + SUB_STAGES - 1) / SUB_STAGES; ++sub) {
-                        const uint32_t at = wait_tile();
-                        if (!ok) break;
+                    const int k0 = w.split * t.k_len, steps = min(t.k_blocks, k0 + t.k_len) - k0, chains = (steps + SUB_STEPS - 1) / SUB_STEPS;
+                    const int c = half * 64;
+                    float acc[4][W];
+                    auto add_up = [&](uint32_t from, bool first) {
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const int c = half * 64 + (k >> 2) * 128 + (k & 3) * 16;
-                            if (c >= cols) continue;
-                            uint32_t r[16];
-                            tmem_ld16(at + c, r);
+                        for (int k = 0; k < 4; k += 2) {
+                            if (c + k * W >= cols) break;
+                            uint32_t r[2 * W];
+                            tmem_ld32(from + c + k * W, r);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) acc[k][i] = sub ? acc[k][i] + __uint_as_float(r[i]) : __uint_as_float(r[i]);
+                            for (int i = 0; i < 2 * W; ++i) {
+                                const float v = __uint_as_float(r[i]);
+                                acc[k + i / W][i % W] = first ? v : acc[k + i / W][i % W] + v;
+                            }
                         }
-                        release_tile();
+                    };
+                    for (int sub = 0; sub < chains; ++sub, ++chain) {
+                        wait_sum(ss->big_full, chain);
+                        if (!ok) break;
+                        add_up(tmem + 2 * C::BN + (chain & 1u) * C::BN + lanes, sub == 0);
+                        release_sum(ss->big_empty, chain);
                     }
                     if (!ok) break;
+                    wait_sum(ss->acc_full, tile);
+                    if (!ok) break;
+                    add_up(at, false);
+                    release_sum(ss->acc_empty, tile);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int c = half * 64 + (k >> 2) * 128 + (k & 3) * 16;
-                        if (c < cols) use(acc[k], c);
-                    }
+                    for (int k = 0; k < 4; ++k)
+                        if (c + k * W < cols) use(acc[k], c + k * W);
                 }
+                ++tile;
             }
             if constexpr (MODE == STATS) {
                 if (ok && in) p.part[(int64_t)((w.n0 / t.run) * 2 + half) * t.M + row] = make_float2(m, s);
@@ -740,14 +776,15 @@ template <int CG, int MODE, bool SPLIT> static int launch_product(const Maps &ma
     int64_t units = 0;
     for (int i = 0; i < p.tasks; ++i) units += p.task[i].units();
     const int64_t clusters = units < sm_count() / CG ? units : sm_count() / CG;
+    using C = Cfg<CG, SPLIT>;
     static bool allowed[MAX_DEVICES];
     const int dev = current_device();
     if (dev < 0) return fail(GRWS_ERR_CUDA, "no current device");
     if (!__atomic_load_n(&allowed[dev], __ATOMIC_RELAXED)) {
-        GRWS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<CG, MODE, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<CG>::SMEM));
+        GRWS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<CG, MODE, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         __atomic_store_n(&allowed[dev], true, __ATOMIC_RELAXED);
     }
-    return launch_next(product_kernel<CG, MODE, SPLIT>, dim3((unsigned)(clusters * CG)), THREADS, Cfg<CG>::SMEM, st, CG, maps, p);
+    return launch_next(product_kernel<CG, MODE, SPLIT>, dim3((unsigned)(clusters * CG)), THREADS, C::SMEM, st, CG, maps, p);
 }
 
 }  // namespace prod

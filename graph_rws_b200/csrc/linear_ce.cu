@@ -333,6 +333,7 @@ static __device__ int g_status;
 // plan: how a call is cut up, and where its workspace lies
 // ---------------------------------------------------------------------------------------------
 constexpr size_t PIECE_BYTES = 512ull << 20;       // workspace for G
+constexpr int64_t PIECE_UNIT = 256;                // its columns come in whole tiles
 
 struct Plan {
     bool tensor;
@@ -368,11 +369,15 @@ static void cut(int64_t tiles, int64_t K, int64_t least, int64_t unit, int64_t *
 }
 
 static int64_t in_32s(int64_t N) { return ceil_div(N, (int64_t)32) * 32; }
-static int columns_per_tile(int64_t N) {
-    const int64_t tiles = ceil_div(N, (int64_t)prod::BN);
+static int64_t column_tiles(int64_t N, int planes) { return ceil_div(N, (int64_t)prod::tile_width(planes)); }
+static int columns_per_tile(int64_t N, int planes) {
+    const int64_t tiles = column_tiles(N, planes);
     return (int)(tiles == 1 ? in_32s(N) : ceil_div(ceil_div(N, tiles), (int64_t)64) * 64);
 }
-static int64_t tiles_of(int64_t M, int64_t N, int cg) { return ceil_div(M, (int64_t)(prod::BM * cg)) * ceil_div(N, (int64_t)prod::BN); }
+static int64_t tiles_of(int64_t M, int64_t N, int cg, int planes) { return ceil_div(M, (int64_t)(prod::BM * cg)) * column_tiles(N, planes); }
+// What 64 inner elements of a tile take, in steps of a 256 x 256 tile (some 0.4 us of a pair of SMs): fp32 has six products of half the width
+static int64_t step_cost(int planes) { return planes == 3 ? 3 : 1; }
+
 // CTAs that share a tile: pairs where there are more rows than one CTA's
 static int cta_group(int64_t M) { return M > prod::BM ? 2 : 1; }
 
@@ -414,7 +419,8 @@ static int64_t deal_units(int64_t u0, int64_t l0, int64_t u1, int64_t l1, int64_
 // Parts of the inner axes of dx (classes of a piece) and dw (rows), which run in one launch: short units leave the CTAs equally
 // busy, but every part is one more plane of fp32 sums through memory.  Costs are in
 // units of one 64-element step of one tile, about 0.4 us of a pair of SMs; a launch that adds planes up takes some 6 us.
-static double cut_products(int64_t tiles0, int64_t k0, double sums0, int64_t tiles1, int64_t k1, double sums1, int64_t ctas, int64_t *parts0, int64_t *parts1) {
+static double cut_products(int64_t tiles0, int64_t k0, double sums0, int64_t tiles1, int64_t k1, double sums1, int64_t step, int64_t ctas, int64_t *parts0,
+                           int64_t *parts1) {
     static const int64_t tries[] = {1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 12, 14, 16, 18, 20, 24, 28, 32, 37, 48, 64, 74, 96, 128, 148};
     const double step_us = 0.4, plane_us = 8.0 / 2.5e6;          // an fp32 number written and read at 2.5 TB/s
     double best = 1e300;
@@ -423,7 +429,7 @@ static double cut_products(int64_t tiles0, int64_t k0, double sums0, int64_t til
         for (int64_t b : tries) {
             if (b > 1 && (k1 / b < 8 || tiles1 * b > 6 * ctas)) break;
             const int64_t l0 = ceil_div(k0, a), l1 = ceil_div(k1, b), u0 = tiles0 * a, u1 = tiles1 * b;
-            const int64_t t0 = unit_time(l0), t1 = unit_time(l1);
+            const int64_t t0 = unit_time(l0 * step), t1 = unit_time(l1 * step);
             double cost = (double)(l1 >= l0 ? deal_units(u1, t1, u0, t0, ctas, nullptr, nullptr) : deal_units(u0, t0, u1, t1, ctas, nullptr, nullptr));
             if (a > 1) cost += (6.0 + (double)a * sums0 * plane_us) / step_us;
             if (b > 1) cost += (6.0 + (double)b * sums1 * plane_us) / step_us;
@@ -478,24 +484,24 @@ static Plan make_plan(const Problem &p, bool backward) {
     if (q.pack_w) q.w = place(at, (size_t)q.planes * w_rows * q.ldw * 2);
     const int cg = cta_group(n);
     if (!backward) {
-        const int64_t bn = columns_per_tile(V);
-        cut_runs(n, ceil_div(n, (int64_t)(prod::BM * cg)), ceil_div(V, bn), ceil_div(d, (int64_t)prod::BK) * (q.planes == 3 ? 6 : 1), sm_count() / cg, true, &q.run, &q.parts);
+        const int64_t bn = columns_per_tile(V, q.planes);
+        cut_runs(n, ceil_div(n, (int64_t)(prod::BM * cg)), ceil_div(V, bn), ceil_div(d, (int64_t)prod::BK) * step_cost(q.planes), sm_count() / cg, true, &q.run, &q.parts);
         q.stats = place(at, (size_t)q.parts * 2 * n * sizeof(float2));
         place_rows(at, n, &q);
     } else {
-        int64_t most = (int64_t)(PIECE_BYTES / (2 * q.planes)) / n / prod::BN * prod::BN;
-        if (most < prod::BN) most = prod::BN;
+        int64_t most = (int64_t)(PIECE_BYTES / (2 * q.planes)) / n / PIECE_UNIT * PIECE_UNIT;
+        if (most < PIECE_UNIT) most = PIECE_UNIT;
         const int pg = cta_group(n > d ? n : d);
         const int64_t k1 = ceil_div(n, (int64_t)prod::BK);
         double best = 1e300;
         // the largest piece, or one down to half of it whose products leave the SMs more equally busy
-        const int64_t all = ceil_div(V, (int64_t)prod::BN) * prod::BN, top = most < all ? most : all;
+        const int64_t all = ceil_div(V, PIECE_UNIT) * PIECE_UNIT, top = most < all ? most : all;
         for (int64_t k = 8; k >= 4; --k) {
-            const int64_t piece = ceil_div(top * k / 8, (int64_t)prod::BN) * prod::BN;
+            const int64_t piece = ceil_div(top * k / 8, PIECE_UNIT) * PIECE_UNIT;
             const int64_t c = piece < V ? piece : V;
-            const int64_t tiles0 = tiles_of(n, d, pg), tiles1 = p.class_major ? tiles_of(c, d, pg) : tiles_of(d, c, pg);
+            const int64_t tiles0 = tiles_of(n, d, pg, q.planes), tiles1 = p.class_major ? tiles_of(c, d, pg, q.planes) : tiles_of(d, c, pg, q.planes);
             int64_t a, b;
-            const double cost = (cut_products(tiles0, ceil_div(c, (int64_t)prod::BK), (double)n * d, tiles1, k1, (double)d * c, sm_count() / pg, &a, &b) +
+            const double cost = (cut_products(tiles0, ceil_div(c, (int64_t)prod::BK), (double)n * d, tiles1, k1, (double)d * c, step_cost(q.planes), sm_count() / pg, &a, &b) +
                                  (c < V ? (double)n * d * 8.0 / 5.0e6 / 0.4 : 0.0)) * (double)ceil_div(V, c);
             if (cost < best) { best = cost; q.piece = c; q.dx_parts = a; q.dw_parts = b; }
         }
@@ -551,7 +557,7 @@ template <typename T> static int pack_operands(const Problem &p, const Plan &q, 
 static int set_task(prod::Task *t, CUtensorMap *ma, CUtensorMap *mb, int cg, int dtype, const View &a, int a_outer, const View &b, int b_outer, int64_t M,
                     int64_t N, int64_t K) {
     t->M = M; t->N = N;
-    t->bn = columns_per_tile(N);
+    t->bn = columns_per_tile(N, a.planes);
     t->m_tiles = (int)ceil_div(M, (int64_t)(prod::BM * cg));
     t->n_tiles = (int)ceil_div(N, (int64_t)t->bn);
     t->run = 1; t->runs = t->n_tiles; t->splits = 1;
@@ -559,7 +565,7 @@ static int set_task(prod::Task *t, CUtensorMap *ma, CUtensorMap *mb, int cg, int
     t->group = t->m_tiles < 16 ? t->m_tiles : 16;
     t->a_outer = a_outer; t->b_outer = b_outer;
     if (int rc = prod::encode_map(ma, a.p, dtype, a.cols, a.rows, a.ld, a.planes, a.plane, 64, a_outer ? prod::BK : prod::BM)) return rc;
-    return prod::encode_map(mb, b.p, dtype, b.cols, b.rows, b.ld, b.planes, b.plane, 64, b_outer ? prod::BK : prod::BN / cg);
+    return prod::encode_map(mb, b.p, dtype, b.cols, b.rows, b.ld, b.planes, b.plane, 64, b_outer ? prod::BK : prod::tile_width(b.planes) / cg);
 }
 
 // where a SUM task's results go: planes of fp32 sums, or the rounded output
@@ -646,7 +652,7 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
         if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, o.dtype, o.x, 0, o.w, !p.class_major, p.n, cols, p.d)) return rc;
         if (int rc = prod::encode_map(&maps.c[0], G.p, o.dtype, cols, p.n, q.ldg, q.planes, G.plane, q.planes == 3 ? 16 : 64, 32)) return rc;
         int64_t run, runs;
-        cut_runs(p.n, r.task[0].m_tiles, r.task[0].n_tiles, r.task[0].k_blocks * (q.planes == 3 ? 6 : 1), sm_count() / cg, false, &run, &runs);
+        cut_runs(p.n, r.task[0].m_tiles, r.task[0].n_tiles, r.task[0].k_blocks * step_cost(q.planes), sm_count() / cg, false, &run, &runs);
         r.task[0].run = (int)run;
         r.task[0].runs = (int)runs;
         r.task[0].b_row0 = (int)v0;
@@ -688,7 +694,7 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
         // few units per CTA: dealt out by length (many: in order, so that those at work at a time share operands in L2)
         if (r.tasks > 1 && units <= 12 * ctas) {
             r.deal = 1;
-            deal_units(r.task[0].units(), unit_time(r.task[0].k_len), r.task[1].units(), unit_time(r.task[1].k_len), units < ctas ? units : ctas, &r.deal_less, &r.deal_more);
+            deal_units(r.task[0].units(), unit_time(r.task[0].k_len * step_cost(q.planes)), r.task[1].units(), unit_time(r.task[1].k_len * step_cost(q.planes)), units < ctas ? units : ctas, &r.deal_less, &r.deal_more);
         }
         if (int rc = launch_product<prod::SUM>(pg, q.planes, maps, r, st)) return rc;
         if (dw && sum_dw) if (int rc = launch_round<T>(p, dw_sum, q.dw_parts, M, N, q.ld_dw, r.scale, dw_out, ldo, 1, st)) return rc;
