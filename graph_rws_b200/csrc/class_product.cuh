@@ -34,19 +34,20 @@ using namespace cls;
 
 constexpr int BM = 128, BK = 64;                    // rows per CTA, inner elements per stage
 constexpr int tile_width(int planes) { return planes == 3 ? 128 : 256; }            // columns per tile at most
-constexpr int MAX_STAGES = 8;
+constexpr int MAX_STAGES = 8, SMEM_BYTES = 231936;        // 227 KB less what the barriers take
 constexpr int EPILOGUE_WARPS = 8, TMA_WARP = 8, MMA_WARP = 9, THREADS = 320;
 constexpr long long WAIT_LIMIT_CYCLES = 3000000000ll;   // about 1.5 to 2.5 s of SM clocks
 constexpr int MAX_TASKS = 2;
 constexpr int PIECE_BYTES = 64 * BK * 2;                // 64 of the outer axis of an operand: what one copy brings of B
-constexpr int BOX_BYTES = 32 * 128;                     // what a warp stores at once: 32 rows of 64 16-bit or 32 fp32 numbers
 constexpr int SUB_STEPS = 2;                            // fp32: steps of 64 inner elements whose hi hi is summed in tensor memory
 
 template <int CG, bool SPLIT> struct Cfg {
     static constexpr int BN = tile_width(SPLIT ? 3 : 1);
     static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN / CG * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES = 196608 / STAGE_BYTES;           // 192 KB: 4 to 8
-    static constexpr int SMEM = STAGES * STAGE_BYTES + EPILOGUE_WARPS * BOX_BYTES + 1024;      // + alignment of the first stage
+    // what a warp stores at once: 32 rows of 64 16-bit or 32 fp32 numbers, or of three planes of 32
+    static constexpr int BOX_BYTES = SPLIT ? 3 * 32 * 64 : 32 * 128;
+    static constexpr int STAGES = (SMEM_BYTES - 1024 - EPILOGUE_WARPS * BOX_BYTES) / STAGE_BYTES;          // (1,024: alignment of the first stage)
+    static constexpr int SMEM = STAGES * STAGE_BYTES + EPILOGUE_WARPS * BOX_BYTES + 1024;
     static_assert(STAGES <= MAX_STAGES && STAGES >= 4, "stages");
 };
 
@@ -495,7 +496,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
     } else {
         const int quarter = warp & 3, half = warp >> 2;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        const uint32_t box = ring + C::STAGES * C::STAGE_BYTES + warp * BOX_BYTES;
+        const uint32_t box = ring + C::STAGES * C::STAGE_BYTES + warp * C::BOX_BYTES;
         uint32_t tile = 0;
         [[maybe_unused]] uint32_t chain = 0;
         bool ok = true;
@@ -558,8 +559,8 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                 const int cols = (int)min((int64_t)t.bn, t.N - col0);          // of this tile
                 const int mine = (int)max((int64_t)-1, min((int64_t)C::BN, label - p.v0 - col0));    // label's column, if within
                 (void)mine;
-                // W columns from c on: 64, for fp32 16
-                constexpr int W = SPLIT ? 16 : 64;
+                // W columns from c on
+                constexpr int W = SPLIT ? 32 : 64;
                 auto put16 = [&](const float (&v)[W], uint32_t mask) {
                     if (p.bf16) {
 #pragma unroll
@@ -600,7 +601,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                             put16(v, factor == 0.0f ? 0u : ~0u);
                             box_out(mc, (int)col0 + c, row0, 0, false);
                         } else {
-                            // the three planes of 16 columns: boxes of 32-byte lines
+                            // the three planes: boxes of 64-byte lines, not swizzled
                             if (factor == 0.0f) {
 #pragma unroll
                                 for (int i = 0; i < W; ++i) v[i] = 0.0f;
@@ -618,13 +619,13 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                                     q[2][j / 2] = pack2<true>(d[0], d[1]);
                                 }
 #pragma unroll
-                                for (int k = 0; k < 3; ++k) st_shared16(box + k * 1024 + lane * 32 + i * 2, q[k][0], q[k][1], q[k][2], q[k][3]);
+                                for (int k = 0; k < 3; ++k) st_shared16(box + k * 2048 + lane * 64 + i * 2, q[k][0], q[k][1], q[k][2], q[k][3]);
                             }
                             fence_async_smem();
                             __syncwarp();
                             if (lane == 0) {
 #pragma unroll
-                                for (int k = 0; k < 3; ++k) tma_store(mc, box + k * 1024, (int)col0 + c, row0, k);
+                                for (int k = 0; k < 3; ++k) tma_store(mc, box + k * 2048, (int)col0 + c, row0, k);
                                 bulk_commit();
                             }
                         }
@@ -646,27 +647,19 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                                 __syncwarp();
                                 return;
                             }
+                        }
 #pragma unroll
-                            for (int h = 0; h < W; h += 32) {
-                                if (c + h >= cols) return;
-                                box_free();
-#pragma unroll
-                                for (int i = 0; i < 32; i += 4)
-                                    put(i / 4, __float_as_uint(v[h + i]), __float_as_uint(v[h + i + 1]), __float_as_uint(v[h + i + 2]), __float_as_uint(v[h + i + 3]));
-                                box_out(mc, (int)col0 + c + h, row0, w.split, t.add);
-                            }
-                        } else {
-                            // 16 fp32 columns: lines of 64 bytes
+                        for (int h = 0; h < W; h += 32) {
+                            if (c + h >= cols) return;
                             box_free();
 #pragma unroll
-                            for (int i = 0; i < W; i += 4)
-                                st_shared16(box + lane * 64 + i * 4, __float_as_uint(v[i]), __float_as_uint(v[i + 1]), __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]));
-                            if (!t.out) { box_out(mc, (int)col0 + c, row0, w.split, t.add); return; }
+                            for (int i = 0; i < 32; i += 4)
+                                put(i / 4, __float_as_uint(v[h + i]), __float_as_uint(v[h + i + 1]), __float_as_uint(v[h + i + 2]), __float_as_uint(v[h + i + 3]));
+                            if (!t.out) { box_out(mc, (int)col0 + c + h, row0, w.split, t.add); continue; }
                             __syncwarp();
-                            for (int r = 0; r < 32 && row0 + r < t.M; r += 2) {
-                                const int rr = r + (lane >> 4), cc = lane & 15;
-                                if (row0 + rr < t.M && c + cc < cols)
-                                    static_cast<float *>(t.out)[(row0 + rr) * t.ldo + col0 + c + cc] = __uint_as_float(ld_shared32(box + rr * 64 + cc * 4));
+                            for (int r = 0; r < 32 && row0 + r < t.M; ++r) {
+                                const uint32_t one = ld_shared32(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                                if (c + h + lane < cols) static_cast<float *>(t.out)[(row0 + r) * t.ldo + col0 + c + h + lane] = __uint_as_float(one);
                             }
                             __syncwarp();
                         }
@@ -693,19 +686,16 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                 } else {
                     const int k0 = w.split * t.k_len, steps = min(t.k_blocks, k0 + t.k_len) - k0, chains = (steps + SUB_STEPS - 1) / SUB_STEPS;
                     const int c = half * 64;
-                    float acc[4][W];
+                    float acc[2][W];
                     auto add_up = [&](uint32_t from, bool first) {
 #pragma unroll
-                        for (int k = 0; k < 4; k += 2) {
+                        for (int k = 0; k < 2; ++k) {
                             if (c + k * W >= cols) break;
-                            uint32_t r[2 * W];
+                            uint32_t r[W];
                             tmem_ld32(from + c + k * W, r);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 2 * W; ++i) {
-                                const float v = __uint_as_float(r[i]);
-                                acc[k + i / W][i % W] = first ? v : acc[k + i / W][i % W] + v;
-                            }
+                            for (int i = 0; i < W; ++i) acc[k][i] = first ? __uint_as_float(r[i]) : acc[k][i] + __uint_as_float(r[i]);
                         }
                     };
                     for (int sub = 0; sub < chains; ++sub, ++chain) {
@@ -720,7 +710,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                     add_up(at, false);
                     release_sum(ss->acc_empty, tile);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
+                    for (int k = 0; k < 2; ++k)
                         if (c + k * W < cols) use(acc[k], c + k * W);
                 }
                 ++tile;

@@ -289,40 +289,44 @@ template <typename T> __global__ void __launch_bounds__(256) round_kernel(const 
     }
 }
 
-// Operand for the tensor cores from one whose rows no TMA copy can start at (or of fp32: three bf16 planes): rows of `ldp`
-// elements, a multiple of 8.  A thread per 8 elements.
-template <typename T> __global__ void __launch_bounds__(256) pack_kernel(const T *__restrict__ src, int64_t ld, int64_t rows, int64_t cols,
-                                                                         uint16_t *__restrict__ dst, int64_t ldp, int64_t plane) {
-    const int64_t per_row = ldp / 8, total = rows * per_row;
+// Operands for the tensor cores from those whose rows no TMA copy can start at (or of fp32: three bf16 planes): rows of `ldp`
+// elements, a multiple of 8.  A thread per 8 elements, both operands in one launch.
+struct PackTask { const void *src; uint16_t *dst; int64_t ld, rows, cols, ldp; };
+
+template <typename T> __device__ __forceinline__ void pack8(const PackTask &t, int64_t i) {
+    const int64_t per_row = t.ldp / 8, row = i / per_row, c = (i - row * per_row) * 8, plane = t.rows * t.ldp;
+    const T *s = static_cast<const T *>(t.src) + row * t.ld + c;
+    uint16_t *d = t.dst + row * t.ldp + c;
+    if constexpr (sizeof(T) == 2) {
+        uint32_t q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t lo = c + 2 * j < t.cols ? reinterpret_cast<const uint16_t *>(s)[2 * j] : 0;
+            const uint32_t hi = c + 2 * j + 1 < t.cols ? reinterpret_cast<const uint16_t *>(s)[2 * j + 1] : 0;
+            q[j] = lo | hi << 16;
+        }
+        *reinterpret_cast<uint4 *>(d) = make_uint4(q[0], q[1], q[2], q[3]);
+    } else {
+        uint32_t q[3][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float a[2], b[2], e[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) prod::split3(c + 2 * j + h < t.cols ? to_float(s[2 * j + h]) : 0.0f, a[h], b[h], e[h]);
+            q[0][j] = prod::pack2<true>(a[0], a[1]);
+            q[1][j] = prod::pack2<true>(b[0], b[1]);
+            q[2][j] = prod::pack2<true>(e[0], e[1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4 *>(d + k * plane) = make_uint4(q[k][0], q[k][1], q[k][2], q[k][3]);
+    }
+}
+template <typename T> __global__ void __launch_bounds__(256) pack_kernel(const PackTask a, const PackTask b) {
+    const int64_t first = a.rows * (a.ldp / 8), total = first + b.rows * (b.ldp / 8);
     wait_for_previous();
     let_next_start();
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / per_row, c = (i - row * per_row) * 8;
-        const T *s = src + row * ld + c;
-        uint16_t *d = dst + row * ldp + c;
-        if constexpr (sizeof(T) == 2) {
-            uint32_t q[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t lo = c + 2 * j < cols ? reinterpret_cast<const uint16_t *>(s)[2 * j] : 0;
-                const uint32_t hi = c + 2 * j + 1 < cols ? reinterpret_cast<const uint16_t *>(s)[2 * j + 1] : 0;
-                q[j] = lo | hi << 16;
-            }
-            *reinterpret_cast<uint4 *>(d) = make_uint4(q[0], q[1], q[2], q[3]);
-        } else {
-            uint32_t q[3][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float a[2], b[2], e[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) prod::split3(c + 2 * j + h < cols ? to_float(s[2 * j + h]) : 0.0f, a[h], b[h], e[h]);
-                q[0][j] = prod::pack2<true>(a[0], a[1]);
-                q[1][j] = prod::pack2<true>(b[0], b[1]);
-                q[2][j] = prod::pack2<true>(e[0], e[1]);
-            }
-#pragma unroll
-            for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4 *>(d + k * plane) = make_uint4(q[k][0], q[k][1], q[k][2], q[k][3]);
-        }
+        if (i < first) pack8<T>(a, i); else pack8<T>(b, i - first);
     }
 }
 
@@ -440,11 +444,10 @@ static double cut_products(int64_t tiles0, int64_t k0, double sums0, int64_t til
 }
 
 // 16-bit operands always go to the tensor cores (140 x 32 x 7: 20.7 us against 24.7 on the general cores, 300 x 256 x 40: 23
-// against 66).  fp32 costs them six products of packed planes: 35 against 25 us and 48 against 68; narrow rows, where a tile's
-// sums are over after a step or two, stay on the general cores for longer (170,000 x 16 x 7: 310 against 189).
+// against 66), fp32 from 2^21 products on (128 x 128 x 128: 33 us against 43; 256 x 64 x 47: 35 against 33; 140 x 32 x 7: 29
+// against 25, and five launches more).
 static bool on_tensor_cores(int64_t n, int64_t d, int64_t V, int dtype) {
-    const double products = (double)n * (double)d * (double)V;
-    return dtype != GRWS_F32 || products >= (double)(1 << 26) || (d >= 192 && products >= (double)(1 << 21));
+    return dtype != GRWS_F32 || (double)n * (double)d * (double)V >= (double)(1 << 21);
 }
 
 static Plan make_plan(const Problem &p, bool backward) {
@@ -535,22 +538,17 @@ template <typename T> static int launch_round(const Problem &p, const float *par
 struct View { const void *p; int64_t rows, cols, ld, plane; int planes; };
 struct Operands { View x, w; int dtype; };
 
-template <typename T> static int launch_pack(const void *src, int64_t ld, int64_t rows, int64_t cols, void *dst, int64_t ldp, cudaStream_t st) {
-    int64_t g = ceil_div(rows * (ldp / 8), (int64_t)256);
-    const int64_t most = (int64_t)sm_count() * 8;
-    if (g > most) g = most;
-    return launch_next(pack_kernel<T>, dim3((unsigned)g), 256, 0, st, 1, static_cast<const T *>(src), ld, rows, cols, static_cast<uint16_t *>(dst), ldp,
-                       rows * ldp);
-}
-
 template <typename T> static int pack_operands(const Problem &p, const Plan &q, char *scratch, Operands *o, cudaStream_t st) {
     const int64_t w_rows = p.class_major ? p.V : p.d, w_cols = p.class_major ? p.d : p.V;
     o->x = View{q.pack_x ? scratch + q.x : p.x, p.n, p.d, q.ldx, p.n * q.ldx, q.planes};
     o->w = View{q.pack_w ? scratch + q.w : p.w, w_rows, w_cols, q.ldw, w_rows * q.ldw, q.planes};
     o->dtype = p.dtype == GRWS_F16 ? GRWS_F16 : GRWS_BF16;
-    if (q.pack_x) if (int rc = launch_pack<T>(p.x, p.ldx, p.n, p.d, scratch + q.x, q.ldx, st)) return rc;
-    if (q.pack_w) if (int rc = launch_pack<T>(p.w, p.ldw, w_rows, w_cols, scratch + q.w, q.ldw, st)) return rc;
-    return GRWS_OK;
+    PackTask a = {}, b = {};
+    if (q.pack_x) a = PackTask{p.x, reinterpret_cast<uint16_t *>(scratch + q.x), p.ldx, p.n, p.d, q.ldx};
+    if (q.pack_w) b = PackTask{p.w, reinterpret_cast<uint16_t *>(scratch + q.w), p.ldw, w_rows, w_cols, q.ldw};
+    const int64_t blocks = ceil_div(a.rows * (a.ldp / 8) + b.rows * (b.ldp / 8), (int64_t)256), most = (int64_t)sm_count() * 8;
+    if (blocks == 0) return GRWS_OK;
+    return launch_next(pack_kernel<T>, dim3((unsigned)(blocks < most ? blocks : most)), 256, 0, st, 1, a, b);
 }
 
 // sets a product up: its tile counts and the maps of its operands; `outer`: the operand's rows are the inner axis
@@ -569,10 +567,10 @@ static int set_task(prod::Task *t, CUtensorMap *ma, CUtensorMap *mb, int cg, int
 }
 
 // where a SUM task's results go: planes of fp32 sums, or the rounded output
-static int set_sums(prod::Task *t, CUtensorMap *mc, int planes, int64_t parts, float *sum, int64_t ld, bool add) {
+static int set_sums(prod::Task *t, CUtensorMap *mc, int64_t parts, float *sum, int64_t ld, bool add) {
     t->splits = (int)parts;
     t->add = add;
-    return prod::encode_map(mc, sum, GRWS_F32, t->N, t->M, ld, (int)parts, t->M * ld, planes == 3 ? 16 : 32, 32);
+    return prod::encode_map(mc, sum, GRWS_F32, t->N, t->M, ld, (int)parts, t->M * ld, 32, 32);
 }
 static int set_rounded(prod::Task *t, CUtensorMap *mc, int dtype, void *out, int64_t ldo) {
     t->rounded = 1;
@@ -581,7 +579,7 @@ static int set_rounded(prod::Task *t, CUtensorMap *mc, int dtype, void *out, int
         t->ldo = ldo;
         return GRWS_OK;
     }
-    return prod::encode_map(mc, out, dtype, t->N, t->M, ldo, 1, 0, dtype == GRWS_F32 ? 16 : 64, 32);
+    return prod::encode_map(mc, out, dtype, t->N, t->M, ldo, 1, 0, dtype == GRWS_F32 ? 32 : 64, 32);
 }
 
 static int status_word(int **word) {
@@ -650,7 +648,7 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
         prod::Maps maps;
         const int cg = cta_group(p.n);
         if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, o.dtype, o.x, 0, o.w, !p.class_major, p.n, cols, p.d)) return rc;
-        if (int rc = prod::encode_map(&maps.c[0], G.p, o.dtype, cols, p.n, q.ldg, q.planes, G.plane, q.planes == 3 ? 16 : 64, 32)) return rc;
+        if (int rc = prod::encode_map(&maps.c[0], G.p, o.dtype, cols, p.n, q.ldg, q.planes, G.plane, q.planes == 3 ? 32 : 64, 32)) return rc;
         int64_t run, runs;
         cut_runs(p.n, r.task[0].m_tiles, r.task[0].n_tiles, r.task[0].k_blocks * step_cost(q.planes), sm_count() / cg, false, &run, &runs);
         r.task[0].run = (int)run;
@@ -679,13 +677,13 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
                                    : set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, o.x, 1, G, 1, M, N, p.n);
                 if (rc != GRWS_OK) return rc;
                 t->k_len = (int)q.dw_len;
-                rc = sum_dw ? set_sums(t, &maps.c[i], q.planes, q.dw_parts, dw_sum, q.ld_dw, false) : set_rounded(t, &maps.c[i], p.dtype, dw_out, ldo);
+                rc = sum_dw ? set_sums(t, &maps.c[i], q.dw_parts, dw_sum, q.ld_dw, false) : set_rounded(t, &maps.c[i], p.dtype, dw_out, ldo);
             } else {
                 rc = set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, G, 0, o.w, p.class_major, p.n, p.d, cols);
                 if (rc != GRWS_OK) return rc;
                 t->b_k0 = (int)v0;
                 t->k_len = (int)q.dx_len;
-                rc = sum_dx ? set_sums(t, &maps.c[i], q.planes, ceil_div((int64_t)t->k_blocks, q.dx_len), dx_sum, q.ld_dx, v0 > 0)      // (a last, shorter piece: fewer)
+                rc = sum_dx ? set_sums(t, &maps.c[i], ceil_div((int64_t)t->k_blocks, q.dx_len), dx_sum, q.ld_dx, v0 > 0)      // (a last, shorter piece: fewer)
                             : set_rounded(t, &maps.c[i], p.dtype, dx, p.d);
             }
             if (rc != GRWS_OK) return rc;
