@@ -52,17 +52,18 @@ __global__ void __launch_bounds__(1024) grad_norm_kernel(const float *__restrict
     }
 }
 
-// Joins the parts of the rows' statistics and takes the rows' losses: 32 rows a block, 8 threads a row, in a fixed order.  The
-// block that is done last adds the blocks' sums up; `done` was set to 0 by the kernel before.
-constexpr int ROWS_PER_BLOCK = 32;
-__global__ void __launch_bounds__(256) rows_kernel(const Problem p, const float2 *__restrict__ part, int parts, const float *__restrict__ label_score,
-                                                   float2 *__restrict__ state, float *__restrict__ loss, float *__restrict__ count,
-                                                   float2 *__restrict__ partial, int *__restrict__ done) {
+// Joins the parts of the rows' statistics and takes the rows' losses: GROUPS threads a row, in a fixed order.  The block that is
+// done last adds the blocks' sums up; `done` was set to 0 by the kernel before.
+template <int GROUPS> __global__ void __launch_bounds__(256) rows_kernel(const Problem p, const float2 *__restrict__ part, int parts,
+                                                                         const float *__restrict__ label_score, float2 *__restrict__ state,
+                                                                         float *__restrict__ loss, float *__restrict__ count, float2 *__restrict__ partial,
+                                                                         int *__restrict__ done) {
+    constexpr int ROWS = 256 / GROUPS;
     __shared__ float red[64];
-    __shared__ float2 joined[8][ROWS_PER_BLOCK];
+    __shared__ float2 joined[GROUPS][ROWS];
     __shared__ bool last;
-    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
-    const int64_t row = (int64_t)blockIdx.x * ROWS_PER_BLOCK + lane;
+    const int at = threadIdx.x % ROWS, group = threadIdx.x / ROWS;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + at;
     float l = 0.0f, counted = 0.0f, m = NEG_INF, s = 0.0f, score = 0.0f;
     int64_t label = -1;
     wait_for_previous();
@@ -72,16 +73,20 @@ __global__ void __launch_bounds__(256) rows_kernel(const Problem p, const float2
             score = label_score[row];          // (nothing was written there for a label that is no class)
         }
 #pragma unroll 4
-        for (int i = group; i < parts; i += 8) {
+        for (int i = group; i < parts; i += GROUPS) {
             const float2 q = part[(int64_t)i * p.n + row];
             join_stats(m, s, q.x, q.y, LOG2E);
         }
     }
-    joined[group][lane] = make_float2(m, s);
-    __syncthreads();
-    if (group == 0 && row < p.n) {
+    if constexpr (GROUPS > 1) {
+        joined[group][at] = make_float2(m, s);
+        __syncthreads();
+        if (group == 0) {
 #pragma unroll
-        for (int i = 1; i < 8; ++i) join_stats(m, s, joined[i][lane].x, joined[i][lane].y, LOG2E);
+            for (int i = 1; i < GROUPS; ++i) join_stats(m, s, joined[i][at].x, joined[i][at].y, LOG2E);
+        }
+    }
+    if (group == 0 && row < p.n) {
         state[row] = make_float2(m, s);
         if (label != p.ignore_index) {
             l = label >= 0 && label < p.V ? logf(s) - (score - m) : NAN;
@@ -90,14 +95,11 @@ __global__ void __launch_bounds__(256) rows_kernel(const Problem p, const float2
         if (p.reduction == RED_NONE) loss[row] = l;
     }
     if (p.reduction == RED_NONE) return;
-    if (group == 0) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) { l += __shfl_xor_sync(0xffffffffu, l, o); counted += __shfl_xor_sync(0xffffffffu, counted, o); }
-        if (lane == 0) {
-            partial[blockIdx.x] = make_float2(l, counted);
-            __threadfence();
-            last = atomicAdd(done, 1) == (int)gridDim.x - 1;
-        }
+    block_sum2(l, counted, red);
+    if (threadIdx.x == 0) {
+        partial[blockIdx.x] = make_float2(l, counted);
+        __threadfence();
+        last = atomicAdd(done, 1) == (int)gridDim.x - 1;
     }
     __syncthreads();
     if (!last) return;
@@ -107,6 +109,8 @@ __global__ void __launch_bounds__(256) rows_kernel(const Problem p, const float2
     block_sum2(l, counted, red);
     if (threadIdx.x == 0) finish_loss(l, counted, p.reduction, loss, count);
 }
+// eight threads a row where there are parts for them
+static int rows_per_block(int64_t parts) { return parts > 4 ? 32 : 256; }
 
 // ---------------------------------------------------------------------------------------------
 // Small fp32 calls, in fp32 arithmetic on the general cores: 64 x 64 tiles, 16 deep, 4 x 4 a thread.
@@ -360,7 +364,7 @@ static size_t place(size_t &at, size_t bytes) {
 }
 static void place_rows(size_t &at, int64_t n, Plan *q) {
     q->label_score = place(at, (size_t)n * sizeof(float));
-    q->partial = place(at, (size_t)ceil_div(n, (int64_t)ROWS_PER_BLOCK) * sizeof(float2));
+    q->partial = place(at, (size_t)ceil_div(n, (int64_t)rows_per_block(q->parts)) * sizeof(float2));
     q->done = place(at, sizeof(int));
 }
 // parts of an inner axis of K so that `tiles` output tiles give every SM two blocks; none shorter than `least`
@@ -707,8 +711,9 @@ template <typename T> static int forward(const Problem &p, const Plan &q, float 
     if (int rc = q.tensor ? tensor_forward<T>(p, q, part, label_score, done, scratch, st)
                           : launch_next(plain_stats_kernel, dim3((unsigned)ceil_div(p.n, (int64_t)TM), (unsigned)q.parts), 256, 0, st, 1, p, part, label_score, done))
         return rc;
-    return launch_next(rows_kernel, dim3((unsigned)ceil_div(p.n, (int64_t)ROWS_PER_BLOCK)), 256, 0, st, 1, p, part, (int)(q.tensor ? 2 * q.parts : q.parts),
-                       label_score, state, loss, count, partial, done);
+    const int rows = rows_per_block(q.parts);
+    return launch_next(rows == 32 ? rows_kernel<8> : rows_kernel<1>, dim3((unsigned)ceil_div(p.n, (int64_t)rows)), 256, 0, st, 1, p, part,
+                       (int)(q.tensor ? 2 * q.parts : q.parts), label_score, state, loss, count, partial, done);
 }
 
 static int plain_backward(const Problem &p, const Plan &q, float *dx, float *dw, char *scratch, cudaStream_t st) {
