@@ -1,7 +1,6 @@
 """Losses over the class axis on the library's kernels (csrc/linear_ce.cu, csrc/distill.cu): softmax cross entropy of a
 linear classifier that never keeps its scores, and distillation from a teacher's best scores.  The reference's steps take
 F.cross_entropy of the last layer's output (helper/engine.py:66-75)."""
-import contextlib
 import functools
 
 import torch
@@ -14,7 +13,6 @@ from ..core import _DT, _ptr, _scratch, _stream
 _REDUCTIONS = {'none': _native.REDUCE_NONE, 'mean': _native.REDUCE_MEAN, 'sum': _native.REDUCE_SUM}
 _INDEX_BYTES = {torch.int64: 8, torch.int32: 4}
 MAX_KEPT = 1024
-_HERE = contextlib.nullcontext()
 
 
 def _reduction(name):
@@ -48,9 +46,12 @@ def _stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _on(device):
-    """Context in which ``device`` is the current device (a guard costs time: none where it is already)."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _on(device, call):
+    """``call()`` with ``device`` as the current device (a guard costs time: none where it is already)."""
+    if torch.cuda.current_device() == device.index:
+        return call()
+    with torch.cuda.device(device):
+        return call()
 
 
 def _outputs(rows, per_row, reduction, device):
@@ -65,48 +66,53 @@ def _ce_scratch_bytes(device_index, *args):
     return _native.lib().grws_linear_ce_scratch_bytes(*args)
 
 
-def _ce_scratch(x, w, class_major, n, d, V, backward):
-    # where an operand starts matters to 16 bytes only
-    return _scratch(_ce_scratch_bytes(x.device.index, 16 + _ptr(x) % 16, _stride(x), 16 + _ptr(w) % 16, _stride(w), class_major, n, d, V,
-                                      _DT[x.dtype], backward), x.device)
+def _ce_operands(x, w, class_major, V):
+    """Leading arguments of the C calls, and the arguments that the size of their scratch depends on (where an operand
+    starts matters to 16 bytes only)."""
+    xp, wp, ldx, ldw = x.data_ptr(), w.data_ptr(), _stride(x), _stride(w)
+    n, d = x.shape
+    return (xp, ldx, wp, ldw, class_major), (x.device.index, 16 + xp % 16, ldx, 16 + wp % 16, ldw, class_major, n, d, V, _DT[x.dtype])
 
 
 class _LinearCrossEntropyFunction(Function):
     @staticmethod
     def forward(ctx, x, weight, labels, ignore_index, reduction):
-        lib = _native.lib()
         x, labels = _rows_of(x), labels.contiguous()
-        class_major = weight.stride(1) != 1 and weight.stride(0) == 1
+        class_major = int(weight.stride(1) != 1 and weight.stride(0) == 1)
         w = _rows_of(weight.t() if class_major else weight)
         (n, d), V = x.shape, weight.shape[1]
         loss, state = _outputs(n, 2, reduction, x.device)
-        count = state.data_ptr() + 8 * n
-        args = (_ptr(x), _stride(x), _ptr(w), _stride(w), int(class_major))
-        with _on(x.device):
-            scratch = _ce_scratch(x, w, int(class_major), n, d, V, 0)
-            _native.check(lib.grws_linear_ce_fwd(*args, _ptr(labels), _INDEX_BYTES[labels.dtype], ignore_index, n, d, V, _DT[x.dtype],
-                                                 reduction, loss.data_ptr(), state.data_ptr(), count, scratch.data_ptr(),
-                                                 scratch.numel(), _stream(x.device)))
+
+        def call():
+            operands, key = _ce_operands(x, w, class_major, V)
+            scratch = _scratch(_ce_scratch_bytes(*key, 0), x.device)
+            sp = state.data_ptr()
+            return _native.lib().grws_linear_ce_fwd(*operands, labels.data_ptr(), _INDEX_BYTES[labels.dtype], ignore_index, n, d, V, _DT[x.dtype],
+                                                    reduction, loss.data_ptr(), sp, sp + 8 * n, scratch.data_ptr(), scratch.numel(),
+                                                    _stream(x.device))
+        _native.check(_on(x.device, call))
         ctx.save_for_backward(x, w, labels, state)
-        ctx.args = (ignore_index, reduction, class_major)
+        ctx.args = (ignore_index, reduction, class_major, V)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_loss):
-        lib = _native.lib()
         x, w, labels, state = ctx.saved_tensors
-        ignore_index, reduction, class_major = ctx.args
-        (n, d), V = x.shape, w.shape[0] if class_major else w.shape[1]
+        ignore_index, reduction, class_major, V = ctx.args
+        n, d = x.shape
         grad_loss = grad_loss.contiguous()
         dx = torch.empty((n, d), dtype=x.dtype, device=x.device) if ctx.needs_input_grad[0] else None
         dw = torch.empty(w.shape, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[1] else None
-        args = (_ptr(x), _stride(x), _ptr(w), _stride(w), int(class_major))
-        with _on(x.device):
-            scratch = _ce_scratch(x, w, int(class_major), n, d, V, 1)
-            _native.check(lib.grws_linear_ce_bwd(*args, _ptr(labels), _INDEX_BYTES[labels.dtype], ignore_index, n, d, V, _DT[x.dtype],
-                                                 reduction, _ptr(grad_loss), state.data_ptr(), state.data_ptr() + 8 * n, _ptr(dx),
-                                                 _ptr(dw), scratch.data_ptr(), scratch.numel(), _stream(x.device)))
+
+        def call():
+            operands, key = _ce_operands(x, w, class_major, V)
+            scratch = _scratch(_ce_scratch_bytes(*key, 1), x.device)
+            sp = state.data_ptr()
+            return _native.lib().grws_linear_ce_bwd(*operands, labels.data_ptr(), _INDEX_BYTES[labels.dtype], ignore_index, n, d, V, _DT[x.dtype],
+                                                    reduction, grad_loss.data_ptr(), sp, sp + 8 * n, _ptr(dx), _ptr(dw), scratch.data_ptr(),
+                                                    scratch.numel(), _stream(x.device))
+        _native.check(_on(x.device, call))
         return dx, dw.t() if class_major and dw is not None else dw, None, None, None
 
 
@@ -145,16 +151,18 @@ def _distill_scratch_bytes(device_index, rows, classes):
 class _DistillationFunction(Function):
     @staticmethod
     def forward(ctx, logits, teacher, ids, temperature, reduction):
-        lib = _native.lib()
         logits, teacher, ids = _rows_of(logits), _rows_of(teacher), _rows_of(ids)
         (n, V), K = logits.shape, ids.shape[1]
         loss, state = _outputs(n, 4, reduction, logits.device)
-        with _on(logits.device):
+
+        def call():
             scratch = _scratch(_distill_scratch_bytes(logits.device.index, n, V), logits.device)
-            _native.check(lib.grws_distill_fwd(
-                _ptr(logits), _stride(logits), _DT[logits.dtype], _ptr(teacher), _stride(teacher), _DT[teacher.dtype], _ptr(ids),
-                _stride(ids), _INDEX_BYTES[ids.dtype], n, V, K, temperature, reduction, loss.data_ptr(), state.data_ptr(),
-                state.data_ptr() + 16 * n, scratch.data_ptr(), scratch.numel(), _stream(logits.device)))
+            sp = state.data_ptr()
+            return _native.lib().grws_distill_fwd(
+                logits.data_ptr(), _stride(logits), _DT[logits.dtype], teacher.data_ptr(), _stride(teacher), _DT[teacher.dtype], ids.data_ptr(),
+                _stride(ids), _INDEX_BYTES[ids.dtype], n, V, K, temperature, reduction, loss.data_ptr(), sp, sp + 16 * n, scratch.data_ptr(),
+                scratch.numel(), _stream(logits.device))
+        _native.check(_on(logits.device, call))
         ctx.save_for_backward(logits, teacher, ids, state)
         ctx.args = (temperature, reduction)
         return loss
@@ -162,7 +170,6 @@ class _DistillationFunction(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_loss):
-        lib = _native.lib()
         logits, teacher, ids, state = ctx.saved_tensors
         temperature, reduction = ctx.args
         (n, V), K = logits.shape, ids.shape[1]
@@ -171,12 +178,17 @@ class _DistillationFunction(Function):
         # can be walked in the same 16-byte pieces
         ld = _stride(logits)
         ldo = ld if ld <= V + 16 else -(-V // 8) * 8
-        dlogits = torch.empty((n, ldo), dtype=logits.dtype, device=logits.device)[:, :V]
-        with _on(logits.device):
-            _native.check(lib.grws_distill_bwd(
-                _ptr(logits), ld, _DT[logits.dtype], _ptr(teacher), _stride(teacher), _DT[teacher.dtype], _ptr(ids), _stride(ids),
-                _INDEX_BYTES[ids.dtype], n, V, K, temperature, reduction, _ptr(grad_loss), state.data_ptr(), state.data_ptr() + 16 * n,
-                _ptr(dlogits), ldo, _stream(logits.device)))
+        dlogits = torch.empty((n, ldo), dtype=logits.dtype, device=logits.device)
+        if ldo != V:
+            dlogits = dlogits[:, :V]
+
+        def call():
+            sp = state.data_ptr()
+            return _native.lib().grws_distill_bwd(
+                logits.data_ptr(), ld, _DT[logits.dtype], teacher.data_ptr(), _stride(teacher), _DT[teacher.dtype], ids.data_ptr(), _stride(ids),
+                _INDEX_BYTES[ids.dtype], n, V, K, temperature, reduction, grad_loss.data_ptr(), sp, sp + 16 * n, dlogits.data_ptr(), ldo,
+                _stream(logits.device))
+        _native.check(_on(logits.device, call))
         return dlogits, None, None, None, None
 
 
