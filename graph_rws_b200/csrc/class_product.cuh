@@ -223,6 +223,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
                  : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// what was loaded is used behind this point only: the compiler sees no tie between the wait and the registers
+__device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                      "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                      "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]));
+    asm volatile("" : "+r"(r[30]), "+r"(r[31]));
+}
 
 // shared-memory matrix descriptor, 128-byte swizzle.  Inner axis contiguous: 8-row groups 1,024 bytes apart, a step of 16
 // inner elements is 32 bytes.  Outer axis contiguous: 64-element pieces of it `lbo` apart, groups of 8 inner elements 1,024
@@ -678,6 +685,8 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                         tmem_ld32(at + c, r);
                         tmem_ld32(at + c + 32, r2);
                         tmem_ld_wait();
+                        loaded(r);
+                        loaded(r2);
                         if (k == last) release_sum(ss->acc_empty, tile);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) { v[i] = __uint_as_float(r[i]); v[32 + i] = __uint_as_float(r2[i]); }
@@ -694,6 +703,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                             uint32_t r[W];
                             tmem_ld32(from + c + k * W, r);
                             tmem_ld_wait();
+                            loaded(r);
 #pragma unroll
                             for (int i = 0; i < W; ++i) acc[k][i] = first ? __uint_as_float(r[i]) : acc[k][i] + __uint_as_float(r[i]);
                         }
