@@ -501,9 +501,10 @@ static Plan make_plan(const Problem &p, bool backward) {
         const int pg = cta_group(n > d ? n : d);
         const int64_t k1 = ceil_div(n, (int64_t)prod::BK);
         double best = 1e300;
-        // the largest piece, or one down to half of it whose products leave the SMs more equally busy
+        // all classes at once if they fit; else the largest piece, or one down to half of it whose products leave the SMs more
+        // equally busy
         const int64_t all = ceil_div(V, PIECE_UNIT) * PIECE_UNIT, top = most < all ? most : all;
-        for (int64_t k = 8; k >= 4; --k) {
+        for (int64_t k = 8; k >= (all <= most ? 8 : 4); --k) {
             const int64_t piece = ceil_div(top * k / 8, PIECE_UNIT) * PIECE_UNIT;
             const int64_t c = piece < V ? piece : V;
             const int64_t tiles0 = tiles_of(n, d, pg, q.planes), tiles1 = p.class_major ? tiles_of(c, d, pg, q.planes) : tiles_of(d, c, pg, q.planes);
