@@ -506,7 +506,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
         const uint32_t box = ring + C::STAGES * C::STAGE_BYTES + warp * C::BOX_BYTES;
         uint32_t tile = 0;
         [[maybe_unused]] uint32_t chain = 0;
-        bool ok = true;
+        bool ok = true, some = false;          // some: the warp has rows to store
         // waits for an accumulator's `use`-th sum, and gives it back
         auto wait_sum = [&](uint64_t *full, uint32_t use) {
             ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[use & 1u]), (use >> 1) & 1u, abort_flag, limit));
@@ -533,7 +533,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
         auto box_out = [&](const CUtensorMap *map, int x, int y, int z, bool add) {
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) {
+            if (lane == 0 && some) {
                 if (add) tma_add(map, box, x, y, z); else tma_store(map, box, x, y, z);
                 bulk_commit();
             }
@@ -546,6 +546,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
             const int row0 = (w.m * CG + (int)rank) * BM + quarter * 32;
             const int64_t row = row0 + lane;
             const bool in = row < t.M;
+            some = row0 < t.M;
             [[maybe_unused]] float m = NEG_INF, s = 0.0f, factor = 0.0f, weight = 0.0f;
             [[maybe_unused]] int64_t label = -1;
             if constexpr (MODE != SUM) {
@@ -630,7 +631,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                             }
                             fence_async_smem();
                             __syncwarp();
-                            if (lane == 0) {
+                            if (lane == 0 && some) {
 #pragma unroll
                                 for (int k = 0; k < 3; ++k) tma_store(mc, box + k * 2048, (int)col0 + c, row0, k);
                                 bulk_commit();

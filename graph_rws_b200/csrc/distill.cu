@@ -20,7 +20,7 @@ using namespace cls;
 constexpr int MAX_KEPT = 1024;
 constexpr int THREADS = 256;
 constexpr int CTAS_PER_SM = 8;
-constexpr int SHORT_ROW = 16384;         // classes up to which a group of lanes takes a row (else a CTA), given the rows
+constexpr int SHORT_ROW_BYTES = 32768;   // rows up to which a group of lanes may take one
 constexpr int SHORT_KEPT = 64;           // entries that such a group holds in shared memory
 constexpr int LONG_HELD = 2;             // entries per lane of the warp that takes a long row's loss, loaded ahead
 constexpr int SPLIT_MIN = 4096;          // classes below which a row is not cut any further
@@ -206,7 +206,7 @@ template <typename T, int L, int H> __device__ __forceinline__ float row_loss(co
     return l;
 }
 
-// ---- rows of up to SHORT_ROW classes: L lanes a row, the losses of a block's rows summed ----
+// ---- short rows: L lanes a row, the losses of a block's rows summed ----
 template <typename T, int L, int U, int EDGE, int H> __global__ void __launch_bounds__(THREADS) short_fwd_kernel(const Args a) {
     wait_for_previous();
     let_next_start();
@@ -421,8 +421,14 @@ template <typename T> __global__ void __launch_bounds__(THREADS) long_bwd_kernel
 
 static int64_t grid_limit() { return (int64_t)sm_count() * CTAS_PER_SM; }
 
-// A warp (or less) per row while that gives every SM 16 warps to run: no barrier, no idle warps at a row's end.
-static bool short_rows(int64_t n, int64_t V, int K) { return K <= SHORT_KEPT && (V <= 1024 || (V <= SHORT_ROW && n >= (int64_t)sm_count() * 16)); }
+// A warp (or less) per row, which has no barrier and no idle warps at a row's end, while there are rows enough to fill the SMs
+// with warps; else a CTA per row or part of a row.  Warp against CTA, us forward and backward, bf16: 100,000 x 1,000 191 / 1,008;
+// 1,000 x 2,000 10.7 / 16.7; 500 x 8,000 16.7 / 12.6, 2,000 x 8,000 23 / 27; 1,000 x 16,000 25.5 / 22, 5,000 x 16,000 96 / 106;
+// 20,000 x 32,000 677 / 652.  fp32: 2,000 x 8,000 41 / 41, 20,000 x 8,000 323 / 364; 5,000 x 16,000 194 / 173.
+static bool short_rows(int64_t n, int64_t V, int K, size_t es) {
+    const int64_t bytes = V * (int64_t)es, full = (int64_t)sm_count() * 4;
+    return K <= SHORT_KEPT && (V <= 1024 || (bytes <= SHORT_ROW_BYTES && n >= full && n >= bytes / 16));
+}
 // Parts of a long row: as many as give every SM work, none shorter than SPLIT_MIN classes; part lengths are whole pieces.
 static void split_rows(int64_t n, int64_t V, int *splits, int *part) {
     int64_t s = ceil_div(grid_limit() / 2, n > 0 ? n : 1);
@@ -466,7 +472,7 @@ template <typename T> static int launch_short_rows(const Args &a, bool fwd, int6
 
 template <typename T> static int launch(Args a, bool fwd, float *loss, float *count, cudaStream_t st) {
     int64_t grid = 0;
-    if (short_rows(a.n, a.V, a.K)) {
+    if (short_rows(a.n, a.V, a.K, sizeof(T))) {
         if (int rc = launch_short_rows<T>(a, fwd, &grid, st)) return rc;
     } else {
         split_rows(a.n, a.V, &a.splits, &a.part);
