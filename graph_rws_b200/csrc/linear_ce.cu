@@ -342,6 +342,10 @@ static __device__ int g_status;
 // ---------------------------------------------------------------------------------------------
 constexpr size_t PIECE_BYTES = 512ull << 20;       // workspace for G
 constexpr int64_t PIECE_UNIT = 256;                // its columns come in whole tiles
+// Rows of packed operands and of G are whole lines of 128 bytes: a copy's 128-byte line of another row start touches two lines
+// of L2, and what an SM takes in from L2 bounds the products (5,003 x 301 x 49,999 in fp16: 842 us with rows of whole 16 bytes,
+// 753 with these; 8,192 x 301 x 10,007 in bf16: 273 and 222; 8,192 x 2,048 x 10,007: 1,201 and 1,008)
+constexpr int64_t LINE = 64;
 
 struct Plan {
     bool tensor;
@@ -483,10 +487,13 @@ static Plan make_plan(const Problem &p, bool backward) {
     }
     q.planes = p.dtype == GRWS_F32 ? 3 : 1;
     const int64_t w_rows = p.class_major ? V : d, w_cols = p.class_major ? d : V;
-    q.pack_x = needs_packing(p.x, p.ldx, p.dtype);
+    // x whose rows are no whole lines is packed for many classes, which read it as often (bf16, 8,192 x 1,000 x 50,000: 2,663 us
+    // as it is, 2,430 packed; x 10,000: 479 and 462; 8,192 x 304 x 10,000: 210 and 211; x 1,000: 54 and 58); a copy of w, as
+    // large as what dw writes, costs what it saves (8,192 x 1,000 x 50,000: 2,663 and 2,666; 1,000 rows: 329 and 387)
+    q.pack_x = needs_packing(p.x, p.ldx, p.dtype) || (p.ldx % LINE != 0 && V >= 16384);
     q.pack_w = needs_packing(p.w, p.ldw, p.dtype);
-    q.ldx = q.pack_x ? ceil_div(d, (int64_t)8) * 8 : p.ldx;
-    q.ldw = q.pack_w ? ceil_div(w_cols, (int64_t)8) * 8 : p.ldw;
+    q.ldx = q.pack_x ? ceil_div(d, LINE) * LINE : p.ldx;
+    q.ldw = q.pack_w ? ceil_div(w_cols, LINE) * LINE : p.ldw;
     if (q.pack_x) q.x = place(at, (size_t)q.planes * n * q.ldx * 2);
     if (q.pack_w) q.w = place(at, (size_t)q.planes * w_rows * q.ldw * 2);
     const int cg = cta_group(n);
@@ -513,7 +520,7 @@ static Plan make_plan(const Problem &p, bool backward) {
                                  (c < V ? (double)n * d * 8.0 / 5.0e6 / 0.4 : 0.0)) * (double)ceil_div(V, c);
             if (cost < best) { best = cost; q.piece = c; q.dx_parts = a; q.dw_parts = b; }
         }
-        q.ldg = ceil_div(q.piece, (int64_t)8) * 8;
+        q.ldg = ceil_div(q.piece, LINE) * LINE;
         const int64_t k0 = ceil_div(q.piece, (int64_t)prod::BK);
         q.dx_len = ceil_div(k0, q.dx_parts);
         q.dx_parts = ceil_div(k0, q.dx_len);

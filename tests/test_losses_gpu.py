@@ -114,6 +114,17 @@ def test_cross_entropy_reductions_and_ignored_rows(n, d, V, dtype, reduction):
     check_ce(x, w, y.int(), reduction, g)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("class_major", [False, True])
+@pytest.mark.parametrize("V", [16376, 16384, 16391])
+def test_cross_entropy_rows_that_are_no_whole_lines(V, dtype, class_major):
+    """Rows of 208 bytes (416 in fp32) within wider ones of NaN, on both sides of the number of classes from which they are copied."""
+    x, w, y = ce_inputs(261, 104, V, dtype, class_major)
+    wide = torch.full((261, 120), float("nan"), dtype=dtype, device="cuda")
+    wide[:, 8:112] = x
+    check_ce(wide[:, 8:112], w, y)
+
+
 def test_cross_entropy_against_differences():
     """The gradient of an fp32 loss against central differences in 64 bits along random directions."""
     x, w, y = ce_inputs(33, 20, 50, torch.float32, ignored=0.2)
