@@ -65,9 +65,10 @@ struct Task {
     int b_row0, b_k0;                     // first column / inner element of B within its tensor map
     int64_t M, N;
     // SUM: partial sums [splits][M][] in fp32 (added to what is there if `add`), or the output rounded to the operands' type,
-    // through the map of the outputs; or to `out` with rows of ldo, where these are no multiple of 16 bytes apart
+    // through the map of the outputs; or to `out` with rows of ldo, where these are no multiple of 16 bytes apart or `turned`
     int rounded, add;
     void *out; int64_t ldo;
+    bool turned;                          // `out` takes the transpose
     __host__ __device__ int units() const { return m_tiles * runs * splits; }
 };
 
@@ -642,6 +643,19 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                         for (int i = 0; i < W; ++i) v[i] *= factor;
                         if constexpr (!SPLIT) {
                             if (t.rounded) {
+                                if (t.turned) {
+                                    // straight from the registers: a warp's 32 rows of one column lie side by side in `out`
+                                    if (!in) return;
+                                    uint16_t *o = static_cast<uint16_t *>(t.out) + (col0 + c) * t.ldo + row;
+#pragma unroll
+                                    for (int i = 0; i < W; i += 2, o += 2 * t.ldo) {
+                                        if (c + i >= cols) break;
+                                        const uint32_t two = p.bf16 ? pack2<true>(v[i], v[i + 1]) : pack2<false>(v[i], v[i + 1]);
+                                        o[0] = (uint16_t)two;
+                                        if (c + i + 1 < cols) o[t.ldo] = (uint16_t)(two >> 16);
+                                    }
+                                    return;
+                                }
                                 box_free();
                                 put16(v, ~0u);
                                 if (!t.out) { box_out(mc, (int)col0 + c, row0, 0, false); return; }

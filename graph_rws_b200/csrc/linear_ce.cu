@@ -355,6 +355,7 @@ struct Plan {
     int64_t run, parts;                            // forward: class tiles per unit, parts of the class axis
     int64_t piece;                                 // backward: classes per piece
     int64_t dx_parts, dx_len, dw_parts, dw_len;    // parts of the two products' inner axes (classes of a piece, rows)
+    bool turn_dw;                                  // dw of [d, V] as the transpose of G^T x
     size_t x, w;                                   // packed operands
     size_t stats, label_score, partial, done;      // forward scratch
     size_t norm, G, dx_sum, dw_sum;                // backward scratch
@@ -458,6 +459,16 @@ static bool on_tensor_cores(int64_t n, int64_t d, int64_t V, int dtype) {
     return dtype != GRWS_F32 || (double)n * (double)d * (double)V >= (double)(1 << 21);
 }
 
+// dw of a [d, V] weight is x^T G, whose rows d come in tiles of 128 or 256, or the transpose of G^T x, whose columns d come in
+// 32s, and which leaves the registers as 64-byte pieces of rows.  The latter where it multiplies a quarter less (bf16, the
+// backward pass with the forward one: 5,003 x 301 x 49,999 in 580 us against 619, 30,000 x 100 x 49,999 in 2,358 against 2,609,
+// 8,192 x 320 x 10,000 in 258 against 269; 30,000 x 600 x 49,999, a fifth less, in 6,931 against 6,840).
+static bool turns(const Problem &p, int cg, int planes) {
+    if (p.class_major || planes != 1) return false;
+    const int64_t before = (column_tiles(p.d, planes) - 1) * columns_per_tile(p.d, planes), rows = (int64_t)prod::BM * cg;
+    return 3 * ceil_div(p.d, rows) * rows >= 4 * (before + in_32s(p.d - before));
+}
+
 static Plan make_plan(const Problem &p, bool backward) {
     Plan q = {};
     const int64_t n = p.n, d = p.d, V = p.V;
@@ -507,18 +518,21 @@ static Plan make_plan(const Problem &p, bool backward) {
         if (most < PIECE_UNIT) most = PIECE_UNIT;
         const int pg = cta_group(n > d ? n : d);
         const int64_t k1 = ceil_div(n, (int64_t)prod::BK);
-        double best = 1e300;
         // all classes at once if they fit; else the largest piece, or one down to half of it whose products leave the SMs more
         // equally busy
         const int64_t all = ceil_div(V, PIECE_UNIT) * PIECE_UNIT, top = most < all ? most : all;
-        for (int64_t k = 8; k >= (all <= most ? 8 : 4); --k) {
-            const int64_t piece = ceil_div(top * k / 8, PIECE_UNIT) * PIECE_UNIT;
-            const int64_t c = piece < V ? piece : V;
-            const int64_t tiles0 = tiles_of(n, d, pg, q.planes), tiles1 = p.class_major ? tiles_of(c, d, pg, q.planes) : tiles_of(d, c, pg, q.planes);
-            int64_t a, b;
-            const double cost = (cut_products(tiles0, ceil_div(c, (int64_t)prod::BK), (double)n * d, tiles1, k1, (double)d * c, step_cost(q.planes), sm_count() / pg, &a, &b) +
-                                 (c < V ? (double)n * d * 8.0 / 5.0e6 / 0.4 : 0.0)) * (double)ceil_div(V, c);
-            if (cost < best) { best = cost; q.piece = c; q.dx_parts = a; q.dw_parts = b; }
+        for (q.turn_dw = turns(p, pg, q.planes);; q.turn_dw = false) {
+            double best = 1e300;
+            for (int64_t k = 8; k >= (all <= most ? 8 : 4); --k) {
+                const int64_t piece = ceil_div(top * k / 8, PIECE_UNIT) * PIECE_UNIT;
+                const int64_t c = piece < V ? piece : V;
+                const int64_t tiles0 = tiles_of(n, d, pg, q.planes), tiles1 = p.class_major || q.turn_dw ? tiles_of(c, d, pg, q.planes) : tiles_of(d, c, pg, q.planes);
+                int64_t a, b;
+                const double cost = (cut_products(tiles0, ceil_div(c, (int64_t)prod::BK), (double)n * d, tiles1, k1, (double)d * c, step_cost(q.planes), sm_count() / pg, &a, &b) +
+                                     (c < V ? (double)n * d * 8.0 / 5.0e6 / 0.4 : 0.0)) * (double)ceil_div(V, c);
+                if (cost < best) { best = cost; q.piece = c; q.dx_parts = a; q.dw_parts = b; }
+            }
+            if (!q.turn_dw || q.dw_parts == 1) break;          // (the sums of parts are added up as they lie)
         }
         q.ldg = ceil_div(q.piece, LINE) * LINE;
         const int64_t k0 = ceil_div(q.piece, (int64_t)prod::BK);
@@ -684,12 +698,19 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
             prod::Task *t = &r.task[i];
             int rc;
             if (is_dw) {
-                // [d, V]: x^T G; [V, d]: G^T x
-                rc = p.class_major ? set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, G, 1, o.x, 1, M, N, p.n)
-                                   : set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, o.x, 1, G, 1, M, N, p.n);
+                // [d, V]: x^T G, or the transpose of G^T x; [V, d]: G^T x
+                rc = p.class_major || q.turn_dw ? set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, G, 1, o.x, 1, cols, p.d, p.n)
+                                                : set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, o.x, 1, G, 1, M, N, p.n);
                 if (rc != GRWS_OK) return rc;
                 t->k_len = (int)q.dw_len;
-                rc = sum_dw ? set_sums(t, &maps.c[i], q.dw_parts, dw_sum, q.ld_dw, false) : set_rounded(t, &maps.c[i], p.dtype, dw_out, ldo);
+                if (q.turn_dw) {
+                    t->rounded = 1;
+                    t->turned = true;
+                    t->out = dw_out;
+                    t->ldo = ldo;
+                } else {
+                    rc = sum_dw ? set_sums(t, &maps.c[i], q.dw_parts, dw_sum, q.ld_dw, false) : set_rounded(t, &maps.c[i], p.dtype, dw_out, ldo);
+                }
             } else {
                 rc = set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, G, 0, o.w, p.class_major, p.n, p.d, cols);
                 if (rc != GRWS_OK) return rc;

@@ -146,6 +146,13 @@ def test_cross_entropy_in_pieces_of_the_classes(dtype, class_major):
     check_ce(*ce_inputs(70001, 24, 4501, dtype, class_major, ignored=0.2))
 
 
+@pytest.mark.parametrize("d", [40, 301])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_cross_entropy_narrow_weights_in_pieces(d, dtype):
+    """Gradients of [d, classes] weights whose few rows fill no tile, from several pieces of the classes."""
+    check_ce(*ce_inputs(9001, d, 33001, dtype, ignored=0.1))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_cross_entropy_strides(dtype):
     """Operands cut from wider ones, at odd offsets, and orders that need a copy."""
