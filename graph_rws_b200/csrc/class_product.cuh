@@ -641,21 +641,31 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                     } else {
 #pragma unroll
                         for (int i = 0; i < W; ++i) v[i] *= factor;
+                        if (t.turned) {
+                            // straight from the registers: a warp's 32 rows of one column lie side by side in `out`
+                            if (!in) return;
+                            const int64_t at = (col0 + c) * t.ldo + row;
+                            if constexpr (SPLIT) {
+                                float *o = static_cast<float *>(t.out) + at;
+#pragma unroll
+                                for (int i = 0; i < W; ++i, o += t.ldo) {
+                                    if (c + i >= cols) break;
+                                    *o = v[i];
+                                }
+                            } else {
+                                uint16_t *o = static_cast<uint16_t *>(t.out) + at;
+#pragma unroll
+                                for (int i = 0; i < W; i += 2, o += 2 * t.ldo) {
+                                    if (c + i >= cols) break;
+                                    const uint32_t two = p.bf16 ? pack2<true>(v[i], v[i + 1]) : pack2<false>(v[i], v[i + 1]);
+                                    o[0] = (uint16_t)two;
+                                    if (c + i + 1 < cols) o[t.ldo] = (uint16_t)(two >> 16);
+                                }
+                            }
+                            return;
+                        }
                         if constexpr (!SPLIT) {
                             if (t.rounded) {
-                                if (t.turned) {
-                                    // straight from the registers: a warp's 32 rows of one column lie side by side in `out`
-                                    if (!in) return;
-                                    uint16_t *o = static_cast<uint16_t *>(t.out) + (col0 + c) * t.ldo + row;
-#pragma unroll
-                                    for (int i = 0; i < W; i += 2, o += 2 * t.ldo) {
-                                        if (c + i >= cols) break;
-                                        const uint32_t two = p.bf16 ? pack2<true>(v[i], v[i + 1]) : pack2<false>(v[i], v[i + 1]);
-                                        o[0] = (uint16_t)two;
-                                        if (c + i + 1 < cols) o[t.ldo] = (uint16_t)(two >> 16);
-                                    }
-                                    return;
-                                }
                                 box_free();
                                 put16(v, ~0u);
                                 if (!t.out) { box_out(mc, (int)col0 + c, row0, 0, false); return; }

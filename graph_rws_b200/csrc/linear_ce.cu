@@ -460,11 +460,12 @@ static bool on_tensor_cores(int64_t n, int64_t d, int64_t V, int dtype) {
 }
 
 // dw of a [d, V] weight is x^T G, whose rows d come in tiles of 128 or 256, or the transpose of G^T x, whose columns d come in
-// 32s, and which leaves the registers as 64-byte pieces of rows.  The latter where it multiplies a quarter less (bf16, the
-// backward pass with the forward one: 5,003 x 301 x 49,999 in 580 us against 619, 30,000 x 100 x 49,999 in 2,358 against 2,609,
-// 8,192 x 320 x 10,000 in 258 against 269; 30,000 x 600 x 49,999, a fifth less, in 6,931 against 6,840).
+// 32s, and which leaves the registers as 64-byte pieces of rows (128 of fp32).  The latter where it multiplies a quarter less
+// (forward and backward, bf16: 5,003 x 301 x 49,999 in 580 us against 619, 30,000 x 100 x 49,999 in 2,358 against 2,609, 8,192 x
+// 320 x 10,000 in 258 against 269; fp32: 8,192 x 96 x 49,999 in 2,284 against 2,745; a fifth less, bf16, 30,000 x 600 x 49,999:
+// 6,931 against 6,840).
 static bool turns(const Problem &p, int cg, int planes) {
-    if (p.class_major || planes != 1) return false;
+    if (p.class_major) return false;
     const int64_t before = (column_tiles(p.d, planes) - 1) * columns_per_tile(p.d, planes), rows = (int64_t)prod::BM * cg;
     return 3 * ceil_div(p.d, rows) * rows >= 4 * (before + in_32s(p.d - before));
 }

@@ -154,6 +154,17 @@ def test_cross_entropy_narrow_weights_in_pieces(d, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,d,V", [(700, 96, 11003), (700, 97, 11008), (400, 161, 16391), (3001, 301, 9001)])
+def test_cross_entropy_narrow_weights(n, d, V, dtype):
+    """The same from all classes at once, with odd and even rows, columns behind the last whole 32 and a cut of the weight."""
+    x, w, y = ce_inputs(n, d, V, dtype, ignored=0.1)
+    check_ce(x, w, y)
+    wide = torch.full((d, V + 9), float("nan"), dtype=dtype, device="cuda")
+    wide[:, 3:V + 3] = w
+    check_ce(x, wide[:, 3:V + 3], y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_cross_entropy_strides(dtype):
     """Operands cut from wider ones, at odd offsets, and orders that need a copy."""
     x, w, y = ce_inputs(70, 48, 90, dtype)
