@@ -16,7 +16,7 @@ def _free_port():
 
 
 def _worker(rank, world, port, out):
-    """The product kernel is CUDA-only: the CPU checker takes its place; the layer, its autograd function, the
+    """The product kernel is CUDA-only: the CPU oracle takes its place; the layer, its autograd function, the
     sharded graph and the gathers of both directions are the shipped code."""
     os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
     dist.init_process_group("gloo", rank=rank, world_size=world)
