@@ -183,7 +183,11 @@ template <typename T, int N> __device__ __forceinline__ void add_pieces(float &m
 }
 
 // Kernels of one call follow each other as programmatic dependents: the next one is launched while this one still runs, sets
-// itself up and waits here before it touches memory.  Every kernel waits, so each may rely on all before it.
+// itself up and waits here before it touches memory.  Every kernel waits, so each may rely on all before it.  What lies in
+// memory does change during a kernel's lifetime, then: whatever is read behind the wait is read by ordinary loads.  __ldg and
+// pointers that are const and __restrict__ promise that it does not; such a load may be non-coherent, and may be moved
+// ahead of the wait.  (A call's inputs are no exception: the kernel before the first one may be the last of another call,
+// which lets its dependents start as early.)
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -209,7 +213,7 @@ inline int launch_next(void (*kernel)(P...), dim3 grid, int threads, size_t smem
 
 // The integer at i of an array of 4- or 8-byte integers
 __device__ __forceinline__ int64_t load_index(const void *p, int bytes, int64_t i) {
-    return bytes == 8 ? __ldg(static_cast<const long long *>(p) + i) : (int64_t)__ldg(static_cast<const int *>(p) + i);
+    return bytes == 8 ? (int64_t)static_cast<const long long *>(p)[i] : (int64_t)static_cast<const int *>(p)[i];
 }
 
 // Sum of two values over the block's threads, valid in thread 0; red holds 2 * 32 floats.
@@ -233,7 +237,7 @@ __device__ __forceinline__ void finish_loss(float sum, float count, int reductio
     *loss = reduction == RED_MEAN ? sum / count : sum;       // no counted row: 0 / 0
     *count_out = count;
 }
-static __global__ void __launch_bounds__(512) loss_sum_kernel(const float2 *__restrict__ partial, int n, int reduction,
+static __global__ void __launch_bounds__(512) loss_sum_kernel(const float2 *partial, int n, int reduction,
                                                               float *__restrict__ loss, float *__restrict__ count_out) {
     __shared__ float red[64];
     float a = 0.0f, b = 0.0f;
@@ -245,9 +249,9 @@ static __global__ void __launch_bounds__(512) loss_sum_kernel(const float2 *__re
 
 // Factor of all rows from the gradient of the reduced loss.  Without counted rows nothing has a gradient.
 __device__ __forceinline__ float loss_factor(const float *grad_loss, const float *count, int reduction) {
-    const float g = __ldg(grad_loss);
+    const float g = *grad_loss;
     if (reduction != RED_MEAN) return g;
-    const float n = __ldg(count);
+    const float n = *count;
     return n > 0.0f ? g / n : 0.0f;
 }
 

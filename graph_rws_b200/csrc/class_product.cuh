@@ -311,12 +311,12 @@ template <typename P> __device__ __forceinline__ float grad_row_factor(const P &
     if (label == p.ignore_index) return 0.0f;
     if (label < 0 || label >= p.V) return NAN;
     if (p.reduction != RED_NONE) return 1.0f;
-    const float norm = __ldg(p.norm);
-    return norm > 0.0f ? __ldg(p.grad + row) / norm : __ldg(p.grad + row);
+    const float norm = *p.norm, g = p.grad[row];
+    return norm > 0.0f ? g / norm : g;
 }
 template <typename P> __device__ __forceinline__ float grad_alpha(const P &p) {
     if (p.reduction != RED_NONE) return loss_factor(p.grad, p.count, p.reduction);
-    const float norm = __ldg(p.norm);
+    const float norm = *p.norm;
     return norm > 0.0f ? norm : 1.0f;
 }
 

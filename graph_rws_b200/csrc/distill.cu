@@ -44,7 +44,7 @@ struct Args {
 
 __device__ __forceinline__ float teacher_at(const Args &a, int row, int j) {
     const int64_t i = (int64_t)row * a.ldt + j;
-    if (a.t_dtype == GRWS_F32) return __ldg(static_cast<const float *>(a.t) + i);
+    if (a.t_dtype == GRWS_F32) return static_cast<const float *>(a.t)[i];
     if (a.t_dtype == GRWS_F16) return to_float(static_cast<const __half *>(a.t)[i]);
     return to_float(static_cast<const __nv_bfloat16 *>(a.t)[i]);
 }
@@ -81,7 +81,7 @@ template <typename T, int U> struct Batch { uint4 u[U]; };
 template <typename T, int U> __device__ __forceinline__ void load_batch(Batch<T, U> &b, const uint4 *body, int k, int lanes, int pieces) {
     constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
 #pragma unroll
-    for (int i = 0; i < U; ++i) b.u[i] = k + i * lanes < pieces ? __ldg(body + k + i * lanes) : make_uint4(none, none, none, none);
+    for (int i = 0; i < U; ++i) b.u[i] = k + i * lanes < pieces ? body[k + i * lanes] : make_uint4(none, none, none, none);
 }
 
 // What a lane needs of a row before it can do anything is asked for in one go: its first U pieces, its part of the elements
@@ -244,7 +244,7 @@ template <typename T, int L, int U, int EDGE, int H> __global__ void __launch_bo
 
 __device__ __forceinline__ float row_factor(const Args &a, int row, const float4 &st) {
     if (st.w == 0.0f) return 0.0f;
-    const float g = a.reduction == RED_NONE ? __ldg(a.grad + row) : loss_factor(a.grad, a.count, a.reduction);
+    const float g = a.reduction == RED_NONE ? a.grad[row] : loss_factor(a.grad, a.count, a.reduction);
     return g * a.T;
 }
 

@@ -31,7 +31,7 @@ struct Problem {
 };
 
 // largest finite |gradient| of a row: with it a row's factor is at most 1, whatever the scale of the loss
-__global__ void __launch_bounds__(1024) grad_norm_kernel(const float *__restrict__ grad, int64_t n, float *__restrict__ norm) {
+__global__ void __launch_bounds__(1024) grad_norm_kernel(const float *grad, int64_t n, float *norm) {
     __shared__ float red[32];
     float m = 0.0f;
     wait_for_previous();
@@ -54,8 +54,8 @@ __global__ void __launch_bounds__(1024) grad_norm_kernel(const float *__restrict
 
 // Joins the parts of the rows' statistics and takes the rows' losses: GROUPS threads a row, in a fixed order.  The block that is
 // done last adds the blocks' sums up; `done` was set to 0 by the kernel before.
-template <int GROUPS> __global__ void __launch_bounds__(256) rows_kernel(const Problem p, const float2 *__restrict__ part, int parts,
-                                                                         const float *__restrict__ label_score, float2 *__restrict__ state,
+template <int GROUPS> __global__ void __launch_bounds__(256) rows_kernel(const Problem p, const float2 *part, int parts,
+                                                                         const float *label_score, float2 *__restrict__ state,
                                                                          float *__restrict__ loss, float *__restrict__ count, float2 *__restrict__ partial,
                                                                          int *__restrict__ done) {
     constexpr int ROWS = 256 / GROUPS;
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(256) plain_products_kernel(const Problem p, co
 
 // out(m, n) = alpha * sum of the partial planes [parts][M][ldp] in order, rounded once to the output's type; out(m, n) at
 // m * om + n * on.  Four columns a thread.
-template <typename T> __global__ void __launch_bounds__(256) round_kernel(const Problem p, const float *__restrict__ part, int parts, int64_t M, int64_t N,
+template <typename T> __global__ void __launch_bounds__(256) round_kernel(const Problem p, const float *part, int parts, int64_t M, int64_t N,
                                                                           int64_t ldp, float scale, T *__restrict__ out, int64_t om, int64_t on) {
     wait_for_previous();
     let_next_start();
