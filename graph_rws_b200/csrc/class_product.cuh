@@ -9,7 +9,9 @@
 // fp32 operands come as three bf16 planes (x = hi + mid + lo exactly to 24 bits): six products, hi hi, hi mid, mid hi, mid mid,
 // hi lo, lo hi.  What is left out (mid lo and below) is 2^-24 of a product.  The tensor cores cut every sum off towards zero,
 // so these sums are kept short: the five small pairs have an accumulator of their own, hi hi one for every two steps of the
-// inner axis, and the epilogue adds them up in registers, rounding to nearest.  Tiles have 128 columns, so that two of each
+// inner axis, and the epilogue adds them up in registers, rounding to nearest.  An infinite operand has planes of 0, and so has
+// most of what it is multiplied with: where hi hi is not finite, it is the result, and the small pairs (inf 0) are left
+// out.  Tiles have 128 columns, so that two of each
 // accumulator fit and a thread's 64 sums stay in registers; a stage is one plane of both operands, which all products that
 // need it read from where it lies.
 //
@@ -325,10 +327,12 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b)
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-// v as three bf16 numbers; what is not finite goes into the first alone
+// v as three bf16 numbers: of a value past bf16's largest number (fp32's lowest, as a mask, is one) the first takes that number
+// and the others the rest; what is not finite goes into the first alone
 __device__ __forceinline__ void split3(float v, float &a, float &b, float &c) {
-    a = __bfloat162float(__float2bfloat16_rn(v));
-    const bool fin = fabsf(a) < INFINITY;
+    constexpr float MOST = 3.3895313892515355e38f;          // (2 - 2^-7) 2^127
+    const bool fin = fabsf(v) < INFINITY;
+    a = __bfloat162float(__float2bfloat16_rn(fin ? fminf(fmaxf(v, -MOST), MOST) : v));
     const float r = fin ? v - a : 0.0f;
     b = __bfloat162float(__float2bfloat16_rn(r));
     c = r - b;
@@ -721,7 +725,7 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                     const int k0 = w.split * t.k_len, steps = min(t.k_blocks, k0 + t.k_len) - k0, chains = (steps + SUB_STEPS - 1) / SUB_STEPS;
                     const int c = half * 64;
                     float acc[2][W];
-                    auto add_up = [&](uint32_t from, bool first) {
+                    auto add_up = [&](uint32_t from, bool first, bool small) {
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             if (c + k * W >= cols) break;
@@ -730,19 +734,23 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                             tmem_ld_wait();
                             loaded(r);
 #pragma unroll
-                            for (int i = 0; i < W; ++i) acc[k][i] = first ? __uint_as_float(r[i]) : acc[k][i] + __uint_as_float(r[i]);
+                            for (int i = 0; i < W; ++i) {
+                                const float v = __uint_as_float(r[i]);
+                                if (first) acc[k][i] = v;
+                                else if (!small || fabsf(acc[k][i]) < INFINITY) acc[k][i] += v;
+                            }
                         }
                     };
                     for (int sub = 0; sub < chains; ++sub, ++chain) {
                         wait_sum(ss->big_full, chain);
                         if (!ok) break;
-                        add_up(tmem + 2 * C::BN + (chain & 1u) * C::BN + lanes, sub == 0);
+                        add_up(tmem + 2 * C::BN + (chain & 1u) * C::BN + lanes, sub == 0, false);
                         release_sum(ss->big_empty, chain);
                     }
                     if (!ok) break;
                     wait_sum(ss->acc_full, tile);
                     if (!ok) break;
-                    add_up(at, false);
+                    add_up(at, false, true);
                     release_sum(ss->acc_empty, tile);
 #pragma unroll
                     for (int k = 0; k < 2; ++k)
