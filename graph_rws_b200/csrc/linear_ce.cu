@@ -25,20 +25,20 @@ struct Problem {
     int dtype, reduction;
     const float2 *state;                 // [n]: maximum, sum of exponentials
     const float *grad, *count;           // backward: gradient of the loss, number of counted rows
-    const float *norm;                   // backward without a reduction: largest |gradient| of a row
+    const float *norm;                   // backward without a reduction: largest |gradient| of a row that counts
     __host__ __device__ int64_t w_k() const { return class_major ? 1 : ldw; }
     __host__ __device__ int64_t w_v() const { return class_major ? ldw : 1; }
 };
 
-// largest finite |gradient| of a row: with it a row's factor is at most 1, whatever the scale of the loss
-__global__ void __launch_bounds__(1024) grad_norm_kernel(const float *grad, int64_t n, float *norm) {
+// largest finite |gradient| of a row that is not ignored: with it a row's factor is at most 1, whatever the scale of the loss
+__global__ void __launch_bounds__(1024) grad_norm_kernel(const Problem p, float *norm) {
     __shared__ float red[32];
     float m = 0.0f;
     wait_for_previous();
     let_next_start();
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
-        const float g = fabsf(grad[i]);
-        if (g < INFINITY) m = fmaxf(m, g);
+    for (int64_t i = threadIdx.x; i < p.n; i += blockDim.x) {
+        const float g = fabsf(p.grad[i]);
+        if (g < INFINITY && load_index(p.labels, p.label_bytes, i) != p.ignore_index) m = fmaxf(m, g);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -774,7 +774,7 @@ static int plain_backward(const Problem &p, const Plan &q, float *dx, float *dw,
 template <typename T> static int backward(Problem p, const Plan &q, void *dx, void *dw, char *scratch, cudaStream_t st) {
     if (p.reduction == RED_NONE) {
         float *norm = reinterpret_cast<float *>(scratch + q.norm);
-        if (int rc = launch_next(grad_norm_kernel, dim3(1), 1024, 0, st, 1, p.grad, p.n, norm)) return rc;
+        if (int rc = launch_next(grad_norm_kernel, dim3(1), 1024, 0, st, 1, p, norm)) return rc;
         p.norm = norm;
     }
     return q.tensor ? tensor_backward<T>(p, q, dx, dw, scratch, st) : plain_backward(p, q, static_cast<float *>(dx), static_cast<float *>(dw), scratch, st);
