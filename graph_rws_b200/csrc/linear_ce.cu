@@ -293,15 +293,15 @@ template <typename T> __global__ void __launch_bounds__(256) round_kernel(const 
     }
 }
 
-// Operands for the tensor cores from those whose rows no TMA copy can start at (or of fp32: three bf16 planes): rows of `ldp`
+// Operands for the tensor cores from those whose rows no TMA copy can start at (or as three bf16 planes): rows of `ldp`
 // elements, a multiple of 8.  A thread per 8 elements, both operands in one launch.
 struct PackTask { const void *src; uint16_t *dst; int64_t ld, rows, cols, ldp; };
 
-template <typename T> __device__ __forceinline__ void pack8(const PackTask &t, int64_t i) {
+template <typename T, int PLANES> __device__ __forceinline__ void pack8(const PackTask &t, int64_t i) {
     const int64_t per_row = t.ldp / 8, row = i / per_row, c = (i - row * per_row) * 8, plane = t.rows * t.ldp;
     const T *s = static_cast<const T *>(t.src) + row * t.ld + c;
     uint16_t *d = t.dst + row * t.ldp + c;
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (PLANES == 1) {
         uint32_t q[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -325,12 +325,12 @@ template <typename T> __device__ __forceinline__ void pack8(const PackTask &t, i
         for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4 *>(d + k * plane) = make_uint4(q[k][0], q[k][1], q[k][2], q[k][3]);
     }
 }
-template <typename T> __global__ void __launch_bounds__(256) pack_kernel(const PackTask a, const PackTask b) {
+template <typename T, int PLANES> __global__ void __launch_bounds__(256) pack_kernel(const PackTask a, const PackTask b) {
     const int64_t first = a.rows * (a.ldp / 8), total = first + b.rows * (b.ldp / 8);
     wait_for_previous();
     let_next_start();
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        if (i < first) pack8<T>(a, i); else pack8<T>(b, i - first);
+        if (i < first) pack8<T, PLANES>(a, i); else pack8<T, PLANES>(b, i - first);
     }
 }
 
@@ -349,12 +349,13 @@ constexpr int64_t LINE = 64;
 
 struct Plan {
     bool tensor;
-    int planes;                                    // of an operand: 1, or 3 of bf16 for fp32
+    int planes;                                    // of an operand: 1, or 3 of bf16 (see planes_of)
     bool pack_x, pack_w;
     int64_t ldx, ldw, ldg, ld_dx, ld_dw;           // rows of the operands as the tensor cores read them, of fp32 sums
     int64_t run, parts;                            // forward: class tiles per unit, parts of the class axis
     int64_t piece;                                 // backward: classes per piece
     int64_t dx_parts, dx_len, dw_parts, dw_len;    // parts of the two products' inner axes (classes of a piece, rows)
+    bool sum_dx, sum_dw;                           // through planes of fp32 sums, even of one part
     bool turn_dw;                                  // dw of [d, V] as the transpose of G^T x
     size_t x, w;                                   // packed operands
     size_t stats, label_score, partial, done;      // forward scratch
@@ -394,7 +395,16 @@ static int64_t step_cost(int planes) { return planes == 3 ? 3 : 1; }
 // CTAs that share a tile: pairs where there are more rows than one CTA's
 static int cta_group(int64_t M) { return M > prod::BM ? 2 : 1; }
 
-static bool needs_packing(const void *p, int64_t ld, int dtype) { return dtype == GRWS_F32 || !aligned16(p) || ld % 8 != 0; }
+static bool needs_packing(const void *p, int64_t ld, int planes) { return planes == 3 || !aligned16(p) || ld % 8 != 0; }
+
+// fp32 operands are three bf16 planes.  So are fp16 ones (exactly), and with them G, in the backward pass of rows' losses
+// without a reduction: rows' gradients may be decades apart, dw needs one scale for all rows, and a row's softmax, some 2^-16
+// of its gradient where classes are many, would leave fp16's range from 10^-5 of the largest gradient on.  That is six
+// products for one and up to two launches more: forward and backward of 1,024 x 512 x 32,768 497 us against 156 of the mean, 5,003
+// x 301 x 49,999 2,914 against 647; 140 x 32 x 7 160 against 155.
+static int planes_of(const Problem &p, bool backward) {
+    return p.dtype == GRWS_F32 || (p.dtype == GRWS_F16 && backward && p.reduction == RED_NONE) ? 3 : 1;
+}
 
 // Class tiles that one unit of the scores takes: as many as leave the SMs equally busy.  A tile step takes about 0.4 us; a unit
 // costs the latency of its rows' data (0.8 us) and, forward, a statistic per row (of two warps each) written and read at some
@@ -497,13 +507,13 @@ static Plan make_plan(const Problem &p, bool backward) {
         q.bytes = at;
         return q;
     }
-    q.planes = p.dtype == GRWS_F32 ? 3 : 1;
+    q.planes = planes_of(p, backward);
     const int64_t w_rows = p.class_major ? V : d, w_cols = p.class_major ? d : V;
     // x whose rows are no whole lines is packed for many classes, which read it as often (bf16, 8,192 x 1,000 x 50,000: 2,663 us
     // as it is, 2,430 packed; x 10,000: 479 and 462; 8,192 x 304 x 10,000: 210 and 211; x 1,000: 54 and 58); a copy of w, as
     // large as what dw writes, costs what it saves (8,192 x 1,000 x 50,000: 2,663 and 2,666; 1,000 rows: 329 and 387)
-    q.pack_x = needs_packing(p.x, p.ldx, p.dtype) || (p.ldx % LINE != 0 && V >= 16384);
-    q.pack_w = needs_packing(p.w, p.ldw, p.dtype);
+    q.pack_x = needs_packing(p.x, p.ldx, q.planes) || (p.ldx % LINE != 0 && V >= 16384);
+    q.pack_w = needs_packing(p.w, p.ldw, q.planes);
     q.ldx = q.pack_x ? ceil_div(d, LINE) * LINE : p.ldx;
     q.ldw = q.pack_w ? ceil_div(w_cols, LINE) * LINE : p.ldw;
     if (q.pack_x) q.x = place(at, (size_t)q.planes * n * q.ldx * 2);
@@ -522,7 +532,8 @@ static Plan make_plan(const Problem &p, bool backward) {
         // all classes at once if they fit; else the largest piece, or one down to half of it whose products leave the SMs more
         // equally busy
         const int64_t all = ceil_div(V, PIECE_UNIT) * PIECE_UNIT, top = most < all ? most : all;
-        for (q.turn_dw = turns(p, pg, q.planes);; q.turn_dw = false) {
+        const bool summed = q.planes == 3 && p.dtype != GRWS_F32;          // (the kernel rounds to the type of its operands or to fp32)
+        for (q.turn_dw = !summed && turns(p, pg, q.planes);; q.turn_dw = false) {
             double best = 1e300;
             for (int64_t k = 8; k >= (all <= most ? 8 : 4); --k) {
                 const int64_t piece = ceil_div(top * k / 8, PIECE_UNIT) * PIECE_UNIT;
@@ -545,8 +556,10 @@ static Plan make_plan(const Problem &p, bool backward) {
         q.ld_dw = ceil_div(p.class_major ? d : q.piece, (int64_t)4) * 4;
         q.norm = place(at, sizeof(float));
         q.G = place(at, (size_t)q.planes * n * q.ldg * 2);
-        if (q.dx_parts > 1 || q.piece < V) q.dx_sum = place(at, (size_t)q.dx_parts * n * q.ld_dx * sizeof(float));
-        if (q.dw_parts > 1) q.dw_sum = place(at, (size_t)q.dw_parts * (p.class_major ? q.piece : d) * q.ld_dw * sizeof(float));
+        q.sum_dx = summed || q.dx_parts > 1 || q.piece < V;
+        q.sum_dw = summed || q.dw_parts > 1;
+        if (q.sum_dx) q.dx_sum = place(at, (size_t)q.dx_parts * n * q.ld_dx * sizeof(float));
+        if (q.sum_dw) q.dw_sum = place(at, (size_t)q.dw_parts * (p.class_major ? q.piece : d) * q.ld_dw * sizeof(float));
     }
     q.bytes = at;
     return q;
@@ -569,13 +582,15 @@ template <typename T> static int pack_operands(const Problem &p, const Plan &q, 
     const int64_t w_rows = p.class_major ? p.V : p.d, w_cols = p.class_major ? p.d : p.V;
     o->x = View{q.pack_x ? scratch + q.x : p.x, p.n, p.d, q.ldx, p.n * q.ldx, q.planes};
     o->w = View{q.pack_w ? scratch + q.w : p.w, w_rows, w_cols, q.ldw, w_rows * q.ldw, q.planes};
-    o->dtype = p.dtype == GRWS_F16 ? GRWS_F16 : GRWS_BF16;
+    o->dtype = q.planes == 1 && p.dtype == GRWS_F16 ? GRWS_F16 : GRWS_BF16;
     PackTask a = {}, b = {};
     if (q.pack_x) a = PackTask{p.x, reinterpret_cast<uint16_t *>(scratch + q.x), p.ldx, p.n, p.d, q.ldx};
     if (q.pack_w) b = PackTask{p.w, reinterpret_cast<uint16_t *>(scratch + q.w), p.ldw, w_rows, w_cols, q.ldw};
     const int64_t blocks = ceil_div(a.rows * (a.ldp / 8) + b.rows * (b.ldp / 8), (int64_t)256), most = (int64_t)sm_count() * 8;
     if (blocks == 0) return GRWS_OK;
-    return launch_next(pack_kernel<T>, dim3((unsigned)(blocks < most ? blocks : most)), 256, 0, st, 1, a, b);
+    void (*kernel)(const PackTask, const PackTask) = pack_kernel<T, sizeof(T) == 4 ? 3 : 1>;
+    if constexpr (std::is_same<T, __half>::value) if (q.planes == 3) kernel = pack_kernel<T, 3>;
+    return launch_next(kernel, dim3((unsigned)(blocks < most ? blocks : most)), 256, 0, st, 1, a, b);
 }
 
 // sets a product up: its tile counts and the maps of its operands; `outer`: the operand's rows are the inner axis
@@ -623,12 +638,12 @@ static int status_word(int **word) {
     return GRWS_OK;
 }
 
-static int product_params(const Problem &p, prod::Params *r) {
+static int product_params(const Problem &p, int dtype, prod::Params *r) {
     int *status = nullptr;
     if (int rc = status_word(&status)) return rc;
     *r = prod::Params{};
     r->tasks = 1;
-    r->bf16 = p.dtype != GRWS_F16;
+    r->bf16 = dtype != GRWS_F16;
     r->labels = p.labels; r->label_bytes = p.label_bytes; r->ignore_index = p.ignore_index; r->V = p.V;
     r->reduction = p.reduction; r->grad = p.grad; r->count = p.count; r->norm = p.norm;
     r->state = p.state;
@@ -647,7 +662,7 @@ template <typename T> static int tensor_forward(const Problem &p, const Plan &q,
     Operands o;
     if (int rc = pack_operands<T>(p, q, scratch, &o, st)) return rc;
     prod::Params r;
-    if (int rc = product_params(p, &r)) return rc;
+    if (int rc = product_params(p, o.dtype, &r)) return rc;
     prod::Maps maps;
     const int cg = cta_group(p.n);
     if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, o.dtype, o.x, 0, o.w, !p.class_major, p.n, p.V, p.d)) return rc;
@@ -660,18 +675,17 @@ template <typename T> static int tensor_forward(const Problem &p, const Plan &q,
 }
 
 // G in fp16 is held as 2^12 G: |G| <= 1, and a probability of 2^-26 is still a normal number
-static float stored_scale(const Problem &p) { return p.dtype == GRWS_F16 ? 4096.0f : 1.0f; }
+static float stored_scale(const Operands &o) { return o.dtype == GRWS_F16 ? 4096.0f : 1.0f; }
 
 template <typename T> static int tensor_backward(const Problem &p, const Plan &q, void *dx, void *dw, char *scratch, cudaStream_t st) {
     Operands o;
     if (int rc = pack_operands<T>(p, q, scratch, &o, st)) return rc;
     float *dx_sum = reinterpret_cast<float *>(scratch + q.dx_sum), *dw_sum = reinterpret_cast<float *>(scratch + q.dw_sum);
-    const bool sum_dx = q.dx_parts > 1 || q.piece < p.V, sum_dw = q.dw_parts > 1;
     for (int64_t v0 = 0; v0 < p.V; v0 += q.piece) {
         const int64_t cols = p.V - v0 < q.piece ? p.V - v0 : q.piece;
         const View G = {scratch + q.G, p.n, cols, q.ldg, p.n * q.ldg, q.planes};
         prod::Params r;
-        if (int rc = product_params(p, &r)) return rc;
+        if (int rc = product_params(p, o.dtype, &r)) return rc;
         prod::Maps maps;
         const int cg = cta_group(p.n);
         if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, o.dtype, o.x, 0, o.w, !p.class_major, p.n, cols, p.d)) return rc;
@@ -682,11 +696,11 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
         r.task[0].runs = (int)runs;
         r.task[0].b_row0 = (int)v0;
         r.v0 = v0;
-        r.scale = stored_scale(p);
+        r.scale = stored_scale(o);
         if (int rc = launch_product<prod::GRAD>(cg, q.planes, maps, r, st)) return rc;
 
-        if (int rc = product_params(p, &r)) return rc;
-        r.scale = 1.0f / stored_scale(p);
+        if (int rc = product_params(p, o.dtype, &r)) return rc;
+        r.scale = 1.0f / stored_scale(o);
         r.tasks = 0;
         const int pg = cta_group(p.n > p.d ? p.n : p.d);
         const int64_t M = p.class_major ? cols : p.d, N = p.class_major ? p.d : cols, ldo = p.class_major ? p.d : p.V;
@@ -710,14 +724,14 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
                     t->out = dw_out;
                     t->ldo = ldo;
                 } else {
-                    rc = sum_dw ? set_sums(t, &maps.c[i], q.dw_parts, dw_sum, q.ld_dw, false) : set_rounded(t, &maps.c[i], p.dtype, dw_out, ldo);
+                    rc = q.sum_dw ? set_sums(t, &maps.c[i], q.dw_parts, dw_sum, q.ld_dw, false) : set_rounded(t, &maps.c[i], p.dtype, dw_out, ldo);
                 }
             } else {
                 rc = set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, G, 0, o.w, p.class_major, p.n, p.d, cols);
                 if (rc != GRWS_OK) return rc;
                 t->b_k0 = (int)v0;
                 t->k_len = (int)q.dx_len;
-                rc = sum_dx ? set_sums(t, &maps.c[i], ceil_div((int64_t)t->k_blocks, q.dx_len), dx_sum, q.ld_dx, v0 > 0)      // (a last, shorter piece: fewer)
+                rc = q.sum_dx ? set_sums(t, &maps.c[i], ceil_div((int64_t)t->k_blocks, q.dx_len), dx_sum, q.ld_dx, v0 > 0)      // (a last, shorter piece: fewer)
                             : set_rounded(t, &maps.c[i], p.dtype, dx, p.d);
             }
             if (rc != GRWS_OK) return rc;
@@ -729,9 +743,9 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
             deal_units(r.task[0].units(), unit_time(r.task[0].k_len * step_cost(q.planes)), r.task[1].units(), unit_time(r.task[1].k_len * step_cost(q.planes)), units < ctas ? units : ctas, &r.deal_less, &r.deal_more);
         }
         if (int rc = launch_product<prod::SUM>(pg, q.planes, maps, r, st)) return rc;
-        if (dw && sum_dw) if (int rc = launch_round<T>(p, dw_sum, q.dw_parts, M, N, q.ld_dw, r.scale, dw_out, ldo, 1, st)) return rc;
+        if (dw && q.sum_dw) if (int rc = launch_round<T>(p, dw_sum, q.dw_parts, M, N, q.ld_dw, r.scale, dw_out, ldo, 1, st)) return rc;
     }
-    return dx && sum_dx ? launch_round<T>(p, dx_sum, q.dx_parts, p.n, p.d, q.ld_dx, 1.0f / stored_scale(p), dx, p.d, 1, st) : GRWS_OK;
+    return dx && q.sum_dx ? launch_round<T>(p, dx_sum, q.dx_parts, p.n, p.d, q.ld_dx, 1.0f / stored_scale(o), dx, p.d, 1, st) : GRWS_OK;
 }
 
 template <typename T> static int forward(const Problem &p, const Plan &q, float *loss, float2 *state, float *count, char *scratch, cudaStream_t st) {
@@ -811,7 +825,13 @@ __attribute__((visibility("default")))
 size_t grws_linear_ce_scratch_bytes(const void *x, int64_t ldx, const void *w, int64_t ldw, int class_major, int64_t rows, int64_t width,
                                     int64_t classes, int dtype, int backward) {
     if (rows <= 0 || width <= 0 || classes <= 0) return 0;
-    return lce::make_plan(lce::problem(x, ldx, w, ldw, class_major, nullptr, 8, 0, rows, width, classes, dtype, 0), backward != 0).bytes;
+    const auto bytes = [&](int reduction) {
+        return lce::make_plan(lce::problem(x, ldx, w, ldw, class_major, nullptr, 8, 0, rows, width, classes, dtype, reduction), backward != 0).bytes;
+    };
+    const size_t reduced = bytes(cls::RED_MEAN);
+    if (backward != 1 || dtype != GRWS_F16) return reduced;
+    const size_t rowwise = bytes(cls::RED_NONE);
+    return rowwise > reduced ? rowwise : reduced;
 }
 
 __attribute__((visibility("default")))

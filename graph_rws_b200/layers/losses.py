@@ -107,7 +107,7 @@ class _LinearCrossEntropyFunction(Function):
 
         def call():
             operands, key = _ce_operands(x, w, class_major, V)
-            scratch = _scratch(_ce_scratch_bytes(*key, 1), x.device)
+            scratch = _scratch(_ce_scratch_bytes(*key, 1 if reduction == _native.REDUCE_NONE else 2), x.device)
             sp = state.data_ptr()
             return _native.lib().grws_linear_ce_bwd(*operands, labels.data_ptr(), _INDEX_BYTES[labels.dtype], ignore_index, n, d, V, _DT[x.dtype],
                                                     reduction, grad_loss.data_ptr(), sp, sp + 8 * n, _ptr(dx), _ptr(dw), scratch.data_ptr(),

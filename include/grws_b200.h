@@ -276,7 +276,8 @@ int grws_layer_norm_bwd(const void *x, const void *gamma, const void *dy, const 
  *          from the forward to the backward call, 16-byte aligned state;
  *   grad_loss  gradient of `loss`, of its size;
  *   dx [rows, width] and dw (in w's order) contiguous, of `dtype`; either may be null.
- * The scratch of a call depends on where its operands lie (x, w: looked at, not read).
+ * The scratch of a call depends on where its operands lie (x, w: looked at, not read).  `backward`: 0 forward, 1 backward of any
+ * reduction, 2 backward of a mean or a sum (in fp16 rows' losses take more: their gradients may be decades apart).
  * ------------------------------------------------------------------------------------------ */
 typedef enum { GRWS_REDUCE_NONE = 0, GRWS_REDUCE_MEAN = 1, GRWS_REDUCE_SUM = 2 } grws_reduction;
 
