@@ -329,6 +329,9 @@ template <typename T, int L, int U, int EDGE, int H> __global__ void __launch_bo
 }
 
 // ---- longer rows: a CTA per row, or per part of a row where there are few rows ----
+// end of the part that starts at lo (lo + part may pass 31 bits)
+__device__ __forceinline__ int part_end(const Args &a, int lo) { return a.V - lo > a.part ? lo + a.part : a.V; }
+
 template <typename T> __global__ void __launch_bounds__(THREADS) long_fwd_kernel(const Args a) {
     wait_for_previous();
     let_next_start();
@@ -339,7 +342,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) long_fwd_kernel
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int row = (int)(item / a.splits);
         const int split = (int)(item - (int64_t)row * a.splits);
-        const int lo = split * a.part, hi = min(a.V, lo + a.part);
+        const int lo = split * a.part, hi = part_end(a, lo);
         float m = NEG_INF, s = 0.0f;
         const T *z = static_cast<const T *>(a.z) + (int64_t)row * a.ldz;
         Entry held[LONG_HELD];
@@ -415,7 +418,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) long_bwd_kernel
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int row = (int)(item / a.splits);
         const int lo = (int)(item - (int64_t)row * a.splits) * a.part;
-        row_grad<T, THREADS, 4, 1, 1>(a, row, lo, min(a.V, lo + a.part), threadIdx.x, true, s_ids, s_p, [] { __syncthreads(); });
+        row_grad<T, THREADS, 4, 1, 1>(a, row, lo, part_end(a, lo), threadIdx.x, true, s_ids, s_p, [] { __syncthreads(); });
     }
 }
 
