@@ -60,11 +60,19 @@ def check_device_status(device=None):
     """Synchronises the current stream of ``device`` and raises RuntimeError (status -5) if any
     tcgen05 SpMM or linear cross entropy launch on that device gave up on a pipeline wait since the last check: its output
     is then incomplete.  The kernels' waits are bounded, so a broken pipeline ends with this status
-    instead of hanging the GPU.  Call it where the host synchronises anyway (end of an epoch)."""
+    instead of hanging the GPU.  Every word is read and cleared before anything is raised, so that the next check
+    tells of later launches only.  Call it where the host synchronises anyway (end of an epoch)."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with torch.cuda.device(device):
-        _native.check(_native.lib().grws_spmm_check(_stream(device)))
-        _native.check(_native.lib().grws_linear_ce_check(_stream(device)))
+        lib = _native.lib()
+        errors = []
+        for check in (lib.grws_spmm_check, lib.grws_linear_ce_check):
+            try:
+                _native.check(check(_stream(device)))
+            except RuntimeError as e:
+                errors.append(str(e))
+    if errors:
+        raise RuntimeError("; ".join(errors))
 
 
 def _scratch(nbytes: int, device):
