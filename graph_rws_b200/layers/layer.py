@@ -35,17 +35,21 @@ def _spmm_graph(graph, dense):
     return out[:, :n] if pad else out
 
 
+def _spmm_recorded(graph, dense, warps_per_block=8):
+    """A @ dense of a forward pass, its time recorded (0.0 unless timing is on)."""
+    if core._timing_enabled and not hasattr(graph, 'gather_dense'):
+        output, timing = core.spmm_tc(graph.window_offset, graph.original_col_indices, graph.values_as(dense.dtype),
+                                      dense.contiguous(), warps_per_block)
+    else:
+        output, timing = _spmm_graph(graph, dense), 0.0
+    record_spmm_time(timing)
+    return output
+
+
 class BCSRSPMMFunction(Function):
     @staticmethod
     def forward(ctx, graph, features, weight, warps_per_block):
-        x_mult_w = torch.matmul(features, weight)
-        if core._timing_enabled and not hasattr(graph, 'gather_dense'):
-            output, timing = core.spmm_tc(graph.window_offset, graph.original_col_indices,
-                                          graph.values_as(x_mult_w.dtype), x_mult_w.contiguous(),
-                                          warps_per_block)
-        else:
-            output, timing = _spmm_graph(graph, x_mult_w), 0.0
-        record_spmm_time(timing)
+        output = _spmm_recorded(graph, torch.matmul(features, weight), warps_per_block)
         ctx.save_for_backward(features, weight)
         ctx.graph = graph
         ctx.warps_per_block = warps_per_block
@@ -96,8 +100,7 @@ class BCSRAggregateFunction(Function):
     @staticmethod
     def forward(ctx, graph, features):
         ctx.graph, ctx.rows = graph, features.shape[0]
-        record_spmm_time(0.0)
-        return _spmm_graph(graph, features)
+        return _spmm_recorded(graph, features)
 
     @staticmethod
     def backward(ctx, grad_output):
