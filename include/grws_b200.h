@@ -294,8 +294,9 @@ int grws_linear_ce_bwd(const void *x, int64_t ldx, const void *w, int64_t ldw, i
                        size_t scratch_bytes, void *stream);
 
 /* Every wait of the tensor-core kernel is bounded; a launch whose wait ran out leaves its output incomplete and its code in a
- * word of the device.  Synchronises `stream`, reads and clears the word: GRWS_ERR_DEVICE if a launch gave up.  (The first
- * call on a device looks up the word's address and allows the kernels their shared memory: make it before any capture.) */
+ * word of the device.  Synchronises `stream`, which must not be capturing, reads and clears the word: GRWS_ERR_DEVICE if a
+ * launch gave up.  It need not be called ahead of a capture: the forward and backward calls set up what they need at their
+ * first use, which may be a captured one. */
 int grws_linear_ce_check(void *stream);
 
 /* Distillation from a teacher's best scores: T^2 KL(p || softmax(logits / T)), p the softmax over a row's
