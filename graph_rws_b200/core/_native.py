@@ -38,6 +38,7 @@ SIGNATURES = {
     "grws_linear_ce_bwd": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32,
                                    c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
     "grws_linear_ce_check": (c_i32, [c_vp]),
+    "grws_linear_ce_set_wait_limit": (c_i32, [ctypes.c_longlong]),
     "grws_distill_scratch_bytes": (c_sz, [c_i64, c_i64]),
     "grws_distill_fwd": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_i64, c_i32, c_vp, c_i64, c_i32, c_i64, c_i64, c_i64,
                                  ctypes.c_float, c_i32, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),

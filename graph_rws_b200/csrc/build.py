@@ -50,16 +50,20 @@ SELFTEST_LIB = os.path.join(HERE, "libgrws_b200_selftest.so")
 
 
 def build_selftest(force: bool = False) -> str:
-    """The same library with the SpMM kernel's profiling build compiled in (-DGRWS_TC5_PROFILING):
-    per-role wait counters, and the switch the time-out self-test uses to withhold one barrier
-    arrive.  Only spmm_tcgen05.cu is compiled again; the other objects are the product's."""
+    """The same library with the tcgen05 kernels' self-test build compiled in (-DGRWS_TC5_PROFILING):
+    the SpMM's per-role wait counters, and the switches the time-out self-tests use to withhold a
+    barrier arrive or a stage's copies.  The other objects are the product's."""
     build()
-    src = os.path.join(HERE, "spmm_tcgen05.cu")
+    again = [os.path.join(HERE, "spmm_tcgen05.cu"), os.path.join(HERE, "linear_ce.cu")]
     if not force and os.path.exists(SELFTEST_LIB) and os.path.getmtime(SELFTEST_LIB) >= os.path.getmtime(LIB):
         return SELFTEST_LIB
-    obj = os.path.join(HERE, "build", "spmm_tcgen05.selftest.o")
-    subprocess.check_call([NVCC] + FLAGS + ["-DGRWS_TC5_PROFILING", "-c", src, "-o", obj])
-    objs = [os.path.join(HERE, "build", os.path.basename(s) + ".o") for s in sources() if s != src] + [obj]
+    objs = [os.path.join(HERE, "build", os.path.basename(s) + ".o") for s in sources() if s not in again]
+    procs = []
+    for src in again:
+        objs.append(os.path.join(HERE, "build", os.path.basename(src)[:-3] + ".selftest.o"))
+        procs.append(subprocess.Popen([NVCC] + FLAGS + ["-DGRWS_TC5_PROFILING", "-c", src, "-o", objs[-1]]))
+    if any([p.wait() for p in procs]):
+        raise RuntimeError("nvcc failed")
     subprocess.check_call([NVCC, "-shared", "-o", SELFTEST_LIB] + objs + ["-lcudart", "-ccbin", "/usr/bin/g++"])
     return SELFTEST_LIB
 

@@ -91,6 +91,9 @@ struct Params {
     float scale;                          // GRAD: power of two that keeps G within its type; SUM: its inverse
     int *status;
     long long wait_limit;
+#ifdef GRWS_TC5_PROFILING
+    int withhold;                         // self-test: stages that the first CTA fills before it stops filling (0: all)
+#endif
 };
 
 struct alignas(64) Maps { CUtensorMap a[MAX_TASKS], b[MAX_TASKS], c[MAX_TASKS]; };       // operands, output
@@ -401,6 +404,9 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                     const uint32_t bytes = CG * (C::A_BYTES + pieces * PIECE_BYTES);
                     for (int kb = k0; ok && kb < k1; ++kb) {
                         for (int plane = 0; plane < PLANES; ++plane) {
+#ifdef GRWS_TC5_PROFILING
+                            if (p.withhold > 0 && blockIdx.x == 0 && issued == p.withhold) { ok = false; break; }
+#endif
                             if (!mbar_wait(smem_u32(&ss->empty[stage]), phase ^ 1u, abort_flag, limit)) { give_up(ss, p, WAIT_STAGE); ok = false; break; }
                             const uint32_t bar = full0 + stage * 8, a = ring + stage * C::STAGE_BYTES, b = a + C::A_BYTES;
                             const int ka = kb * BK, kB = b_k0 + ka;

@@ -8,6 +8,8 @@
 //
 // r_i comes in two factors: alpha, one number for all rows, applied where dx and dw are rounded to their type, and a row's own
 // factor in G, which is 1 (or 0 for an ignored row) where the loss is a mean or a sum.
+#include <stdlib.h>
+
 #include "class_product.cuh"
 
 namespace grws {
@@ -336,6 +338,7 @@ template <typename T, int PLANES> __global__ void __launch_bounds__(256) pack_ke
 
 // Worst status of a tensor-core launch on this device since it was last read
 static __device__ int g_status;
+static long long g_wait_limit = prod::WAIT_LIMIT_CYCLES;
 
 // ---------------------------------------------------------------------------------------------
 // plan: how a call is cut up, and where its workspace lies
@@ -649,7 +652,11 @@ static int product_params(const Problem &p, int dtype, prod::Params *r) {
     r->state = p.state;
     r->scale = 1.0f;
     r->status = status;
-    r->wait_limit = prod::WAIT_LIMIT_CYCLES;
+    r->wait_limit = __atomic_load_n(&g_wait_limit, __ATOMIC_RELAXED);
+#ifdef GRWS_TC5_PROFILING
+    const char *withhold = getenv("GRWS_CE_WITHHOLD");
+    r->withhold = withhold ? atoi(withhold) : 0;
+#endif
     return GRWS_OK;
 }
 
@@ -905,6 +912,13 @@ int grws_linear_ce_check(void *stream) {
                                        "a tile was never finished"};
     return fail(GRWS_ERR_DEVICE, "a linear cross entropy launch on this device gave up waiting: %s (code %d); its output is incomplete",
                 status >= 1 && status <= 4 ? what[status] : "unknown wait", status);
+}
+
+__attribute__((visibility("default")))
+int grws_linear_ce_set_wait_limit(long long sm_clocks) {
+    GRWS_REQUIRE(sm_clocks >= 0, "negative limit");
+    __atomic_store_n(&lce::g_wait_limit, sm_clocks > 0 ? sm_clocks : prod::WAIT_LIMIT_CYCLES, __ATOMIC_RELAXED);
+    return GRWS_OK;
 }
 
 }  // extern "C"

@@ -298,6 +298,8 @@ int grws_linear_ce_bwd(const void *x, int64_t ldx, const void *w, int64_t ldw, i
  * launch gave up.  It need not be called ahead of a capture: the forward and backward calls set up what they need at their
  * first use, which may be a captured one. */
 int grws_linear_ce_check(void *stream);
+/* The limit of one wait in SM clocks for launches made after the call (0: the default, about 1.5 to 2.5 s). */
+int grws_linear_ce_set_wait_limit(long long sm_clocks);
 
 /* Distillation from a teacher's best scores: T^2 KL(p || softmax(logits / T)), p the softmax over a row's
  * kept teacher scores at temperature T.
