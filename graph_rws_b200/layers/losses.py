@@ -118,7 +118,7 @@ class _LinearCrossEntropyFunction(Function):
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
                          reduction: str = 'mean') -> torch.Tensor:
-    """Softmax cross entropy of the scores ``x @ weight`` against ``labels``, in fp32, without keeping the scores.
+    """Softmax cross entropy of the scores ``x @ weight`` against ``labels``, without keeping the scores.
 
     x [rows, width] and weight [width, classes] (the layout of the layers' weights; the transpose of a
     [classes, width] matrix is as good) are fp32, fp16 or bf16 CUDA matrices of one type, labels [rows] int32 or
@@ -126,7 +126,17 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     and the gradients NaN.  'mean' divides by the number of counted rows (none: NaN, and no gradient),
     'none' returns a loss per row.  The backward pass computes the scores again, a piece of the classes
     at a time, and returns gradients of the operands' type; there is no second derivative.  Results do
-    not change from call to call."""
+    not change from call to call.
+
+    Scores, softmax statistics, losses and all sums are fp32.  Of 16-bit operands the scores' gradient G is
+    rounded to their type before the products with it, as a 16-bit layer's would be (fp16 without a
+    reduction, where rows' gradients may be decades apart, keeps it to 24 bits and takes some four times as
+    long).  Classes may be masked in the weight with the type's lowest value.  The gradient of the weight is
+    ``x.T @ G``: an ignored row's part of it is 0 only if its ``x`` is finite.  The workspace of
+    the backward pass holds G for as many classes as fit 512 MiB (256 at least, so more from a million
+    rows on, in fp32 from 350,000) and fp32 sums of the gradients where they come in parts.  That of
+    either pass holds copies of operands that the tensor cores do not read as they lie: unaligned
+    rows, and fp32 as three bf16 planes (1.5 times its size)."""
     red = _reduction(reduction)
     _matrix(x, "x")
     _matrix(weight, "weight")
@@ -199,10 +209,13 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
 
     logits [rows, classes] and teacher_logits [rows, kept] are fp32, fp16 or bf16 CUDA matrices, each of its own
     type, teacher_ids [rows, kept] the classes of the kept scores (int32 or int64, at most 1,024 a row).  An id
-    below 0 is a missing entry, as padded column ids are; a row without entries counts nothing.  A class
+    below 0 is a missing entry, as padded column ids are, and a score of -inf has no weight; a row without
+    entries of any weight counts nothing.  A class
     that occurs twice in a row counts with both scores; an id past the classes makes the row's loss
     and gradient NaN.  'mean' divides by the number of rows with entries (none: NaN, and no gradient), 'none'
-    returns a loss per row.  Only ``logits`` has a gradient, and no second one."""
+    returns a loss per row.  Only ``logits`` has a gradient, and no second one.  A row's loss is the
+    difference of two fp32 logarithms times T^2, off by some 2^-21 T^2: T in the hundreds leaves few digits of
+    a loss of order 1."""
     red = _reduction(reduction)
     _matrix(logits, "logits")
     _matrix(teacher_logits, "teacher_logits")

@@ -183,7 +183,9 @@ class GCN_BCSR(nn.Module):
         """Cross entropy of the scores that ``forward`` returns, of the rows ``rows`` (an index or a slice; all by
         default) against their ``labels``, without computing the scores as a matrix: the last layer aggregates its
         input at the hidden width, and ``linear_cross_entropy`` goes over the classes piece by piece.  For
-        many classes: forward multiplies the graph at class width and keeps rows x classes for backward."""
+        many classes: forward multiplies the graph at class width and keeps rows x classes for backward.
+        The last layer is not called as a module, so forward hooks on it do not run, and it is not
+        checkpointed: there is nothing of class width to recompute."""
         if features.device.type != 'cuda':
             features = features.to('cuda', non_blocking=True)
         graph_list = self._ensure_graph_list(graphs)

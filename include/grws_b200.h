@@ -276,8 +276,14 @@ int grws_layer_norm_bwd(const void *x, const void *gamma, const void *dy, const 
  *          from the forward to the backward call, 16-byte aligned state;
  *   grad_loss  gradient of `loss`, of its size;
  *   dx [rows, width] and dw (in w's order) contiguous, of `dtype`; either may be null.
+ * Scores, statistics and sums are fp32; of 16-bit operands the scores' gradient is rounded to `dtype` before the products
+ * with it.  dw is x^T times that gradient: x of an ignored row has to be finite for its part to be 0.
  * The scratch of a call depends on where its operands lie (x, w: looked at, not read).  `backward`: 0 forward, 1 backward of any
- * reduction, 2 backward of a mean or a sum (in fp16 rows' losses take more: their gradients may be decades apart).
+ * reduction, 2 backward of a mean or a sum (in fp16 rows' losses take more: their gradients may be decades apart).  Backward
+ * it holds the scores' gradient for as many classes as fit 512 MiB, 256 at least (rows * 512 bytes in 16 bits, rows * 1536 in
+ * fp32), fp32 sums of dx and dw where they come in parts, and, forward too, copies of operands that the tensor cores cannot read
+ * as they lie: rows off 16-byte boundaries (x's off 128-byte lines too from 16,384 classes on), and fp32, which takes 6 bytes per
+ * element of x and w.
  * ------------------------------------------------------------------------------------------ */
 typedef enum { GRWS_REDUCE_NONE = 0, GRWS_REDUCE_MEAN = 1, GRWS_REDUCE_SUM = 2 } grws_reduction;
 
