@@ -35,16 +35,22 @@ namespace prod {
 using namespace cls;
 
 constexpr int BM = 128, BK = 64;                    // rows per CTA, inner elements per stage
-constexpr int tile_width(int planes) { return planes == 3 ? 128 : 256; }            // columns per tile at most
+// How a product's sums are held.  WHOLE: the inner axis in one accumulator.  PLANES3: operands of three planes, as above.  CHAINS:
+// 16-bit scores of wide rows, whose sum is taken off the tensor cores every CHAIN_STEPS steps; 128-column tiles for the
+// same reason, two accumulators that take the chains in turn.
+enum Kind : int { WHOLE = 0, PLANES3 = 1, CHAINS = 2 };
+constexpr int tile_width(int kind) { return kind == WHOLE ? 256 : 128; }            // columns per tile at most
 constexpr int MAX_STAGES = 8, SMEM_BYTES = 231936;        // 227 KB less what the barriers take
 constexpr int EPILOGUE_WARPS = 8, TMA_WARP = 8, MMA_WARP = 9, THREADS = 320;
 constexpr long long WAIT_LIMIT_CYCLES = 3000000000ll;   // about 1.5 to 2.5 s of SM clocks
 constexpr int MAX_TASKS = 2;
 constexpr int PIECE_BYTES = 64 * BK * 2;                // 64 of the outer axis of an operand: what one copy brings of B
-constexpr int SUB_STEPS = 2;                            // fp32: steps of 64 inner elements whose hi hi is summed in tensor memory
+constexpr int SUB_STEPS = 2;                            // PLANES3: steps of 64 inner elements whose hi hi is summed in tensor memory
+constexpr int CHAIN_STEPS = 4;                          // CHAINS: steps of 64 inner elements in a chain
 
-template <int CG, bool SPLIT> struct Cfg {
-    static constexpr int BN = tile_width(SPLIT ? 3 : 1);
+template <int CG, int KIND> struct Cfg {
+    static constexpr bool SPLIT = KIND == PLANES3;
+    static constexpr int BN = tile_width(KIND);
     static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN / CG * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
     // what a warp stores at once: 32 rows of 64 16-bit or 32 fp32 numbers, or of three planes of 32
     static constexpr int BOX_BYTES = SPLIT ? 3 * 32 * 64 : 32 * 128;
@@ -341,8 +347,9 @@ __device__ __forceinline__ void split3(float v, float &a, float &b, float &c) {
     c = r - b;
 }
 
-template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
-    using C = Cfg<CG, SPLIT>;
+template <int CG, int MODE, int KIND> __global__ void __launch_bounds__(THREADS, 1) product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+    using C = Cfg<CG, KIND>;
+    constexpr bool SPLIT = C::SPLIT;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Shared shared;
     Shared *ss = &shared;
@@ -475,9 +482,16 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
 #pragma unroll
                         for (int k = 0; k < BK / 16; ++k) umma<CG>(to, ad + k * a_step, bd + k * b_step, idesc, add || k > 0);
                     };
-                    ok = wait_empty(ss->acc_empty, tile);
+                    if constexpr (KIND != CHAINS) ok = wait_empty(ss->acc_empty, tile);
                     for (int k = 0; ok && k < steps; ++k) {
-                        if constexpr (!SPLIT) {
+                        if constexpr (KIND == CHAINS) {
+                            if (k % CHAIN_STEPS == 0 && !(ok = wait_empty(ss->big_empty, chain))) break;
+                            if (!(ok = wait_stage(stage, phase))) break;
+                            multiply(tmem + (chain & 1u) * C::BN, stage, stage, k % CHAIN_STEPS != 0);
+                            umma_commit<CG>(smem_u32(&ss->empty[stage]));
+                            advance();
+                            if (k % CHAIN_STEPS == CHAIN_STEPS - 1 || k == steps - 1) { umma_commit<CG>(smem_u32(&ss->big_full[chain & 1u])); ++chain; }
+                        } else if constexpr (!SPLIT) {
                             if (!(ok = wait_stage(stage, phase))) break;
                             multiply(d, stage, stage, k > 0);
                             umma_commit<CG>(smem_u32(&ss->empty[stage]));
@@ -506,7 +520,9 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                             if (k % SUB_STEPS == SUB_STEPS - 1 || k == steps - 1) { umma_commit<CG>(smem_u32(&ss->big_full[chain & 1u])); ++chain; }
                         }
                     }
-                    if (ok) umma_commit<CG>(smem_u32(&ss->acc_full[tile & 1u]));
+                    if constexpr (KIND != CHAINS) {
+                        if (ok) umma_commit<CG>(smem_u32(&ss->acc_full[tile & 1u]));
+                    }
                 }
             }
         }
@@ -709,8 +725,31 @@ template <int CG, int MODE, bool SPLIT> __global__ void __launch_bounds__(THREAD
                         }
                     }
                 };
-                const uint32_t at = tmem + (tile & 1u) * C::BN + lanes;
-                if constexpr (!SPLIT) {
+                [[maybe_unused]] const uint32_t at = tmem + (tile & 1u) * C::BN + lanes;
+                if constexpr (KIND == CHAINS) {
+                    const int chains = (t.k_blocks + CHAIN_STEPS - 1) / CHAIN_STEPS, c = half * 64;
+                    float acc[64];
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
+                    for (int sub = 0; sub < chains; ++sub, ++chain) {
+                        wait_sum(ss->big_full, chain);
+                        if (!ok) break;
+                        if (c < cols) {
+                            uint32_t r[32], r2[32];
+                            const uint32_t from = tmem + (chain & 1u) * C::BN + lanes + c;
+                            tmem_ld32(from, r);
+                            tmem_ld32(from + 32, r2);
+                            tmem_ld_wait();
+                            loaded(r);
+                            loaded(r2);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) { acc[i] += __uint_as_float(r[i]); acc[32 + i] += __uint_as_float(r2[i]); }
+                        }
+                        release_sum(ss->big_empty, chain);
+                    }
+                    if (!ok) break;
+                    if (c < cols) use(acc, c);
+                } else if constexpr (!SPLIT) {
                     wait_sum(ss->acc_full, tile);
                     if (!ok) break;
                     const int last = (cols - 1 - half * 64) >> 7;          // 64-column pieces of this warp, less one (-1: none)
@@ -813,19 +852,19 @@ inline int encode_map(CUtensorMap *map, const void *base, int dtype, int64_t col
     return GRWS_OK;
 }
 
-template <int CG, int MODE, bool SPLIT> static int launch_product(const Maps &maps, const Params &p, cudaStream_t st) {
+template <int CG, int MODE, int KIND> static int launch_product(const Maps &maps, const Params &p, cudaStream_t st) {
     int64_t units = 0;
     for (int i = 0; i < p.tasks; ++i) units += p.task[i].units();
     const int64_t clusters = units < sm_count() / CG ? units : sm_count() / CG;
-    using C = Cfg<CG, SPLIT>;
+    using C = Cfg<CG, KIND>;
     static bool allowed[MAX_DEVICES];
     const int dev = current_device();
     if (dev < 0) return fail(GRWS_ERR_CUDA, "no current device");
     if (!__atomic_load_n(&allowed[dev], __ATOMIC_RELAXED)) {
-        GRWS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<CG, MODE, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        GRWS_CUDA_TRY(cudaFuncSetAttribute(product_kernel<CG, MODE, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         __atomic_store_n(&allowed[dev], true, __ATOMIC_RELAXED);
     }
-    return launch_next(product_kernel<CG, MODE, SPLIT>, dim3((unsigned)(clusters * CG)), THREADS, C::SMEM, st, CG, maps, p);
+    return launch_next(product_kernel<CG, MODE, KIND>, dim3((unsigned)(clusters * CG)), THREADS, C::SMEM, st, CG, maps, p);
 }
 
 }  // namespace prod

@@ -353,6 +353,7 @@ constexpr int64_t LINE = 64;
 struct Plan {
     bool tensor;
     int planes;                                    // of an operand: 1, or 3 of bf16 (see planes_of)
+    int kind, score_kind;                          // how sums are held (prod::Kind), those of the scores
     bool pack_x, pack_w;
     int64_t ldx, ldw, ldg, ld_dx, ld_dw;           // rows of the operands as the tensor cores read them, of fp32 sums
     int64_t run, parts;                            // forward: class tiles per unit, parts of the class axis
@@ -386,17 +387,29 @@ static void cut(int64_t tiles, int64_t K, int64_t least, int64_t unit, int64_t *
 }
 
 static int64_t in_32s(int64_t N) { return ceil_div(N, (int64_t)32) * 32; }
-static int64_t column_tiles(int64_t N, int planes) { return ceil_div(N, (int64_t)prod::tile_width(planes)); }
-static int columns_per_tile(int64_t N, int planes) {
-    const int64_t tiles = column_tiles(N, planes);
+static int64_t column_tiles(int64_t N, int kind) { return ceil_div(N, (int64_t)prod::tile_width(kind)); }
+static int columns_per_tile(int64_t N, int kind) {
+    const int64_t tiles = column_tiles(N, kind);
     return (int)(tiles == 1 ? in_32s(N) : ceil_div(ceil_div(N, tiles), (int64_t)64) * 64);
 }
-static int64_t tiles_of(int64_t M, int64_t N, int cg, int planes) { return ceil_div(M, (int64_t)(prod::BM * cg)) * column_tiles(N, planes); }
+static int64_t tiles_of(int64_t M, int64_t N, int cg, int kind) { return ceil_div(M, (int64_t)(prod::BM * cg)) * column_tiles(N, kind); }
 // What 64 inner elements of a tile take, in steps of a 256 x 256 tile (some 0.4 us of a pair of SMs): fp32 has six products of half the width
-static int64_t step_cost(int planes) { return planes == 3 ? 3 : 1; }
+static int64_t step_cost(int kind) { return kind == prod::PLANES3 ? 3 : 1; }
 
 // CTAs that share a tile: pairs where there are more rows than one CTA's
 static int cta_group(int64_t M) { return M > prod::BM ? 2 : 1; }
+
+// Whether scores of 16-bit operands are summed in chains of 256 elements, which the epilogue adds up to nearest.  The tensor cores cut
+// off every 16 products' sum towards zero: one sum over the width is off by some 1.5 * 2^-24 of itself per 16 elements where all have one
+// sign (65,536 elements: a score of 18 came out 0.007 too small), and losses by 5e-7 (many classes) to 1.2e-6 (two) at a width of 1,024,
+// 4.6e-6 at 4,096, where a chain leaves 1e-7 to 3e-7 at any width.  Tiles of half the columns are what it costs (forward,
+// bf16, us, one sum and chains: 90,941 x 1,440 x 172 75 and 102, 2,000 x 1,440 x 30,000 166 and 208, 8,192 x 4,096 x 32,000 1,500 and
+// 2,015), and nothing where the classes fit one (90,941 x 1,024 x 47 46 and 46, 20,000 x 768 x 100 18.6 and 20.6).  G is rounded to 16 bits, so its
+// scores may be off by more, but not by more than that rounding: 2.4e-5 of a score at 4,096.
+static bool in_chains(int64_t d, int64_t V, bool backward) {
+    if (backward) return d > 4096;
+    return d > (V <= prod::tile_width(prod::CHAINS) ? 768 : 1024);
+}
 
 static bool needs_packing(const void *p, int64_t ld, int planes) { return planes == 3 || !aligned16(p) || ld % 8 != 0; }
 
@@ -477,9 +490,9 @@ static bool on_tensor_cores(int64_t n, int64_t d, int64_t V, int dtype) {
 // (forward and backward, bf16: 5,003 x 301 x 49,999 in 580 us against 619, 30,000 x 100 x 49,999 in 2,358 against 2,609, 8,192 x
 // 320 x 10,000 in 258 against 269; fp32: 8,192 x 96 x 49,999 in 2,284 against 2,745; a fifth less, bf16, 30,000 x 600 x 49,999:
 // 6,931 against 6,840).
-static bool turns(const Problem &p, int cg, int planes) {
+static bool turns(const Problem &p, int cg, int kind) {
     if (p.class_major) return false;
-    const int64_t before = (column_tiles(p.d, planes) - 1) * columns_per_tile(p.d, planes), rows = (int64_t)prod::BM * cg;
+    const int64_t before = (column_tiles(p.d, kind) - 1) * columns_per_tile(p.d, kind), rows = (int64_t)prod::BM * cg;
     return 3 * ceil_div(p.d, rows) * rows >= 4 * (before + in_32s(p.d - before));
 }
 
@@ -511,6 +524,8 @@ static Plan make_plan(const Problem &p, bool backward) {
         return q;
     }
     q.planes = planes_of(p, backward);
+    q.kind = q.planes == 3 ? prod::PLANES3 : prod::WHOLE;
+    q.score_kind = q.planes == 1 && in_chains(d, V, backward) ? prod::CHAINS : q.kind;
     const int64_t w_rows = p.class_major ? V : d, w_cols = p.class_major ? d : V;
     // x whose rows are no whole lines is packed for many classes, which read it as often (bf16, 8,192 x 1,000 x 50,000: 2,663 us
     // as it is, 2,430 packed; x 10,000: 479 and 462; 8,192 x 304 x 10,000: 210 and 211; x 1,000: 54 and 58); a copy of w, as
@@ -523,8 +538,8 @@ static Plan make_plan(const Problem &p, bool backward) {
     if (q.pack_w) q.w = place(at, (size_t)q.planes * w_rows * q.ldw * 2);
     const int cg = cta_group(n);
     if (!backward) {
-        const int64_t bn = columns_per_tile(V, q.planes);
-        cut_runs(n, ceil_div(n, (int64_t)(prod::BM * cg)), ceil_div(V, bn), ceil_div(d, (int64_t)prod::BK) * step_cost(q.planes), sm_count() / cg, true, &q.run, &q.parts);
+        const int64_t bn = columns_per_tile(V, q.score_kind);
+        cut_runs(n, ceil_div(n, (int64_t)(prod::BM * cg)), ceil_div(V, bn), ceil_div(d, (int64_t)prod::BK) * step_cost(q.score_kind), sm_count() / cg, true, &q.run, &q.parts);
         q.stats = place(at, (size_t)q.parts * 2 * n * sizeof(float2));
         place_rows(at, n, &q);
     } else {
@@ -536,14 +551,14 @@ static Plan make_plan(const Problem &p, bool backward) {
         // equally busy
         const int64_t all = ceil_div(V, PIECE_UNIT) * PIECE_UNIT, top = most < all ? most : all;
         const bool summed = q.planes == 3 && p.dtype != GRWS_F32;          // (the kernel rounds to the type of its operands or to fp32)
-        for (q.turn_dw = !summed && turns(p, pg, q.planes);; q.turn_dw = false) {
+        for (q.turn_dw = !summed && turns(p, pg, q.kind);; q.turn_dw = false) {
             double best = 1e300;
             for (int64_t k = 8; k >= (all <= most ? 8 : 4); --k) {
                 const int64_t piece = ceil_div(top * k / 8, PIECE_UNIT) * PIECE_UNIT;
                 const int64_t c = piece < V ? piece : V;
-                const int64_t tiles0 = tiles_of(n, d, pg, q.planes), tiles1 = p.class_major || q.turn_dw ? tiles_of(c, d, pg, q.planes) : tiles_of(d, c, pg, q.planes);
+                const int64_t tiles0 = tiles_of(n, d, pg, q.kind), tiles1 = p.class_major || q.turn_dw ? tiles_of(c, d, pg, q.kind) : tiles_of(d, c, pg, q.kind);
                 int64_t a, b;
-                const double cost = (cut_products(tiles0, ceil_div(c, (int64_t)prod::BK), (double)n * d, tiles1, k1, (double)d * c, step_cost(q.planes), sm_count() / pg, &a, &b) +
+                const double cost = (cut_products(tiles0, ceil_div(c, (int64_t)prod::BK), (double)n * d, tiles1, k1, (double)d * c, step_cost(q.kind), sm_count() / pg, &a, &b) +
                                      (c < V ? (double)n * d * 8.0 / 5.0e6 / 0.4 : 0.0)) * (double)ceil_div(V, c);
                 if (cost < best) { best = cost; q.piece = c; q.dx_parts = a; q.dw_parts = b; }
             }
@@ -597,10 +612,10 @@ template <typename T> static int pack_operands(const Problem &p, const Plan &q, 
 }
 
 // sets a product up: its tile counts and the maps of its operands; `outer`: the operand's rows are the inner axis
-static int set_task(prod::Task *t, CUtensorMap *ma, CUtensorMap *mb, int cg, int dtype, const View &a, int a_outer, const View &b, int b_outer, int64_t M,
+static int set_task(prod::Task *t, CUtensorMap *ma, CUtensorMap *mb, int cg, int kind, int dtype, const View &a, int a_outer, const View &b, int b_outer, int64_t M,
                     int64_t N, int64_t K) {
     t->M = M; t->N = N;
-    t->bn = columns_per_tile(N, a.planes);
+    t->bn = columns_per_tile(N, kind);
     t->m_tiles = (int)ceil_div(M, (int64_t)(prod::BM * cg));
     t->n_tiles = (int)ceil_div(N, (int64_t)t->bn);
     t->run = 1; t->runs = t->n_tiles; t->splits = 1;
@@ -608,7 +623,7 @@ static int set_task(prod::Task *t, CUtensorMap *ma, CUtensorMap *mb, int cg, int
     t->group = t->m_tiles < 16 ? t->m_tiles : 16;
     t->a_outer = a_outer; t->b_outer = b_outer;
     if (int rc = prod::encode_map(ma, a.p, dtype, a.cols, a.rows, a.ld, a.planes, a.plane, 64, a_outer ? prod::BK : prod::BM)) return rc;
-    return prod::encode_map(mb, b.p, dtype, b.cols, b.rows, b.ld, b.planes, b.plane, 64, b_outer ? prod::BK : prod::tile_width(b.planes) / cg);
+    return prod::encode_map(mb, b.p, dtype, b.cols, b.rows, b.ld, b.planes, b.plane, 64, b_outer ? prod::BK : prod::tile_width(kind) / cg);
 }
 
 // where a SUM task's results go: planes of fp32 sums, or the rounded output
@@ -660,9 +675,12 @@ static int product_params(const Problem &p, int dtype, prod::Params *r) {
     return GRWS_OK;
 }
 
-template <int MODE> static int launch_product(int cg, int planes, const prod::Maps &maps, const prod::Params &r, cudaStream_t st) {
-    if (planes == 3) return cg == 2 ? prod::launch_product<2, MODE, true>(maps, r, st) : prod::launch_product<1, MODE, true>(maps, r, st);
-    return cg == 2 ? prod::launch_product<2, MODE, false>(maps, r, st) : prod::launch_product<1, MODE, false>(maps, r, st);
+template <int MODE> static int launch_product(int cg, int kind, const prod::Maps &maps, const prod::Params &r, cudaStream_t st) {
+    if (kind == prod::PLANES3) return cg == 2 ? prod::launch_product<2, MODE, prod::PLANES3>(maps, r, st) : prod::launch_product<1, MODE, prod::PLANES3>(maps, r, st);
+    if constexpr (MODE != prod::SUM) {
+        if (kind == prod::CHAINS) return cg == 2 ? prod::launch_product<2, MODE, prod::CHAINS>(maps, r, st) : prod::launch_product<1, MODE, prod::CHAINS>(maps, r, st);
+    }
+    return cg == 2 ? prod::launch_product<2, MODE, prod::WHOLE>(maps, r, st) : prod::launch_product<1, MODE, prod::WHOLE>(maps, r, st);
 }
 
 template <typename T> static int tensor_forward(const Problem &p, const Plan &q, float2 *part, float *label_score, int *done, char *scratch, cudaStream_t st) {
@@ -672,13 +690,13 @@ template <typename T> static int tensor_forward(const Problem &p, const Plan &q,
     if (int rc = product_params(p, o.dtype, &r)) return rc;
     prod::Maps maps;
     const int cg = cta_group(p.n);
-    if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, o.dtype, o.x, 0, o.w, !p.class_major, p.n, p.V, p.d)) return rc;
+    if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, q.score_kind, o.dtype, o.x, 0, o.w, !p.class_major, p.n, p.V, p.d)) return rc;
     r.task[0].run = (int)q.run;
     r.task[0].runs = (int)q.parts;
     r.part = part;
     r.label_score = label_score;
     r.done = done;
-    return launch_product<prod::STATS>(cg, q.planes, maps, r, st);
+    return launch_product<prod::STATS>(cg, q.score_kind, maps, r, st);
 }
 
 // G in fp16 is held as 2^12 G: |G| <= 1, and a probability of 2^-26 is still a normal number
@@ -695,16 +713,16 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
         if (int rc = product_params(p, o.dtype, &r)) return rc;
         prod::Maps maps;
         const int cg = cta_group(p.n);
-        if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, o.dtype, o.x, 0, o.w, !p.class_major, p.n, cols, p.d)) return rc;
+        if (int rc = set_task(&r.task[0], &maps.a[0], &maps.b[0], cg, q.score_kind, o.dtype, o.x, 0, o.w, !p.class_major, p.n, cols, p.d)) return rc;
         if (int rc = prod::encode_map(&maps.c[0], G.p, o.dtype, cols, p.n, q.ldg, q.planes, G.plane, q.planes == 3 ? 32 : 64, 32)) return rc;
         int64_t run, runs;
-        cut_runs(p.n, r.task[0].m_tiles, r.task[0].n_tiles, r.task[0].k_blocks * step_cost(q.planes), sm_count() / cg, false, &run, &runs);
+        cut_runs(p.n, r.task[0].m_tiles, r.task[0].n_tiles, r.task[0].k_blocks * step_cost(q.score_kind), sm_count() / cg, false, &run, &runs);
         r.task[0].run = (int)run;
         r.task[0].runs = (int)runs;
         r.task[0].b_row0 = (int)v0;
         r.v0 = v0;
         r.scale = stored_scale(o);
-        if (int rc = launch_product<prod::GRAD>(cg, q.planes, maps, r, st)) return rc;
+        if (int rc = launch_product<prod::GRAD>(cg, q.score_kind, maps, r, st)) return rc;
 
         if (int rc = product_params(p, o.dtype, &r)) return rc;
         r.scale = 1.0f / stored_scale(o);
@@ -721,8 +739,8 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
             int rc;
             if (is_dw) {
                 // [d, V]: x^T G, or the transpose of G^T x; [V, d]: G^T x
-                rc = p.class_major || q.turn_dw ? set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, G, 1, o.x, 1, cols, p.d, p.n)
-                                                : set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, o.x, 1, G, 1, M, N, p.n);
+                rc = p.class_major || q.turn_dw ? set_task(t, &maps.a[i], &maps.b[i], pg, q.kind, o.dtype, G, 1, o.x, 1, cols, p.d, p.n)
+                                                : set_task(t, &maps.a[i], &maps.b[i], pg, q.kind, o.dtype, o.x, 1, G, 1, M, N, p.n);
                 if (rc != GRWS_OK) return rc;
                 t->k_len = (int)q.dw_len;
                 if (q.turn_dw) {
@@ -734,7 +752,7 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
                     rc = q.sum_dw ? set_sums(t, &maps.c[i], q.dw_parts, dw_sum, q.ld_dw, false) : set_rounded(t, &maps.c[i], p.dtype, dw_out, ldo);
                 }
             } else {
-                rc = set_task(t, &maps.a[i], &maps.b[i], pg, o.dtype, G, 0, o.w, p.class_major, p.n, p.d, cols);
+                rc = set_task(t, &maps.a[i], &maps.b[i], pg, q.kind, o.dtype, G, 0, o.w, p.class_major, p.n, p.d, cols);
                 if (rc != GRWS_OK) return rc;
                 t->b_k0 = (int)v0;
                 t->k_len = (int)q.dx_len;
@@ -747,9 +765,9 @@ template <typename T> static int tensor_backward(const Problem &p, const Plan &q
         // few units per CTA: dealt out by length (many: in order, so that those at work at a time share operands in L2)
         if (r.tasks > 1 && units <= 12 * ctas) {
             r.deal = 1;
-            deal_units(r.task[0].units(), unit_time(r.task[0].k_len * step_cost(q.planes)), r.task[1].units(), unit_time(r.task[1].k_len * step_cost(q.planes)), units < ctas ? units : ctas, &r.deal_less, &r.deal_more);
+            deal_units(r.task[0].units(), unit_time(r.task[0].k_len * step_cost(q.kind)), r.task[1].units(), unit_time(r.task[1].k_len * step_cost(q.kind)), units < ctas ? units : ctas, &r.deal_less, &r.deal_more);
         }
-        if (int rc = launch_product<prod::SUM>(pg, q.planes, maps, r, st)) return rc;
+        if (int rc = launch_product<prod::SUM>(pg, q.kind, maps, r, st)) return rc;
         if (dw && q.sum_dw) if (int rc = launch_round<T>(p, dw_sum, q.dw_parts, M, N, q.ld_dw, r.scale, dw_out, ldo, 1, st)) return rc;
     }
     return dx && q.sum_dx ? launch_round<T>(p, dx_sum, q.dx_parts, p.n, p.d, q.ld_dx, 1.0f / stored_scale(o), dx, p.d, 1, st) : GRWS_OK;
